@@ -324,6 +324,123 @@ ponni_b200_status ponni_b200_fill_synthetic(ponni_b200_dtype dtype, void* device
                                             int64_t cols, int64_t ld, int64_t col0, uint64_t seed,
                                             int dist, double lo, double hi, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Mixtures of experts: operators that surround and train a set of dense
+ * layers of which each batch column uses top_k.  No counterpart in the
+ * reference, whose models are one chain.
+ *
+ *   route_columns      logits [experts, batch] -> choices, weights, row order
+ *   gather_columns     x [features, batch] -> rows [batch * top_k, features]
+ *   expert_product     rows of expert e times weights[e] (+ bias, activation)
+ *   combine_rows       weighted rows -> y [features, batch]
+ *   gradient_set_clip  norm over many gradient tensors, clipping, packing
+ * and their gradients.
+ *
+ * All pointers are device memory; the calls are asynchronous on `stream` (a
+ * cudaStream_t; NULL is the legacy default stream), allocate nothing (the
+ * creation of a gradient set excepted), may be captured, and restore the
+ * caller's current device.  `dtype` is a ponni_b200_dtype.  A workspace is
+ * caller-owned scratch of at least the bytes that the matching _workspace
+ * function returns, aligned to 256 bytes, in use until the call's kernels
+ * end.  Buffers of one call must not overlap.  The text of the calling thread's
+ * last operator error is ponni_b200_operator_error(). */
+const char* ponni_b200_operator_error(void);
+/* Waits for `stream` and reports what the operators' kernels found on the
+ * device since the last check: PONNI_B200_ERR_DEVICE (a bounded wait gave up),
+ * PONNI_B200_ERR_INVALID_ARGUMENT (group offsets not ascending within the
+ * rows; such calls stay within their buffers, their outputs mean nothing). */
+ponni_b200_status ponni_b200_operator_check(int device, void* stream);
+
+/* How the weights of a column's choices are normalised. */
+#define PONNI_B200_ROUTE_SELECTED 0 /* softmax over the chosen experts' logits */
+#define PONNI_B200_ROUTE_ALL 1      /* the chosen entries of the softmax over all experts */
+
+/* Top-k routing.  logits [num_experts, batch], row stride ld, fp32 / fp16 /
+ * bf16; num_experts <= 1024, top_k <= 8, batch * top_k < 2^31.  Column b
+ * chooses the top_k largest logits, largest first, ties to the lower expert;
+ * -inf and NaN are never chosen and count for nothing, infinite logits share
+ * the weight.  expert, weight, row are [top_k, batch]: the chosen expert, its
+ * weight (fp32) and the row that the choice takes in the order "by expert,
+ * then by column"; -1, 0 and -1 where a column has fewer choices.  column
+ * [batch * top_k]: the column of each row, -1 past the last used row.  offset
+ * [num_experts + 1]: first row of each expert; offset[num_experts] rows are
+ * used. */
+int64_t ponni_b200_route_workspace(int num_experts, int64_t batch);
+ponni_b200_status ponni_b200_route_columns(int dtype, const void* logits, int64_t ld, int num_experts, int top_k,
+                                           int64_t batch, int normalise, int32_t* expert, float* weight, int32_t* row,
+                                           int32_t* column, int32_t* offset, void* workspace, int64_t workspace_bytes,
+                                           int device, void* stream);
+/* Gradient of the weights: d_weight [top_k, batch] -> d_logits [num_experts,
+ * batch] (row stride d_ld, the logits' type).  expert and weight are those of
+ * the forward call; the d_weight of a choice that was not made is not read
+ * into any result. */
+ponni_b200_status ponni_b200_route_columns_backward(int dtype, const void* logits, int64_t ld, int num_experts,
+                                                    int top_k, int64_t batch, int normalise, const int32_t* expert,
+                                                    const float* weight, const float* d_weight, void* d_logits,
+                                                    int64_t d_ld, int device, void* stream);
+
+/* rows[row[j][b]][f] = x[f][b]; rows from *num_used (device memory, normally
+ * offset + num_experts) to batch * top_k are set to zero. */
+ponni_b200_status ponni_b200_gather_columns(int dtype, const void* x, int64_t ld, int features, int64_t batch, int top_k,
+                                            const int32_t* row, const int32_t* num_used, void* rows, int64_t rows_ld,
+                                            int device, void* stream);
+/* y[f][b] = sum_j weight[j][b] rows[row[j][b]][f], in fp32, rounded once;
+ * weight NULL: unit weights (the gradient of gather_columns). */
+ponni_b200_status ponni_b200_combine_rows(int dtype, const void* rows, int64_t rows_ld, int features, int64_t batch,
+                                          int top_k, const int32_t* row, const float* weight, void* y, int64_t ld,
+                                          int device, void* stream);
+/* d_rows[row[j][b]][f] = weight[j][b] d_y[f][b] (unused rows zero) and
+ * d_weight[j][b] = sum_f rows[row[j][b]][f] d_y[f][b]. */
+ponni_b200_status ponni_b200_combine_rows_backward(int dtype, const void* d_y, int64_t ld, const void* rows,
+                                                   int64_t rows_ld, int features, int64_t batch, int top_k,
+                                                   const int32_t* row, const float* weight, const int32_t* num_used,
+                                                   void* d_rows, int64_t d_ld, float* d_weight, int device,
+                                                   void* stream);
+
+/* out[r] = activation(rows[r] weights[e] + bias[e]) for r in [offset[e],
+ * offset[e + 1]); rows in no group give zero.  weights[e] is [inputs, outputs]
+ * as in Matvec (row stride w_ld, expert stride w_stride elements), bias
+ * [experts, outputs] or NULL; one type, fp32 / fp16 / bf16, sums in fp32.
+ * `activation` is the ponni_b200_layer_kind of an activation (PONNI_B200_RELU to
+ * PONNI_B200_MISH) with its flags and scalars,
+ * or -1. */
+int64_t ponni_b200_expert_product_workspace(int dtype, int64_t num_rows, int experts, int inputs, int outputs,
+                                            int backward);
+ponni_b200_status ponni_b200_expert_product(int dtype, const void* rows, int64_t rows_ld, int64_t num_rows,
+                                            const void* weights, int64_t w_ld, int64_t w_stride, const void* bias,
+                                            const int32_t* offset, int experts, int inputs, int outputs, int activation,
+                                            int activation_flags, double scalar0, double scalar1, void* out,
+                                            int64_t out_ld, void* workspace, int64_t workspace_bytes, int device,
+                                            void* stream);
+/* Gradients of rows weights[e] + bias[e]: d_rows (zero for rows in no group),
+ * d_weights [experts, inputs, outputs] and d_bias [experts, outputs], dense;
+ * zero for experts without rows.  A NULL output is not computed. */
+ponni_b200_status ponni_b200_expert_product_backward(int dtype, const void* d_out, int64_t d_out_ld, const void* rows,
+                                                     int64_t rows_ld, int64_t num_rows, const void* weights,
+                                                     int64_t w_ld, int64_t w_stride, const int32_t* offset, int experts,
+                                                     int inputs, int outputs, void* d_rows, int64_t d_rows_ld,
+                                                     void* d_weights, void* d_bias, void* workspace,
+                                                     int64_t workspace_bytes, int device, void* stream);
+
+/* A set of gradient tensors (dense, any mix of the four types) whose memory
+ * stays where it is while the set lives.  _create allocates a device table and
+ * waits for its copy. */
+typedef struct ponni_b200_gradient_set ponni_b200_gradient_set;
+ponni_b200_status ponni_b200_gradient_set_create(const void* const* tensors, const int64_t* counts,
+                                                 const int32_t* dtypes, int num_tensors, int device,
+                                                 ponni_b200_gradient_set** out_set);
+void ponni_b200_gradient_set_destroy(ponni_b200_gradient_set* set);
+int64_t ponni_b200_gradient_set_count(const ponni_b200_gradient_set* set);
+int64_t ponni_b200_gradient_set_workspace(const ponni_b200_gradient_set* set);
+/* *norm (device, fp32) = sqrt(sum g^2) over the set.  Where it is finite and
+ * above max_norm, every g is scaled by max_norm / norm.  flat NULL: in place;
+ * else the (scaled) gradients are written to flat, gradient_set_count values
+ * of flat_dtype in tensor order -- the order of
+ * ponni_b200_set_trainable_parameters_device -- and stay as they are
+ * themselves. */
+ponni_b200_status ponni_b200_gradient_set_clip(ponni_b200_gradient_set* set, double max_norm, void* flat, int flat_dtype,
+                                               float* norm, void* workspace, int64_t workspace_bytes, void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

@@ -16,6 +16,9 @@ from .inference import (Inference, create_inference_model, create_inference_mode
                         create_inference_model_double_precision, create_inference_model_half_precision,
                         create_inference_model_bhalf_precision, build_descriptors, to_dtype_bytes,
                         from_dtype_bytes, bf16_bits, bf16_to_f32, dtype_code, torch_stream_handle)
+from .experts import (Routing, GradientSet, route_columns, route_columns_backward, gather_columns,
+                      gather_columns_backward, combine_rows, combine_rows_backward, expert_product,
+                      expert_product_backward, clip_gradients, check_operators)
 
 
 def device_count() -> int:

@@ -99,7 +99,28 @@ SIGNATURES = {
     "ponni_b200_model_summary": (_STATUS, [_P, ctypes.c_char_p, ctypes.c_size_t]),
     "ponni_b200_fill_synthetic": (_STATUS, [_I, _P, _I64, _I64, _I64, _I64, ctypes.c_uint64, _I,
                                             ctypes.c_double, ctypes.c_double, _P]),
+    "ponni_b200_operator_error": (ctypes.c_char_p, []),
+    "ponni_b200_operator_check": (_STATUS, [_I, _P]),
+    "ponni_b200_route_workspace": (_I64, [_I, _I64]),
+    "ponni_b200_route_columns": (_STATUS, [_I, _P, _I64, _I, _I, _I64, _I, _P, _P, _P, _P, _P, _P, _I64, _I, _P]),
+    "ponni_b200_route_columns_backward": (_STATUS, [_I, _P, _I64, _I, _I, _I64, _I, _P, _P, _P, _P, _I64, _I, _P]),
+    "ponni_b200_gather_columns": (_STATUS, [_I, _P, _I64, _I, _I64, _I, _P, _P, _P, _I64, _I, _P]),
+    "ponni_b200_combine_rows": (_STATUS, [_I, _P, _I64, _I, _I64, _I, _P, _P, _P, _I64, _I, _P]),
+    "ponni_b200_combine_rows_backward": (_STATUS, [_I, _P, _I64, _P, _I64, _I, _I64, _I, _P, _P, _P, _P, _I64, _P, _I,
+                                                   _P]),
+    "ponni_b200_expert_product_workspace": (_I64, [_I, _I64, _I, _I, _I, _I]),
+    "ponni_b200_expert_product": (_STATUS, [_I, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I, _I, _I, _I, _I,
+                                            ctypes.c_double, ctypes.c_double, _P, _I64, _P, _I64, _I, _P]),
+    "ponni_b200_expert_product_backward": (_STATUS, [_I, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I, _I, _I, _P,
+                                                     _I64, _P, _P, _P, _I64, _I, _P]),
+    "ponni_b200_gradient_set_create": (_STATUS, [_P, _P, _P, _I, _I, ctypes.POINTER(_P)]),
+    "ponni_b200_gradient_set_destroy": (None, [_P]),
+    "ponni_b200_gradient_set_count": (_I64, [_P]),
+    "ponni_b200_gradient_set_workspace": (_I64, [_P]),
+    "ponni_b200_gradient_set_clip": (_STATUS, [_P, ctypes.c_double, _P, _I, _P, _P, _I64, _P]),
 }
+
+ROUTE_SELECTED, ROUTE_ALL = 0, 1
 
 _lib = None
 

@@ -1,0 +1,278 @@
+// Norm over many gradient tensors together, and clipping.
+//
+// norm = sqrt(sum over all tensors of g^2).  Where it is finite and above
+// max_norm every g becomes g max_norm / norm, in place or packed into one flat
+// vector in tensor order; otherwise the gradients stay as they are (packed:
+// are copied).
+//
+// Bound by HBM: one read for the norm, one read and one write for the scaling
+// (the read comes from L2 where the set fits it: the second pass goes through
+// the chunks in reverse).  The tensors are cut into chunks once, when the set
+// is made; a block sums its chunks in a fixed order and the partial sums are
+// added in a fixed order, so the norm does not change from run to run.
+// Squares are summed in fp32 over one vector and in fp64 from there: a sum of
+// 2^30 squares keeps fp32's full precision, and the fp32 part is redone in
+// fp64 where it over- or underflows.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "device_math.cuh"
+#include "operators.h"
+
+struct ponni_b200_gradient_set {
+  int device = 0;
+  int64_t total = 0;
+  int64_t num_chunks = 0;
+  void* chunks = nullptr;  // device table
+};
+
+namespace ponni_b200 {
+namespace {
+
+constexpr int kBlock = 512;
+constexpr int kMaxBlocks = 148 * 4;
+
+struct Chunk {
+  void* p;
+  int64_t flat;   // element offset in the packed vector
+  int32_t count;
+  int32_t dtype;
+};
+
+// Vectors of 16 bytes.
+template <class T> struct Vec {
+  static constexpr int n = 16 / sizeof(T);
+  T v[n];
+};
+
+__device__ __forceinline__ double square64(float x) { return (double)x * (double)x; }
+
+template <class T>
+__device__ __forceinline__ double squares(const T* __restrict__ p, int count) {
+  using C = typename Num<T>::C;
+  constexpr int n = Vec<T>::n;
+  double s = 0.0;
+  int done = 0;
+  if (reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+    const int vecs = count / n;
+    for (int i = threadIdx.x; i < vecs; i += kBlock) {
+      const uint4 raw = reinterpret_cast<const uint4*>(p)[i];
+      const Vec<T> v = *reinterpret_cast<const Vec<T>*>(&raw);
+      if constexpr (sizeof(C) == 8) {
+#pragma unroll
+        for (int k = 0; k < n; ++k) s = fma((double)Num<T>::to_c(v.v[k]), (double)Num<T>::to_c(v.v[k]), s);
+      } else {
+        float t = 0.0f;
+#pragma unroll
+        for (int k = 0; k < n; ++k) t = fmaf(Num<T>::to_c(v.v[k]), Num<T>::to_c(v.v[k]), t);
+        if (t > 1e-30f && t < 1e38f) {
+          s += t;
+        } else {
+#pragma unroll
+          for (int k = 0; k < n; ++k) s += square64(Num<T>::to_c(v.v[k]));
+        }
+      }
+    }
+    done = vecs * n;
+  }
+  for (int i = done + threadIdx.x; i < count; i += kBlock) {
+    const double x = (double)Num<T>::to_c(p[i]);
+    s = fma(x, x, s);
+  }
+  return s;
+}
+
+// Sum over the block, the same in every thread.
+__device__ __forceinline__ double block_sum(double v, double* sums) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double t = 0.0;
+#pragma unroll
+  for (int i = 0; i < kBlock / 32; ++i) t += sums[i];
+  return t;
+}
+
+__global__ void __launch_bounds__(kBlock)
+    norm_kernel(const Chunk* __restrict__ chunks, int64_t num_chunks, double* __restrict__ partial) {
+  __shared__ double sums[kBlock / 32];
+  ops::let_successor_start();
+  double s = 0.0;
+  for (int64_t i = blockIdx.x; i < num_chunks; i += gridDim.x) {
+    const Chunk c = chunks[i];
+    switch (c.dtype) {
+      case PONNI_B200_F32: s += squares(static_cast<const float*>(c.p), c.count); break;
+      case PONNI_B200_F64: s += squares(static_cast<const double*>(c.p), c.count); break;
+      case PONNI_B200_F16: s += squares(static_cast<const __half*>(c.p), c.count); break;
+      default: s += squares(static_cast<const __nv_bfloat16*>(c.p), c.count); break;
+    }
+  }
+  const double t = block_sum(s, sums);
+  if (threadIdx.x == 0) partial[blockIdx.x] = t;
+}
+
+template <class T, class O>
+__device__ __forceinline__ O scaled(T x, double scale) {
+  if constexpr (sizeof(T) == 8) return (O)Num<O>::from_c((typename Num<O>::C)((double)x * scale));
+  else if constexpr (sizeof(O) == 8) return (double)Num<T>::to_c(x) * scale;
+  else return Num<O>::from_c(Num<T>::to_c(x) * (float)scale);
+}
+
+template <class T, class O>
+__device__ __forceinline__ void rescale(const T* p, O* out, int count, double scale) {
+  constexpr int n = Vec<T>::n;
+  int done = 0;
+  if (sizeof(T) == sizeof(O) && reinterpret_cast<uintptr_t>(p) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
+    const int vecs = count / n;
+    for (int i = threadIdx.x; i < vecs; i += kBlock) {
+      const uint4 raw = reinterpret_cast<const uint4*>(p)[i];
+      const Vec<T> v = *reinterpret_cast<const Vec<T>*>(&raw);
+      Vec<O> o;
+#pragma unroll
+      for (int k = 0; k < n; ++k) o.v[k] = scaled<T, O>(v.v[k], scale);
+      reinterpret_cast<uint4*>(out)[i] = *reinterpret_cast<uint4*>(&o);
+    }
+    done = vecs * n;
+  }
+#pragma unroll 4
+  for (int i = done + threadIdx.x; i < count; i += kBlock) out[i] = scaled<T, O>(p[i], scale);
+}
+
+// flat_dtype < 0: in place.
+template <class T>
+__device__ __forceinline__ void rescale_to(const Chunk& c, void* flat, int flat_dtype, double scale) {
+  const T* p = static_cast<const T*>(c.p);
+  switch (flat_dtype) {
+    case PONNI_B200_F32: rescale(p, static_cast<float*>(flat) + c.flat, c.count, scale); break;
+    case PONNI_B200_F64: rescale(p, static_cast<double*>(flat) + c.flat, c.count, scale); break;
+    case PONNI_B200_F16: rescale(p, static_cast<__half*>(flat) + c.flat, c.count, scale); break;
+    case PONNI_B200_BF16: rescale(p, static_cast<__nv_bfloat16*>(flat) + c.flat, c.count, scale); break;
+    default: rescale(p, static_cast<T*>(c.p), c.count, scale); break;
+  }
+}
+
+__global__ void __launch_bounds__(kBlock)
+    clip_kernel(const Chunk* __restrict__ chunks, int64_t num_chunks, const double* __restrict__ partial,
+                int num_partial, double max_norm, void* __restrict__ flat, int flat_dtype, float* __restrict__ norm_out) {
+  __shared__ double sums[kBlock / 32];
+  ops::wait_for_predecessor();
+  double s = 0.0;
+  for (int i = threadIdx.x; i < num_partial; i += kBlock) s += partial[i];
+  const double norm = sqrt(block_sum(s, sums));
+  if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
+  const bool clip = norm > max_norm && norm < (double)INFINITY;
+  if (!clip && flat_dtype < 0) return;
+  const double scale = clip ? max_norm / norm : 1.0;
+  for (int64_t i = num_chunks - 1 - blockIdx.x; i >= 0; i -= gridDim.x) {
+    const Chunk c = chunks[i];
+    switch (c.dtype) {
+      case PONNI_B200_F32: rescale_to<float>(c, flat, flat_dtype, scale); break;
+      case PONNI_B200_F64: rescale_to<double>(c, flat, flat_dtype, scale); break;
+      case PONNI_B200_F16: rescale_to<__half>(c, flat, flat_dtype, scale); break;
+      default: rescale_to<__nv_bfloat16>(c, flat, flat_dtype, scale); break;
+    }
+  }
+}
+
+}  // namespace
+}  // namespace ponni_b200
+
+using namespace ponni_b200;
+
+extern "C" {
+
+ponni_b200_status ponni_b200_gradient_set_create(const void* const* tensors, const int64_t* counts,
+                                                 const int32_t* dtypes, int num_tensors, int device,
+                                                 ponni_b200_gradient_set** out) {
+  return ops::entry(device, [&]() -> ponni_b200_status {
+    if (!out) return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "gradient set: output pointer is NULL");
+    *out = nullptr;
+    if (num_tensors < 1 || !tensors || !counts || !dtypes)
+      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "gradient set: needs at least one tensor");
+    int64_t total = 0;
+    for (int i = 0; i < num_tensors; ++i) {
+      if (counts[i] < 0 || counts[i] > ((int64_t)1 << 40) || (counts[i] > 0 && !tensors[i]))
+        return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "gradient set: bad pointer or size of a tensor");
+      if (dtypes[i] < PONNI_B200_F32 || dtypes[i] > PONNI_B200_BF16)
+        return ops::fail(PONNI_B200_ERR_UNSUPPORTED, "gradient set: tensors must be fp32, fp64, fp16 or bf16");
+      if (reinterpret_cast<uintptr_t>(tensors[i]) % ops::element_bytes(dtypes[i]) != 0)
+        return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "gradient set: a tensor is not aligned to its type");
+      total += counts[i];
+    }
+    // About eight chunks a block, 2048 to 16384 elements each.
+    const int64_t per = std::min<int64_t>(16384, std::max<int64_t>(2048, total / (kMaxBlocks * 8) / 512 * 512));
+    std::vector<Chunk> table;
+    int64_t flat = 0;
+    for (int i = 0; i < num_tensors; ++i) {
+      const int64_t z = ops::element_bytes(dtypes[i]);
+      for (int64_t at = 0; at < counts[i]; at += per)
+        table.push_back({static_cast<char*>(const_cast<void*>(tensors[i])) + at * z, flat + at,
+                         (int32_t)std::min(per, counts[i] - at), dtypes[i]});
+      flat += counts[i];
+    }
+    ponni_b200_gradient_set* set = new (std::nothrow) ponni_b200_gradient_set;
+    if (!set) return ops::fail(PONNI_B200_ERR_CUDA, "gradient set: out of host memory");
+    set->device = device;
+    set->total = total;
+    set->num_chunks = (int64_t)table.size();
+    if (!table.empty()) {
+      cudaError_t e = cudaMalloc(&set->chunks, table.size() * sizeof(Chunk));
+      if (e == cudaSuccess) e = cudaMemcpy(set->chunks, table.data(), table.size() * sizeof(Chunk), cudaMemcpyHostToDevice);
+      if (e != cudaSuccess) {
+        if (set->chunks) cudaFree(set->chunks);
+        delete set;
+        cudaGetLastError();
+        return ops::fail_cuda(e, "gradient set");
+      }
+    }
+    *out = set;
+    return PONNI_B200_OK;
+  });
+}
+
+void ponni_b200_gradient_set_destroy(ponni_b200_gradient_set* set) {
+  if (!set) return;
+  {
+    DeviceGuard guard(set->device);
+    if (set->chunks && cudaFree(set->chunks) != cudaSuccess) cudaGetLastError();
+  }
+  delete set;
+}
+
+int64_t ponni_b200_gradient_set_count(const ponni_b200_gradient_set* set) { return set ? set->total : 0; }
+
+int64_t ponni_b200_gradient_set_workspace(const ponni_b200_gradient_set* set) {
+  return set ? (int64_t)kMaxBlocks * (int64_t)sizeof(double) : 0;
+}
+
+ponni_b200_status ponni_b200_gradient_set_clip(ponni_b200_gradient_set* set, double max_norm, void* flat, int flat_dtype,
+                                               float* norm, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!set) return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "clip: gradient set is NULL");
+  return ops::entry(set->device, [&]() -> ponni_b200_status {
+    if (!(max_norm > 0.0)) return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "clip: max_norm must be positive");
+    if (!norm) return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "clip: norm pointer is NULL");
+    if (flat && (flat_dtype < PONNI_B200_F32 || flat_dtype > PONNI_B200_BF16))
+      return ops::fail(PONNI_B200_ERR_UNSUPPORTED, "clip: the packed vector must be fp32, fp64, fp16 or bf16");
+    if (!workspace || workspace_bytes < ponni_b200_gradient_set_workspace(set) ||
+        reinterpret_cast<uintptr_t>(workspace) % 8 != 0)
+      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "clip: workspace is too small or not aligned to 8 bytes");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>(set->num_chunks, kMaxBlocks));
+    const Chunk* chunks = static_cast<const Chunk*>(set->chunks);
+    double* partial = static_cast<double*>(workspace);
+    norm_kernel<<<blocks, kBlock, 0, s>>>(chunks, set->num_chunks, partial);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess)
+      e = ops::launch_after(clip_kernel, dim3(blocks), dim3(kBlock), 0, s, chunks, set->num_chunks,
+                            (const double*)partial, blocks, max_norm, flat, flat ? flat_dtype : -1, norm);
+    if (e != cudaSuccess) return ops::fail_cuda(e, "clip");
+    return ops::launched("clip");
+  });
+}
+
+}  // extern "C"

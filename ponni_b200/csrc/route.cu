@@ -1,0 +1,383 @@
+// Softmax top-k routing of batch columns to experts, the expert-sorted row
+// order that follows from it, and the gradient of the routing weights.
+//
+// logits x[e][b] (feature-major, batch contiguous).  Choices of column b: the
+// top_k largest x[., b], ties to the lower expert; -inf and NaN are never
+// chosen and add nothing to a sum.  With m the column's largest logit and
+// t_e = exp(x_e - m) (1 where x_e = m, so that infinite logits share),
+//   weight_j = t_{e_j} / sum t,   the sum over the chosen experts or over all.
+// Rows: all (column, choice) pairs sorted by expert, then by column.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "device_math.cuh"
+#include "operators.h"
+
+namespace ponni_b200 {
+namespace {
+
+constexpr int kBlock = 256;  // columns of a tile
+constexpr int kWarps = kBlock / 32;
+
+template <class T>
+__device__ __forceinline__ float logit(const T* p) {
+  const float v = Num<T>::to_c(*p);
+  return v == v ? v : -INFINITY;
+}
+
+// Choice and weights of one column; K is the number of choices.
+template <class T, int K>
+__device__ __forceinline__ void choose(const T* __restrict__ x, int64_t ld, int experts, bool over_all, int (&idx)[K],
+                                       float (&w)[K]) {
+  float top[K];
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    top[j] = -INFINITY;
+    idx[j] = -1;
+  }
+  float sum = 0.0f;  // of exp(x - top[0]) over the experts seen
+  auto take = [&](float v, int e) {
+    if (over_all && v > -INFINITY) {
+      if (v > top[0]) sum = (top[0] > -INFINITY ? sum * expf(top[0] - v) : 0.0f) + 1.0f;
+      else sum += v == top[0] ? 1.0f : expf(v - top[0]);
+    }
+    if (v > top[K - 1]) {
+      top[K - 1] = v;
+      idx[K - 1] = e;
+#pragma unroll
+      for (int j = K - 1; j > 0; --j) {
+        if (top[j] > top[j - 1]) {
+          const float tv = top[j];
+          top[j] = top[j - 1];
+          top[j - 1] = tv;
+          const int ti = idx[j];
+          idx[j] = idx[j - 1];
+          idx[j - 1] = ti;
+        }
+      }
+    }
+  };
+  int e = 0;
+  for (; e + 8 <= experts; e += 8) {
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = logit(x + (int64_t)(e + u) * ld);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) take(v[u], e + u);
+  }
+  for (; e < experts; ++e) take(logit(x + (int64_t)e * ld), e);
+#pragma unroll
+  for (int j = 0; j < K; ++j) w[j] = idx[j] < 0 ? 0.0f : top[j] == top[0] ? 1.0f : expf(top[j] - top[0]);
+  if (!over_all) {
+    sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < K; ++j) sum += w[j];
+  }
+#pragma unroll
+  for (int j = 0; j < K; ++j) w[j] = idx[j] < 0 ? 0.0f : w[j] / sum;
+}
+
+// Choices of this block's columns [c0, c1) and how many of them each expert
+// took: counts[expert][block].
+template <class T, int K>
+__global__ void __launch_bounds__(kBlock)
+    choose_kernel(const T* __restrict__ x, int64_t ld, int experts, int64_t batch, int64_t per_block, int over_all,
+                  int* __restrict__ expert, float* __restrict__ weight, int* __restrict__ counts) {
+  extern __shared__ int hist[];
+  ops::let_successor_start();
+  for (int e = threadIdx.x; e < experts; e += kBlock) hist[e] = 0;
+  __syncthreads();
+  const int64_t c0 = blockIdx.x * per_block, c1 = min(batch, c0 + per_block);
+  for (int64_t b = c0 + threadIdx.x; b < c1; b += kBlock) {
+    int idx[K];
+    float w[K];
+    choose<T, K>(x + b, ld, experts, over_all, idx, w);
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      expert[j * batch + b] = idx[j];
+      weight[j * batch + b] = w[j];
+      if (idx[j] >= 0) atomicAdd(&hist[idx[j]], 1);
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < experts; e += kBlock) counts[(int64_t)e * gridDim.x + blockIdx.x] = hist[e];
+}
+
+// Exclusive scan of one value a thread over the block (kBlock threads);
+// every thread also gets the total.
+__device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int s = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, s, d);
+    if (lane >= d) s += o;
+  }
+  if (lane == 31) warp_sums[warp] = s;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    const int t = warp_sums[i];
+    if (i < warp) before += t;
+    total += t;
+  }
+  __syncthreads();
+  return before + s - v;
+}
+
+// counts[e][.] -> rows of expert e taken by earlier blocks; totals[e].
+__global__ void __launch_bounds__(kBlock) scan_kernel(int* __restrict__ counts, int blocks, int* __restrict__ totals) {
+  __shared__ int warp_sums[kWarps];
+  ops::let_successor_start();
+  ops::wait_for_predecessor();
+  int* c = counts + (int64_t)blockIdx.x * blocks;
+  int carry = 0;
+  for (int i0 = 0; i0 < blocks; i0 += kBlock) {
+    const int i = i0 + threadIdx.x;
+    int total;
+    const int before = block_scan(i < blocks ? c[i] : 0, warp_sums, total);
+    if (i < blocks) c[i] = carry + before;
+    carry += total;
+  }
+  if (threadIdx.x == 0) totals[blockIdx.x] = carry;
+}
+
+// Rows of this block's choices.  Within a tile of kBlock columns the rank
+// of a choice is the number of earlier columns that chose the same expert
+// (at most once each): a lane mask per warp and expert in shared memory.
+__global__ void __launch_bounds__(kBlock)
+    place_kernel(const int* __restrict__ expert, int experts, int top_k, int64_t batch, int64_t per_block,
+                 const int* __restrict__ counts, const int* __restrict__ totals, int* __restrict__ row,
+                 int* __restrict__ column, int* __restrict__ offset) {
+  extern __shared__ int sm[];
+  __shared__ int warp_sums[kWarps];
+  int* next = sm;                                                  // [experts]: next row of each expert
+  unsigned* mask = reinterpret_cast<unsigned*>(sm + experts);  // [kWarps][experts]
+  for (int i = threadIdx.x; i < kWarps * experts; i += kBlock) mask[i] = 0;
+  ops::wait_for_predecessor();
+  int carry = 0;
+  for (int e0 = 0; e0 < experts; e0 += kBlock) {
+    const int e = e0 + threadIdx.x;
+    int total;
+    const int before = carry + block_scan(e < experts ? totals[e] : 0, warp_sums, total);
+    if (e < experts) {
+      next[e] = before + counts[(int64_t)e * gridDim.x + blockIdx.x];
+      if (blockIdx.x == 0) offset[e] = before;
+    }
+    carry += total;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) offset[experts] = carry;
+  for (int64_t i = carry + blockIdx.x * (int64_t)kBlock + threadIdx.x; i < batch * top_k;
+       i += (int64_t)gridDim.x * kBlock)
+    column[i] = -1;
+  __syncthreads();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c0 = blockIdx.x * per_block, c1 = min(batch, c0 + per_block);
+  for (int64_t t0 = c0; t0 < c1; t0 += kBlock) {
+    const int64_t b = t0 + threadIdx.x;
+    for (int j = 0; j < top_k; ++j) {
+      const int e = b < c1 ? expert[j * batch + b] : -1;
+      if (e >= 0) atomicOr(&mask[warp * experts + e], 1u << lane);
+    }
+    __syncthreads();
+    if (b < c1) {
+      for (int j = 0; j < top_k; ++j) {
+        const int e = expert[j * batch + b];
+        int r = -1;
+        if (e >= 0) {
+          r = next[e] + __popc(mask[warp * experts + e] & ((1u << lane) - 1u));
+          for (int w = 0; w < warp; ++w) r += __popc(mask[w * experts + e]);
+          column[r] = (int)b;
+        }
+        row[j * batch + b] = r;
+      }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += kBlock) {
+      int n = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        n += __popc(mask[w * experts + e]);
+        mask[w * experts + e] = 0;
+      }
+      next[e] += n;
+    }
+    __syncthreads();
+  }
+}
+
+// d_x[e][b] = p_e (d_p_e - sum_j w_j d_w_j), d_p_e = d_w_j for the chosen
+// experts and 0 for others; p is the softmax over all experts or over the
+// chosen ones.  Over all: the first choice has t = 1, so p_e = t_e weight_0
+// and no second sum is needed.
+template <class T>
+__global__ void __launch_bounds__(kBlock)
+    route_backward_kernel(const T* __restrict__ x, int64_t ld, int experts, int top_k, int64_t batch, int over_all,
+                          const int* __restrict__ expert, const float* __restrict__ weight,
+                          const float* __restrict__ d_weight, T* __restrict__ dx, int64_t d_ld, int per_part) {
+  const int64_t b = blockIdx.x * (int64_t)kBlock + threadIdx.x;
+  if (b >= batch) return;
+  int idx[ops::kMaxTopK];
+  float g[ops::kMaxTopK];
+  float mean = 0.0f;
+#pragma unroll
+  for (int j = 0; j < ops::kMaxTopK; ++j) {
+    idx[j] = -1;
+    g[j] = 0.0f;
+    if (j < top_k) {
+      idx[j] = expert[j * batch + b];
+      if (idx[j] >= 0) {
+        const float w = weight[j * batch + b];
+        g[j] = w * d_weight[j * batch + b];
+        mean += g[j];
+      }
+    }
+  }
+  const int e0 = blockIdx.y * per_part, e1 = min(experts, e0 + per_part);
+  const bool any = idx[0] >= 0;
+  const float best = any && over_all ? logit(x + idx[0] * ld + b) : 0.0f;
+  const float scale = any && over_all ? weight[b] : 0.0f;
+  for (int e = e0; e < e1; ++e) {
+    float d = 0.0f;
+    if (any && over_all) {
+      const float v = logit(x + e * ld + b);
+      const float p = v == best ? scale : expf(v - best) * scale;
+      d = -p * mean;
+    }
+#pragma unroll
+    for (int j = 0; j < ops::kMaxTopK; ++j)
+      if (idx[j] == e) d = over_all ? d + g[j] : g[j] - weight[j * batch + b] * mean;
+    dx[e * d_ld + b] = Num<T>::from_c(d);
+  }
+}
+
+int64_t blocks_of(int64_t batch) { return std::min<int64_t>((batch + kBlock - 1) / kBlock, 592); }
+
+template <class T, int K>
+cudaError_t launch_choose(const void* x, int64_t ld, int experts, int64_t batch, int64_t per_block, int blocks, int all,
+                          int* expert, float* weight, int* counts, cudaStream_t s) {
+  choose_kernel<T, K><<<blocks, kBlock, experts * sizeof(int), s>>>(static_cast<const T*>(x), ld, experts, batch,
+                                                                     per_block, all, expert, weight, counts);
+  return cudaGetLastError();
+}
+template <class T>
+cudaError_t launch_choose_k(int k, const void* x, int64_t ld, int experts, int64_t batch, int64_t per_block, int blocks,
+                            int all, int* expert, float* weight, int* counts, cudaStream_t s) {
+  switch (k) {
+#define PB_CASE(K) \
+  case K: return launch_choose<T, K>(x, ld, experts, batch, per_block, blocks, all, expert, weight, counts, s)
+    PB_CASE(1);
+    PB_CASE(2);
+    PB_CASE(3);
+    PB_CASE(4);
+    PB_CASE(5);
+    PB_CASE(6);
+    PB_CASE(7);
+    PB_CASE(8);
+#undef PB_CASE
+  }
+  return cudaErrorInvalidValue;
+}
+
+ponni_b200_status check_route(int dtype, const void* logits, int64_t ld, int experts, int top_k, int64_t batch,
+                              int normalise) {
+  using namespace ops;
+  if (!is_real_type(dtype)) return fail(PONNI_B200_ERR_UNSUPPORTED, "route: logits must be fp32, fp16 or bf16");
+  if (!logits) return fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route: logits pointer is NULL");
+  if (experts < 1 || experts > kMaxExperts)
+    return fail(PONNI_B200_ERR_UNSUPPORTED, "route: the number of experts must be 1 to 1024");
+  if (top_k < 1 || top_k > kMaxTopK || top_k > experts)
+    return fail(PONNI_B200_ERR_UNSUPPORTED, "route: top_k must be 1 to 8 and at most the number of experts");
+  if (batch < 1 || batch > INT32_MAX / top_k)
+    return fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route: batch must be nonzero and batch * top_k below 2^31");
+  if (ld < batch) return fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route: row stride smaller than the batch size");
+  if (normalise != PONNI_B200_ROUTE_SELECTED && normalise != PONNI_B200_ROUTE_ALL)
+    return fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route: unknown normalisation");
+  return PONNI_B200_OK;
+}
+
+}  // namespace
+}  // namespace ponni_b200
+
+using namespace ponni_b200;
+
+extern "C" {
+
+int64_t ponni_b200_route_workspace(int num_experts, int64_t batch) {
+  if (num_experts < 1 || batch < 1) return 0;
+  return (int64_t)num_experts * (blocks_of(batch) + 1) * (int64_t)sizeof(int);
+}
+
+ponni_b200_status ponni_b200_route_columns(int dtype, const void* logits, int64_t ld, int num_experts, int top_k,
+                                           int64_t batch, int normalise, int32_t* expert, float* weight, int32_t* row,
+                                           int32_t* column, int32_t* offset, void* workspace, int64_t workspace_bytes,
+                                           int device, void* stream) {
+  return ops::entry(device, [&]() -> ponni_b200_status {
+    ponni_b200_status st = check_route(dtype, logits, ld, num_experts, top_k, batch, normalise);
+    if (st) return st;
+    if (!expert || !weight || !row || !column || !offset)
+      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route: output pointer is NULL");
+    if (!workspace || workspace_bytes < ponni_b200_route_workspace(num_experts, batch))
+      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route: workspace is too small");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int64_t tiles = (batch + kBlock - 1) / kBlock;
+    const int64_t most = blocks_of(batch);
+    const int64_t per_block = (tiles + most - 1) / most * kBlock;
+    const int blocks = (int)((batch + per_block - 1) / per_block);
+    int* counts = static_cast<int*>(workspace);
+    int* totals = counts + (int64_t)num_experts * blocks;
+    const int all = normalise == PONNI_B200_ROUTE_ALL;
+    cudaError_t e = cudaErrorInvalidValue;
+    if (dtype == PONNI_B200_F32)
+      e = launch_choose_k<float>(top_k, logits, ld, num_experts, batch, per_block, blocks, all, expert, weight, counts, s);
+    else if (dtype == PONNI_B200_F16)
+      e = launch_choose_k<__half>(top_k, logits, ld, num_experts, batch, per_block, blocks, all, expert, weight, counts, s);
+    else
+      e = launch_choose_k<__nv_bfloat16>(top_k, logits, ld, num_experts, batch, per_block, blocks, all, expert, weight,
+                                         counts, s);
+    if (e == cudaSuccess)
+      e = ops::launch_after(scan_kernel, dim3(num_experts), dim3(kBlock), 0, s, counts, blocks, totals);
+    if (e == cudaSuccess)
+      e = ops::launch_after(place_kernel, dim3(blocks), dim3(kBlock), (size_t)num_experts * (kWarps + 1) * sizeof(int),
+                            s, (const int*)expert, num_experts, top_k, batch, per_block, (const int*)counts,
+                            (const int*)totals, row, column, offset);
+    if (e != cudaSuccess) return ops::fail_cuda(e, "route_columns");
+    return ops::launched("route_columns");
+  });
+}
+
+ponni_b200_status ponni_b200_route_columns_backward(int dtype, const void* logits, int64_t ld, int num_experts,
+                                                    int top_k, int64_t batch, int normalise, const int32_t* expert,
+                                                    const float* weight, const float* d_weight, void* d_logits,
+                                                    int64_t d_ld, int device, void* stream) {
+  return ops::entry(device, [&]() -> ponni_b200_status {
+    ponni_b200_status st = check_route(dtype, logits, ld, num_experts, top_k, batch, normalise);
+    if (st) return st;
+    if (!expert || !weight || !d_weight || !d_logits)
+      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route backward: pointer is NULL");
+    if (d_ld < batch)
+      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route backward: row stride smaller than the batch size");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int per_part = 16;
+    const dim3 grid((unsigned)((batch + kBlock - 1) / kBlock), (unsigned)((num_experts + per_part - 1) / per_part));
+    const int all = normalise == PONNI_B200_ROUTE_ALL;
+    if (dtype == PONNI_B200_F32)
+      route_backward_kernel<float><<<grid, kBlock, 0, s>>>((const float*)logits, ld, num_experts, top_k, batch, all,
+                                                             expert, weight, d_weight, (float*)d_logits, d_ld, per_part);
+    else if (dtype == PONNI_B200_F16)
+      route_backward_kernel<__half><<<grid, kBlock, 0, s>>>((const __half*)logits, ld, num_experts, top_k, batch, all,
+                                                              expert, weight, d_weight, (__half*)d_logits, d_ld,
+                                                              per_part);
+    else
+      route_backward_kernel<__nv_bfloat16><<<grid, kBlock, 0, s>>>(
+          (const __nv_bfloat16*)logits, ld, num_experts, top_k, batch, all, expert, weight, d_weight,
+          (__nv_bfloat16*)d_logits, d_ld, per_part);
+    return ops::launched("route_columns_backward");
+  });
+}
+
+}  // extern "C"
