@@ -402,10 +402,12 @@ ponni_b200_status ponni_b200_combine_rows_backward(int dtype, const void* d_y, i
  * as in Matvec (row stride w_ld, expert stride w_stride elements), bias
  * [experts, outputs] or NULL; one type, fp32 / fp16 / bf16, sums in fp32.
  * `activation` is the ponni_b200_layer_kind of an activation (PONNI_B200_RELU to
- * PONNI_B200_MISH) with its flags and scalars,
- * or -1. */
+ * PONNI_B200_MISH) with its flags and scalars, or -1.  The workspace holds copies
+ * of operands that the copy engine cannot read in place: fp32 ones, and 16-bit
+ * ones whose address or strides are not multiples of 16 bytes; pass `aligned`
+ * nonzero when rows, weights (and d_out) and their strides all are. */
 int64_t ponni_b200_expert_product_workspace(int dtype, int64_t num_rows, int experts, int inputs, int outputs,
-                                            int backward);
+                                            int aligned, int backward, int device);
 ponni_b200_status ponni_b200_expert_product(int dtype, const void* rows, int64_t rows_ld, int64_t num_rows,
                                             const void* weights, int64_t w_ld, int64_t w_stride, const void* bias,
                                             const int32_t* offset, int experts, int inputs, int outputs, int activation,

@@ -108,7 +108,7 @@ SIGNATURES = {
     "ponni_b200_combine_rows": (_STATUS, [_I, _P, _I64, _I, _I64, _I, _P, _P, _P, _I64, _I, _P]),
     "ponni_b200_combine_rows_backward": (_STATUS, [_I, _P, _I64, _P, _I64, _I, _I64, _I, _P, _P, _P, _P, _I64, _P, _I,
                                                    _P]),
-    "ponni_b200_expert_product_workspace": (_I64, [_I, _I64, _I, _I, _I, _I]),
+    "ponni_b200_expert_product_workspace": (_I64, [_I, _I64, _I, _I, _I, _I, _I, _I]),
     "ponni_b200_expert_product": (_STATUS, [_I, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I, _I, _I, _I, _I,
                                             ctypes.c_double, ctypes.c_double, _P, _I64, _P, _I64, _I, _P]),
     "ponni_b200_expert_product_backward": (_STATUS, [_I, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I, _I, _I, _P,

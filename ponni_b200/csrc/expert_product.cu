@@ -1,40 +1,68 @@
 // Products grouped by expert: rows r in [offset[e], offset[e+1]) times
-// weights[e] (in x out, row-major), and the gradients.
+// weights[e] (inputs x outputs, row-major as in Matvec), with bias and
+// activation, and the gradients
+//   kForward  out[r]      = act(rows[r] W_e + b_e)       M rows,   N outputs, K inputs
+//   kRows     d_rows[r]   = d_out[r] W_e^T               M rows,   N inputs,  K outputs
+//   kWeights  d_W_e       = rows_e^T d_out_e             M inputs, N outputs, K rows of the group
+// as tcgen05 products of 128 x BN tiles, K in blocks of 64.
+//
+// Operands are read where they lie: the groups' rows start anywhere, but rows
+// are the outer index of every operand, so a tile starts at any row with an
+// aligned innermost coordinate, and whichever index is contiguous decides
+// between K-major and MN-major shared-memory tiles (no transposed copies):
+//            A                    B
+//   kForward rows     K-major     W_e     MN-major
+//   kRows    d_out    K-major     W_e     K-major
+//   kWeights rows     MN-major    d_out   MN-major
+// A row tile that runs past its group computes on the next group's rows and
+// does not store them; in kWeights the rows past the group are the
+// contraction, so the last K block's are zeroed in shared memory (both
+// operands: the neighbour's values may be infinite).
+//
+// fp32 operands are split exactly into three bf16 parts x = x0 + x1 + x2 and six
+// products are kept (the three dropped are below 2^-24 of the magnitudes).  Each K
+// block of 64 goes into its own TMEM accumulator, the five small products first,
+// and is added to the tile's sum in fp32 registers: the tensor core truncates
+// when it accumulates, so long sums in TMEM would drift by a part of 2^-24 for
+// every step.
+//
+// One persistent CTA per SM: a TMA producer, an MMA warp and eight epilogue
+// warps.  Every role walks the same tile sequence, which it derives from the
+// offsets (read once into shared memory): no host copy of the group sizes.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cstring>
+#include <type_traits>
 
 #include "device_math.cuh"
 #include "operators.h"
+#include "tc_common.cuh"
+
+PONNI_B200_SKIP_ARRIVE_FLAG(ge)
 
 namespace ponni_b200 {
 namespace {
-
-constexpr int kTile = 64, kStep = 16, kBlock = 256;
-
-// The groups as the kernels read them: kept within [0, rows] and ascending
-// whatever the offsets hold; a violation is recorded.
-__device__ __forceinline__ void group_of(const int* __restrict__ offset, int experts, int e, int64_t rows, int64_t& lo,
-                                         int64_t& hi) {
-  lo = min(max((int64_t)offset[e], (int64_t)0), rows);
-  hi = min(max((int64_t)offset[e + 1], lo), rows);
-}
-
-// The first block's check of the offsets (the groups are clamped whatever they hold).
-__device__ __forceinline__ void check_offsets(const int* __restrict__ offset, int experts, int64_t rows, int* error) {
-  for (int e = threadIdx.x; e <= experts; e += blockDim.x) {
-    const int64_t o = offset[e], before = e ? offset[e - 1] : 0;
-    if (o < before || o > rows || (e == 0 && o != 0)) atomicOr(error, 2);
-  }
-}
+using namespace tc;
 
 enum Mode { kForward, kRows, kWeights };
 
+constexpr int kBM = 128, kBK = 64;
+constexpr int kEpiWarps = 8;
+constexpr int kBlock = 32 * (2 + kEpiWarps);
+constexpr int kEpiPitch = 80;  // bytes of a staged output row segment of 64 (+16: conflict-free)
+constexpr int kEpiBytes = kEpiWarps * 32 * kEpiPitch;
+constexpr int kBiasBytes = kEpiWarps * 128 * 4;
+constexpr int kMaxStages = 8;
+constexpr int kSmemLimit = 232448;
+
 struct Args {
-  const void* a;  // kForward: rows; kRows: d_out; kWeights: rows
+  const void* a;  // kForward: rows; kRows: d_out; kWeights: rows (as the caller gave them)
   const void* b;  // kForward, kRows: weights; kWeights: d_out
   void* c;
+  float* partial;  // kWeights, split: fp32 sums of every unit [unit][inputs][outputs]
   int64_t a_ld, b_ld, b_stride, c_ld;
   int64_t rows;
   const int* offset;
@@ -42,129 +70,716 @@ struct Args {
   int experts, inputs, outputs;
   int act, act_flags;
   float s0, s1;
+  int unit_rows;  // kWeights: rows of a unit (a multiple of kBK); 0: a group is one unit
+  int vec;        // c may be written 16 bytes at a time
+  int stages;
   int* error;
 };
 
-template <class T, int MODE>
-__global__ void __launch_bounds__(kBlock) simple_kernel(const Args p) {
-  __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1];
-  const T* a = static_cast<const T*>(p.a);
-  const T* b = static_cast<const T*>(p.b);
-  T* c = static_cast<T*>(p.c);
-  if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) check_offsets(p.offset, p.experts, p.rows, p.error);
+template <class T, int P, int BN> struct Shape {
+  static constexpr int a_bytes = P * kBM * kBK * 2;
+  static constexpr int b_bytes = P * BN * kBK * 2;
+  static constexpr int stage_bytes = a_bytes + b_bytes;
+  static constexpr int acc_cols = P == 3 ? 128 : 256;
+  static constexpr int acc_bufs = 512 / acc_cols;
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+      "[%5];\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+
+// Check of the offsets by one block (the groups are clamped whatever they hold).
+__device__ __forceinline__ void check_offsets(const int* __restrict__ offset, int experts, int64_t rows, int* error) {
+  for (int e = threadIdx.x; e <= experts; e += blockDim.x) {
+    const int64_t o = offset[e], before = e ? offset[e - 1] : 0;
+    if (o < before || o > rows || (e == 0 && o != 0)) atomicOr(error, 2);
+  }
+}
+__device__ __forceinline__ int clamped(int o, int lo, int64_t rows) { return (int)min(max((int64_t)o, (int64_t)lo), rows); }
+
+struct Tile {
+  int e, m0, n0;
+  int lo, hi;    // kForward, kRows: the group's rows; kWeights: the unit's
+  int k_blocks;
+  int64_t slot;  // kWeights, split: the unit's partial sums
+};
+
+// The tile sequence of this CTA: blockIdx.x, blockIdx.x + gridDim.x, ... of all
+// tiles, experts in order, row tiles innermost (neighbouring CTAs share the
+// weight tile).
+template <int MODE, int BN> struct Tiles {
+  const int* lo;
+  const int* hi;
+  int experts, m_tiles, n_tiles, k_blocks, unit_rows;
   int e = 0;
-  int64_t lo = 0, hi = 0, m0 = 0;
-  int m_end, n_end, k_end;
-  if (MODE == kWeights) {
-    e = blockIdx.z;
-    group_of(p.offset, p.experts, e, p.rows, lo, hi);
-    m0 = (int64_t)blockIdx.x * kTile;
-    m_end = p.inputs;
-    n_end = p.outputs;
-    k_end = (int)(hi - lo);
-  } else {
-    int64_t t = blockIdx.x;  // tile of rows: the experts' tiles, then the rows in no group
-    for (; e < p.experts; ++e) {
-      group_of(p.offset, p.experts, e, p.rows, lo, hi);
-      const int64_t tiles = (hi - lo + kTile - 1) / kTile;
-      if (t < tiles) break;
-      t -= tiles;
-    }
-    n_end = MODE == kForward ? p.outputs : p.inputs;
-    k_end = MODE == kForward ? p.inputs : p.outputs;
-    if (e == p.experts) {
-      lo = min(max((int64_t)p.offset[p.experts], (int64_t)0), p.rows);
-      hi = p.rows;
-      k_end = 0;
-    }
-    m0 = t * kTile;
-    if (m0 >= hi - lo) return;
-    m_end = (int)(hi - lo);
+  int64_t t, base = 0;
+
+  __device__ Tiles(const Args& p, const int* lo_, const int* hi_) : lo(lo_), hi(hi_), experts(p.experts), t(blockIdx.x) {
+    const int n = MODE == kRows ? p.inputs : p.outputs, k = MODE == kForward ? p.inputs : p.outputs;
+    m_tiles = (p.inputs + kBM - 1) / kBM;
+    n_tiles = (n + BN - 1) / BN;
+    k_blocks = (k + kBK - 1) / kBK;
+    unit_rows = p.unit_rows;
   }
-  const int n0 = blockIdx.y * kTile;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < k_end; k0 += kStep) {
-    for (int i = threadIdx.x; i < kTile * kStep; i += kBlock) {
-      {
-        const int m = MODE == kWeights ? i % kTile : i / kStep, k = MODE == kWeights ? i / kTile : i % kStep;
-        float v = 0.0f;
-        if (m0 + m < m_end && k0 + k < k_end)
-          v = Num<T>::to_c(MODE == kWeights ? a[(lo + k0 + k) * p.a_ld + m0 + m] : a[(lo + m0 + m) * p.a_ld + k0 + k]);
-        sa[k][m] = v;
+  __device__ __forceinline__ int64_t count(int i) const {
+    const int rows = hi[i] - lo[i];
+    if (MODE != kWeights) return (int64_t)((rows + kBM - 1) / kBM) * n_tiles;
+    return (int64_t)(unit_rows ? (rows + unit_rows - 1) / unit_rows : 1) * m_tiles * n_tiles;
+  }
+  __device__ __forceinline__ bool next(Tile& v) {
+    int64_t c = 0;
+    while (e < experts && t >= base + (c = count(e))) {
+      base += c;
+      ++e;
+    }
+    if (e >= experts) return false;
+    int64_t local = t - base;
+    t += gridDim.x;
+    v.e = e;
+    v.lo = lo[e];
+    v.hi = hi[e];
+    if (MODE != kWeights) {
+      const int m = (v.hi - v.lo + kBM - 1) / kBM;
+      v.n0 = (int)(local / m) * BN;
+      v.m0 = (int)(local % m) * kBM;
+      v.k_blocks = k_blocks;
+    } else {
+      const int per = m_tiles * n_tiles;
+      const int unit = (int)(local / per), i = (int)(local % per);
+      v.m0 = i % m_tiles * kBM;
+      v.n0 = i / m_tiles * BN;
+      v.slot = base / per + unit;
+      if (unit_rows) {
+        v.lo += unit * unit_rows;
+        v.hi = min(v.hi, v.lo + unit_rows);
       }
-      {
-        const int n = MODE == kRows ? i / kStep : i % kTile, k = MODE == kRows ? i % kStep : i / kTile;
-        float v = 0.0f;
-        if (n0 + n < n_end && k0 + k < k_end) {
-          if (MODE == kForward) v = Num<T>::to_c(b[e * p.b_stride + (int64_t)(k0 + k) * p.b_ld + n0 + n]);
-          if (MODE == kRows) v = Num<T>::to_c(b[e * p.b_stride + (int64_t)(n0 + n) * p.b_ld + k0 + k]);
-          if (MODE == kWeights) v = Num<T>::to_c(b[(lo + k0 + k) * p.b_ld + n0 + n]);
+      v.k_blocks = (v.hi - v.lo + kBK - 1) / kBK;
+    }
+    return true;
+  }
+};
+
+// The sum of one output element straight from the fp32 operands: taken where the
+// split parts gave NaN, because an infinite value times another's zero part is
+// NaN where the plain product is infinite.
+template <int MODE>
+__device__ __noinline__ float plain_sum(const Args& p, int e, int lo, int hi, int m, int n) {
+  const float* a = static_cast<const float*>(p.a);
+  const float* b = static_cast<const float*>(p.b);
+  float s = 0.0f;
+  if (MODE == kForward)
+    for (int k = 0; k < p.inputs; ++k)
+      s = fmaf(a[(int64_t)(lo + m) * p.a_ld + k], b[e * p.b_stride + (int64_t)k * p.b_ld + n], s);
+  if (MODE == kRows)
+    for (int k = 0; k < p.outputs; ++k)
+      s = fmaf(a[(int64_t)(lo + m) * p.a_ld + k], b[e * p.b_stride + (int64_t)n * p.b_ld + k], s);
+  if (MODE == kWeights)
+    for (int64_t r = lo; r < hi; ++r) s = fmaf(a[r * p.a_ld + m], b[r * p.b_ld + n], s);
+  return s;
+}
+
+// Sigmoid family for results that are rounded to 16 bits: exp and the
+// reciprocal by the fast units, each within 2^-21 of its value.
+__device__ __forceinline__ float fast_sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+
+template <class T, int KIND>
+__device__ __forceinline__ void activate32(float (&v)[32], int flags, float s0, float s1) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    if constexpr (sizeof(T) == 2 && KIND == EPI_SILU) v[i] = __fdividef(v[i], 1.0f + __expf(-v[i]));
+    else if constexpr (sizeof(T) == 2 && KIND == EPI_SIGMOID) v[i] = fast_sigmoid(v[i]);
+    else v[i] = activation<float>(KIND, flags, v[i], s0, s1);
+  }
+}
+template <class T>
+__device__ __forceinline__ void activate_all(float (&v)[32], int kind, int flags, float s0, float s1) {
+  switch (kind) {
+    case EPI_NONE: return;
+    case EPI_RELU: return activate32<T, EPI_RELU>(v, flags, s0, s1);
+    case EPI_GELU: return activate32<T, EPI_GELU>(v, flags, s0, s1);
+    case EPI_SILU: return activate32<T, EPI_SILU>(v, flags, s0, s1);
+    case EPI_SIGMOID: return activate32<T, EPI_SIGMOID>(v, flags, s0, s1);
+    default:
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i)  // the rarer ones share one loop of 8 values to keep the kernel small
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float x = 0.0f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) x = q == i ? v[8 * q + j] : x;
+          x = activation<float>(kind, flags, x, s0, s1);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[8 * q + j] = q == i ? x : v[8 * q + j];
         }
-        sb[k][n] = v;
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kStep; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][ty + 16 * i], sb[k][tx + 16 * j], acc[i][j]);
-    __syncthreads();
   }
+}
+
+// 32 columns of this warp's 32 rows (one row a lane) to global memory through
+// the warp's staging rows: 64 contiguous bytes of a row at a time.
+template <class O>
+__device__ __forceinline__ void store_rows(const float (&v)[32], unsigned char* stage, O* c, int64_t ld, int m_valid,
+                                           int n_valid, bool vec) {
+  constexpr int kCols = 64 / sizeof(O), kPasses = 32 / kCols, kPer = 16 / sizeof(O);
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int pass = 0; pass < kPasses; ++pass) {
+    alignas(16) O o[kCols];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + ty + 16 * i;
-      const int n = n0 + tx + 16 * j;
-      if (m >= m_end || n >= n_end) continue;
-      float v = acc[i][j];
-      if (MODE == kForward && e < p.experts) {
-        if (p.bias) v += Num<T>::to_c(static_cast<const T*>(p.bias)[(int64_t)e * p.outputs + n]);
-        v = activation<float>(p.act, p.act_flags, v, p.s0, p.s1);
+    for (int i = 0; i < kCols; ++i) o[i] = Num<O>::from_c(v[pass * kCols + i]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      reinterpret_cast<uint4*>(stage + lane * kEpiPitch)[i] = reinterpret_cast<const uint4*>(o)[i];
+    __syncwarp();
+    const int col0 = pass * kCols;
+    if (vec && col0 + kCols <= n_valid) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2), ch = lane & 3;
+        const uint4 u = *reinterpret_cast<const uint4*>(stage + r * kEpiPitch + ch * 16);
+        if (r < m_valid) *reinterpret_cast<uint4*>(c + r * ld + col0 + ch * kPer) = u;
       }
-      if (MODE == kWeights) c[((int64_t)e * p.inputs + m) * p.outputs + n] = Num<T>::from_c(v);
-      else c[(lo + m) * p.c_ld + n] = Num<T>::from_c(v);
+    } else {
+#pragma unroll 4
+      for (int i = 0; i < kCols; ++i) {
+        const int r = i * (32 / kCols) + lane / kCols, col = lane % kCols;
+        const O u = reinterpret_cast<const O*>(stage + r * kEpiPitch)[col];
+        if (r < m_valid && col0 + col < n_valid) c[r * ld + col0 + col] = u;
+      }
     }
+    __syncwarp();
+  }
+}
+
+template <class T, int MODE, int P, int BN>
+__global__ void __launch_bounds__(kBlock, 1)
+    product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Args p) {
+  using S = Shape<T, P, BN>;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint64_t bars[2 * kMaxStages + 2 * 4 + 1];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  unsigned char* base_ptr = smem_raw + (base - raw);
+  unsigned char* epi = base_ptr + p.stages * S::stage_bytes;
+  float* bias_s = reinterpret_cast<float*>(epi + kEpiBytes);
+  int* lo = reinterpret_cast<int*>(epi + kEpiBytes + kBiasBytes);
+  int* hi = lo + p.experts;
+  const uint32_t bar0 = smem_u32(bars);
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto empty = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
+  auto acc_full = [&](int b) { return bar0 + 8u * (2 * kMaxStages + b); };
+  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * kMaxStages + 4 + b); };
+  const uint32_t drain = bar0 + 8u * (2 * kMaxStages + 8);
+  volatile int* abort_flag = &abort_word;
+
+  ops::let_successor_start();
+  if (tid == 0) {
+    abort_word = 0;
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int b = 0; b < S::acc_bufs; ++b) {
+      mbar_init(acc_full(b), 1);
+      mbar_init(acc_empty(b), kEpiWarps);
+    }
+    mbar_init(drain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    fence_proxy_async();
+  }
+  if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), 512);
+  ops::wait_for_predecessor();
+  for (int e = tid; e < p.experts; e += kBlock) {
+    const int l = clamped(p.offset[e], 0, p.rows);
+    lo[e] = l;
+    hi[e] = clamped(p.offset[e + 1], l, p.rows);
+  }
+  if (blockIdx.x == 0) check_offsets(p.offset, p.experts, p.rows, p.error);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  Tiles<MODE, BN> tiles(p, lo, hi);
+  Tile v;
+  int64_t issued = 0;  // stages filled so far (thread 0)
+  if (warp == 0) {
+    // ------------------------------------------------------- producer ----
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 1;  // empty barriers: the first pass finds them free
+      bool ok = true;
+      while (ok && tiles.next(v)) {
+        for (int kb = 0; kb < v.k_blocks; ++kb) {
+          if (!wait_phase_abort(empty(s), ph, abort_flag, PONNI_B200_WAIT_LIMIT)) {
+            ok = false;
+            break;
+          }
+          const uint32_t a = base + (uint32_t)s * S::stage_bytes, b = a + S::a_bytes;
+          mbar_expect_tx(full(s), S::stage_bytes);
+          const int k0 = kb * kBK;
+#pragma unroll
+          for (int q = 0; q < P; ++q) {
+            if (MODE != kWeights) {
+              tma_load_3d(a + q * (kBM * kBK * 2), &map_a, k0, v.lo + v.m0, q, full(s));
+            } else {
+#pragma unroll
+              for (int j = 0; j < kBM / 64; ++j)
+                tma_load_3d(a + q * (kBM * kBK * 2) + j * 8192, &map_a, v.m0 + 64 * j, v.lo + k0, q, full(s));
+            }
+            if (MODE == kRows) {
+              tma_load_3d(b + q * (BN * kBK * 2), &map_b, k0, v.n0, q * p.experts + v.e, full(s));
+            } else {
+#pragma unroll
+              for (int j = 0; j < BN / 64; ++j) {
+                if (MODE == kForward)
+                  tma_load_3d(b + q * (BN * kBK * 2) + j * 8192, &map_b, v.n0 + 64 * j, k0, q * p.experts + v.e, full(s));
+                else
+                  tma_load_3d(b + q * (BN * kBK * 2) + j * 8192, &map_b, v.n0 + 64 * j, v.lo + k0, q, full(s));
+              }
+            }
+          }
+          ++issued;
+          if (++s == p.stages) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      if (!ok) atomicOr(p.error, 1);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA ----
+    constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
+    constexpr bool a_mn = MODE == kWeights, b_mn = MODE != kRows;
+    constexpr uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((a_mn ? 1u : 0u) << 15) |
+                               ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
+    // MN-major: 64-element chunks 8192 bytes apart (leading offset), groups of
+    // 8 k 1024 apart; K-major: rows of 128 bytes, groups of 8 rows 1024 apart.
+    const uint64_t da = smem_desc(base, a_mn ? 8192 : 16, 1024), db = smem_desc(base, b_mn ? 8192 : 16, 1024);
+    const uint32_t a_hi = (uint32_t)(da >> 32), b_hi = (uint32_t)(db >> 32), a_lo0 = (uint32_t)da, b_lo0 = (uint32_t)db;
+    constexpr uint32_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;  // 16 k further, in 16-byte units
+    int s = 0, buf = 0;
+    uint32_t ph = 0, acc_ph = 1;
+    bool ok = true, skip = PONNI_B200_SKIP_ARRIVE();
+    while (ok && tiles.next(v)) {
+      for (int kb = 0; kb < v.k_blocks; ++kb) {
+        const uint32_t d = tmem + (uint32_t)(buf * S::acc_cols);
+        if (P == 3 || kb == 0) {
+          ok = wait_phase_abort(acc_empty(buf), acc_ph, abort_flag, PONNI_B200_WAIT_LIMIT);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
+        ok = wait_phase_abort(full(s), ph, abort_flag, PONNI_B200_WAIT_LIMIT);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t stage = (uint32_t)s * S::stage_bytes;
+        if (MODE == kWeights && kb == v.k_blocks - 1) {
+          const int valid = v.hi - v.lo - kb * kBK;
+          if (valid < kBK) {  // rows of the next group: not part of this sum
+            for (int ch = 0; ch < S::stage_bytes / 8192; ++ch)
+              for (int i = valid * 8 + lane; i < kBK * 8; i += 32)
+                *reinterpret_cast<uint4*>(base_ptr + stage + ch * 8192 + i * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async();
+            __syncwarp();
+          }
+        }
+        const uint32_t a0 = a_lo0 + (stage >> 4), b0 = b_lo0 + ((stage + S::a_bytes) >> 4);
+        if constexpr (P == 1) {
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k)
+            umma_f16_desc_warp(d, a0 + k * a_step, a_hi, b0 + k * b_step, b_hi, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+        } else {
+          constexpr uint32_t ap = kBM * kBK * 2 / 16, bp = BN * kBK * 2 / 16;
+          constexpr int qa[6] = {1, 0, 2, 0, 1, 0}, qb[6] = {1, 2, 0, 1, 0, 0};
+#pragma unroll
+          for (int q = 0; q < 6; ++q)
+#pragma unroll
+            for (int k = 0; k < kBK / 16; ++k)
+              umma_f16_desc_warp(d, a0 + qa[q] * ap + k * a_step, a_hi, b0 + qb[q] * bp + k * b_step, b_hi, idesc,
+                                 (q > 0 || k > 0) ? 1u : 0u);
+        }
+        umma_commit_warp(empty(s));
+        if (P == 3 || kb == v.k_blocks - 1) {
+          if (!skip) umma_commit_warp(acc_full(buf));
+          skip = false;
+          if (++buf == S::acc_bufs) {
+            buf = 0;
+            acc_ph ^= 1u;
+          }
+        }
+        if (++s == p.stages) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+    }
+    if (!ok) {
+      if (lane == 0) atomicOr(p.error, 1);
+      umma_commit_warp(drain);  // the MMAs issued so far, before TMEM is freed
+      (void)mbar_wait_bounded(drain, 0);
+    }
+  } else {
+    // ------------------------------------------------------- epilogue ----
+    const int quarter = warp & 3, half = (warp - 2) >> 2, w = warp - 2;
+    constexpr int kHalf = BN / 2, kChunks = kHalf / 32;
+    unsigned char* stage = epi + w * 32 * kEpiPitch;
+    float* bias_w = bias_s + w * 128;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const int n_end = MODE == kRows ? p.inputs : p.outputs;
+    int buf = 0;
+    uint32_t acc_ph = 0;
+    bool ok = true;
+    auto wait_acc = [&]() -> bool {
+      int got = 0;
+      if (lane == 0) got = wait_phase_abort(acc_full(buf), acc_ph, abort_flag, PONNI_B200_WAIT_LIMIT) ? 1 : 0;
+      got = __shfl_sync(0xffffffffu, got, 0);
+      tc_fence_after();
+      return got != 0;
+    };
+    auto release_acc = [&]() {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty(buf));
+      if (++buf == S::acc_bufs) {
+        buf = 0;
+        acc_ph ^= 1u;
+      }
+    };
+    while (ok && tiles.next(v)) {
+      const int m_end = MODE == kWeights ? p.inputs : v.hi - v.lo;
+      const int row0 = v.m0 + quarter * 32, m_valid = min(32, m_end - row0);
+      const int col0 = v.n0 + half * kHalf;
+      if (MODE == kForward && p.bias) {
+        const T* bias = static_cast<const T*>(p.bias) + (int64_t)v.e * p.outputs;
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+          const int n = col0 + i * 32 + lane;
+          bias_w[i * 32 + lane] = n < n_end ? Num<T>::to_c(bias[n]) : 0.0f;
+        }
+        __syncwarp();
+      }
+      auto finish = [&](float (&x)[32], int c) {
+        const int n = col0 + c * 32, n_valid = n_end - n;
+        if constexpr (P == 3) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (x[i] != x[i] && lane < m_valid && i < n_valid) x[i] = plain_sum<MODE>(p, v.e, v.lo, v.hi, row0 + lane, n + i);
+        }
+        if (MODE == kForward) {
+          if (p.bias) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 b = *reinterpret_cast<const float4*>(bias_w + c * 32 + i);
+              x[i] += b.x;
+              x[i + 1] += b.y;
+              x[i + 2] += b.z;
+              x[i + 3] += b.w;
+            }
+          }
+          activate_all<T>(x, p.act, p.act_flags, p.s0, p.s1);
+        }
+        if (n_valid <= 0 || m_valid <= 0) return;
+        if (MODE == kWeights) {
+          if (p.unit_rows)
+            store_rows<float>(x, stage, p.partial + (v.slot * p.inputs + row0) * p.outputs + n, p.outputs, m_valid,
+                              n_valid, p.vec);
+          else
+            store_rows<T>(x, stage, static_cast<T*>(p.c) + ((int64_t)v.e * p.inputs + row0) * p.outputs + n, p.outputs,
+                          m_valid, n_valid, p.vec);
+        } else {
+          store_rows<T>(x, stage, static_cast<T*>(p.c) + (int64_t)(v.lo + row0) * p.c_ld + n, p.c_ld, m_valid, n_valid,
+                        p.vec);
+        }
+      };
+      if (P == 1 && v.k_blocks > 0) {
+        if (!(ok = wait_acc())) break;
+        const uint32_t t = tmem + lane_base + (uint32_t)(buf * S::acc_cols + half * kHalf);
+#pragma unroll 1
+        for (int c = 0; c < kChunks; ++c) {
+          float x[32];
+          tmem_ld32(t + c * 32, x);
+          if (c == kChunks - 1) release_acc();
+          finish(x, c);
+        }
+      } else {
+        float acc[kChunks][32] = {};
+        if constexpr (P == 3) {
+          for (int kb = 0; kb < v.k_blocks; ++kb) {
+            if (!(ok = wait_acc())) break;
+            const uint32_t t = tmem + lane_base + (uint32_t)(buf * S::acc_cols + half * kHalf);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+              float x[32];
+              tmem_ld32(t + c * 32, x);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) acc[c][i] += x[i];
+            }
+            release_acc();
+          }
+          if (!ok) break;
+        }
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) finish(acc[c], c);
+      }
+    }
+    if (!ok && lane == 0) atomicOr(p.error, 1);
+  }
+  if (MODE != kWeights) {
+    // Rows in no group.
+    const int64_t used = clamped(p.offset[p.experts], 0, p.rows);
+    const int n_end = MODE == kRows ? p.inputs : p.outputs;
+    T* c = static_cast<T*>(p.c);
+    for (int64_t r = used + blockIdx.x; r < p.rows; r += gridDim.x)
+      for (int n = tid; n < n_end; n += kBlock) c[r * p.c_ld + n] = Num<T>::from_c(0.0f);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *abort_flag) {
+    // A role gave up: wait (bounded) for the copies in flight before the CTA ends.
+    for (int64_t i = issued > p.stages ? issued - p.stages : 0; i < issued; ++i)
+      if (!mbar_wait_bounded(full((int)(i % p.stages)), (uint32_t)(i / p.stages) & 1u)) break;
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// d_W_e = sum of its units' partial sums, in order.
+template <class T>
+__global__ void __launch_bounds__(256)
+    sum_units_kernel(const float* __restrict__ partial, T* __restrict__ c, const int* __restrict__ offset, int experts,
+                     int64_t rows, int unit_rows, int64_t per_expert) {
+  __shared__ int64_t first_s;
+  ops::wait_for_predecessor();
+  const int e = blockIdx.y;
+  auto units = [&](int i) {
+    const int l = clamped(offset[i], 0, rows);
+    return (clamped(offset[i + 1], l, rows) - l + unit_rows - 1) / unit_rows;
+  };
+  if (threadIdx.x < 32) {
+    int64_t n = 0;
+    for (int i = threadIdx.x; i < e; i += 32) n += units(i);
+    for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
+    if (threadIdx.x == 0) first_s = n;
+  }
+  __syncthreads();
+  const int n = units(e);
+  const float* src = partial + first_s * per_expert;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < per_expert; i += (int64_t)gridDim.x * 256) {
+    float s = 0.0f;
+#pragma unroll 4
+    for (int u = 0; u < n; ++u) s += src[u * per_expert + i];
+    c[e * per_expert + i] = Num<T>::from_c(s);
+  }
 }
 
 // Column sums of an expert's rows.
 template <class T>
-__global__ void __launch_bounds__(kBlock)
-    simple_bias_kernel(const T* __restrict__ d, int64_t ld, int64_t rows, const int* __restrict__ offset, int experts,
-                       int outputs, T* __restrict__ out) {
-  __shared__ float part[kBlock / 32][32];
+__global__ void __launch_bounds__(256)
+    bias_gradient_kernel(const T* __restrict__ d, int64_t ld, int64_t rows, const int* __restrict__ offset, int experts,
+                         int outputs, T* __restrict__ out) {
+  __shared__ float part[8][32];
   const int e = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockIdx.x * 32 + lane;
-  int64_t lo, hi;
-  group_of(offset, experts, e, rows, lo, hi);
+  const int lo = clamped(offset[e], 0, rows), hi = clamped(offset[e + 1], lo, rows);
   float s = 0.0f;
   if (n < outputs)
-    for (int64_t r = lo + warp; r < hi; r += kBlock / 32) s += Num<T>::to_c(d[r * ld + n]);
+    for (int64_t r = lo + warp; r < hi; r += 8) s += Num<T>::to_c(d[r * ld + n]);
   part[warp][lane] = s;
   __syncthreads();
   if (warp == 0 && n < outputs) {
     float t = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kBlock / 32; ++w) t += part[w][lane];
+    for (int w = 0; w < 8; ++w) t += part[w][lane];
     out[(int64_t)e * outputs + n] = Num<T>::from_c(t);
   }
 }
 
+// ------------------------------------------------------------- staging ----
+// An operand that the copy engine cannot read (fp32, or a base or stride off
+// the 16-byte grid) is laid out in the workspace first: rows of `pitch`
+// elements, fp32 as three bf16 planes.
+struct Stage {
+  const void* src;
+  void* dst;
+  int64_t rows, ld, group_rows, group_stride;  // source row r: (r / group_rows) * group_stride + (r % group_rows) * ld
+  int cols, pitch;
+};
+struct Stages {
+  Stage s[3];
+  int n;
+};
+
+// split3 of finite values; infinities and NaN stay whole in the first part.
+__device__ __forceinline__ void split_any(float x, uint32_t& h0, uint32_t& h1, uint32_t& h2) {
+  split3(x, h0, h1, h2);
+  if ((__float_as_uint(x) & 0x7F800000u) == 0x7F800000u) {
+    h0 = x != x ? 0x7FC00000u : h0;
+    h1 = h2 = 0u;
+  }
+}
+
 template <class T>
-ponni_b200_status launch_simple(int mode, const Args& p, cudaStream_t s) {
-  const int64_t row_tiles = (p.rows + kTile - 1) / kTile + p.experts + 1;
-  auto tiles = [](int n) { return (unsigned)((n + kTile - 1) / kTile); };
-  if (tiles(p.inputs) > 65535 || tiles(p.outputs) > 65535)
-    return ops::fail(PONNI_B200_ERR_UNSUPPORTED, "expert_product: too many inputs or outputs");
-  if (mode == kForward)
-    simple_kernel<T, kForward><<<dim3((unsigned)row_tiles, tiles(p.outputs)), kBlock, 0, s>>>(p);
-  else if (mode == kRows)
-    simple_kernel<T, kRows><<<dim3((unsigned)row_tiles, tiles(p.inputs)), kBlock, 0, s>>>(p);
-  else
-    simple_kernel<T, kWeights><<<dim3(tiles(p.inputs), tiles(p.outputs), p.experts), kBlock, 0, s>>>(p);
-  return ops::launched("expert_product");
+__global__ void __launch_bounds__(256) stage_kernel(const Stages all) {
+  ops::let_successor_start();
+  ops::wait_for_predecessor();
+  const Stage& s = all.s[blockIdx.y];
+  const int vecs = s.pitch / 8;
+  int tx = 1;
+  while (tx < vecs && tx < 256) tx *= 2;
+  const int x = threadIdx.x % tx, y = threadIdx.x / tx, ty = 256 / tx;
+  const int64_t plane = s.rows * (int64_t)s.pitch;
+  for (int64_t r = blockIdx.x * (int64_t)ty + y; r < s.rows; r += (int64_t)gridDim.x * ty) {
+    const T* src = static_cast<const T*>(s.src) +
+                   (s.group_rows == s.rows ? r * s.ld : r / s.group_rows * s.group_stride + r % s.group_rows * s.ld);
+    for (int c = x; c < vecs; c += tx) {
+      T v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = c * 8 + i < s.cols ? src[c * 8 + i] : Num<T>::from_c(0.0f);
+      if constexpr (sizeof(T) == 4) {
+        uint32_t h[3][8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) split_any(v[i], h[0][i], h[1][i], h[2][i]);
+        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(s.dst) + r * s.pitch + c * 8;
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+          *reinterpret_cast<uint4*>(dst + q * plane) = make_uint4(pack_hi16(h[q][0], h[q][1]), pack_hi16(h[q][2], h[q][3]),
+                                                                  pack_hi16(h[q][4], h[q][5]), pack_hi16(h[q][6], h[q][7]));
+      } else {
+        alignas(16) T o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = v[i];
+        *reinterpret_cast<uint4*>(static_cast<T*>(s.dst) + r * s.pitch + c * 8) = *reinterpret_cast<uint4*>(o);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host ----
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled() {
+  static EncodeTiledFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      f = nullptr;
+    }
+    return reinterpret_cast<EncodeTiledFn>(f);
+  }();
+  return fn;
+}
+
+// An operand as the tensor maps describe it: [depth][rows][cols] of 16-bit
+// elements (depth: planes, experts, or planes of experts).
+struct Operand {
+  const void* p;
+  int64_t ld, stride;  // elements
+  int64_t cols, rows, depth;
+};
+
+ponni_b200_status make_map(CUtensorMap& map, const Operand& o, bool half, int box_rows) {
+  EncodeTiledFn enc = encode_tiled();
+  if (!enc) return ops::fail(PONNI_B200_ERR_CUDA, "expert_product: the driver has no tensor maps");
+  const cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.depth};
+  const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(o.depth > 1 ? o.stride : o.ld) * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  if (strides[0] >= (1ull << 40) || strides[1] >= (1ull << 40) ||
+      enc(&map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.p),
+          dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return ops::fail(PONNI_B200_ERR_UNSUPPORTED, "expert_product: operand sizes or strides beyond the copy engine's");
+  return PONNI_B200_OK;
+}
+
+bool on_grid(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * 2 % 16 == 0; }
+
+int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+int64_t pad256(int64_t n) { return (n + 255) / 256 * 256; }
+int64_t staged_bytes(int dtype, int64_t rows, int cols) {
+  return pad256(rows * pad8(cols) * (dtype == PONNI_B200_F32 ? 6 : 2));
+}
+
+// Rows of a unit of d_W: whole groups where those fill the SMs twice, else
+// units small enough for about four tiles an SM (the tail of uneven groups),
+// 1024 rows at least (a unit's partial sums cost 8 bytes an element of W_e).
+int unit_rows_of(int64_t rows, int experts, int inputs, int outputs, int sms) {
+  const int64_t per = (int64_t)((inputs + kBM - 1) / kBM) * ((outputs + 255) / 256);
+  if (per * experts >= 2 * sms || rows <= 1024) return 0;
+  const int64_t unit = std::max<int64_t>(1024, (rows * per / (4 * sms) + kBK - 1) / kBK * kBK);
+  return unit < rows ? (int)std::min<int64_t>(unit, 1 << 30) : 0;
+}
+int64_t partial_bytes(int64_t rows, int experts, int inputs, int outputs, int sms) {
+  const int unit = unit_rows_of(rows, experts, inputs, outputs, sms);
+  return unit ? pad256((rows / unit + experts) * (int64_t)inputs * outputs * 4) : 0;
+}
+
+// Hands out the caller's workspace.
+struct Space {
+  char* at;
+  int64_t left;
+  void* take(int64_t bytes) {
+    if (bytes > left || !at) return nullptr;
+    void* p = at;
+    at += bytes;
+    left -= bytes;
+    return p;
+  }
+};
+
+template <class T, int MODE, int P, int BN>
+ponni_b200_status launch_shape(const Operand& a, const Operand& b, Args p, int sms, int64_t tiles, cudaStream_t stream) {
+  using S = Shape<T, P, BN>;
+  CUtensorMap map_a, map_b;
+  constexpr bool half = std::is_same<T, __half>::value;
+  ponni_b200_status st = make_map(map_a, a, half, MODE == kWeights ? 64 : kBM);
+  if (!st) st = make_map(map_b, b, half, MODE == kRows ? BN : 64);
+  if (st) return st;
+  const int fixed = 1024 + kEpiBytes + kBiasBytes + 2 * p.experts * (int)sizeof(int) + 512;
+  p.stages = std::min(kMaxStages, (kSmemLimit - fixed) / S::stage_bytes);
+  const int smem = 1024 + p.stages * S::stage_bytes + kEpiBytes + kBiasBytes + 2 * p.experts * (int)sizeof(int);
+  auto kern = product_kernel<T, MODE, P, BN>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess)
+    e = ops::launch_after(kern, dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(sms, tiles))), dim3(kBlock),
+                          (size_t)smem, stream, map_a, map_b, p);
+  return e == cudaSuccess ? PONNI_B200_OK : ops::fail_cuda(e, "expert_product");
+}
+
+// Tile width: the widest whose padding costs at most an eighth more columns.
+int tile_width(int n, int most) {
+  auto padded = [&](int w) { return (int64_t)(n + w - 1) / w * w; };
+  int w = most;
+  while (w > 64 && padded(w) * 8 > padded(64) * 9) w /= 2;
+  return w;
+}
+
+template <class T, int MODE>
+ponni_b200_status launch_product(const Operand& a, const Operand& b, const Args& p, int sms, cudaStream_t stream) {
+  constexpr int P = sizeof(T) == 4 ? 3 : 1;
+  const int n = MODE == kRows ? p.inputs : p.outputs;
+  const int w = tile_width(n, P == 3 ? 128 : 256);
+  const int64_t m_tiles = MODE == kWeights
+                              ? (int64_t)((p.inputs + kBM - 1) / kBM) * (p.experts + (p.unit_rows ? p.rows / p.unit_rows : 0))
+                              : p.rows / kBM + std::min<int64_t>(p.experts, p.rows);
+  const int64_t tiles = m_tiles * ((n + w - 1) / w);
+  if (w == 64) return launch_shape<T, MODE, P, 64>(a, b, p, sms, tiles, stream);
+  if (w == 128) return launch_shape<T, MODE, P, 128>(a, b, p, sms, tiles, stream);
+  if constexpr (P == 1) return launch_shape<T, MODE, P, 256>(a, b, p, sms, tiles, stream);
+  return ops::fail(PONNI_B200_ERR_UNSUPPORTED, "expert_product: no tile shape");
 }
 
 template <class F>
@@ -181,14 +796,43 @@ ponni_b200_status check_product(const std::string& at, int dtype, const void* ro
   if (!is_real_type(dtype)) return fail(PONNI_B200_ERR_UNSUPPORTED, at + ": values must be fp32, fp16 or bf16");
   if (experts < 1 || experts > kMaxExperts)
     return fail(PONNI_B200_ERR_UNSUPPORTED, at + ": the number of experts must be 1 to 1024");
-  if (inputs < 1 || outputs < 1) return fail(PONNI_B200_ERR_INVALID_ARGUMENT, at + ": needs inputs and outputs");
-  if (num_rows < 0 || num_rows > INT32_MAX)
-    return fail(PONNI_B200_ERR_INVALID_ARGUMENT, at + ": the number of rows must be below 2^31");
+  if (inputs < 1 || outputs < 1 || inputs > (1 << 24) || outputs > (1 << 24))
+    return fail(PONNI_B200_ERR_INVALID_ARGUMENT, at + ": inputs and outputs must be 1 to 2^24");
+  if (num_rows < 0 || num_rows > INT32_MAX - 65536)
+    return fail(PONNI_B200_ERR_INVALID_ARGUMENT, at + ": the number of rows must be below 2^31 - 65536");
   if ((num_rows > 0 && !rows) || !weights || !offset)
     return fail(PONNI_B200_ERR_INVALID_ARGUMENT, at + ": pointer is NULL");
-  if (rows_ld < inputs || w_ld < outputs || (experts > 1 && w_stride < (int64_t)inputs * w_ld - (w_ld - outputs)))
+  if (rows_ld < inputs || w_ld < outputs || (experts > 1 && w_stride < (int64_t)(inputs - 1) * w_ld + outputs))
     return fail(PONNI_B200_ERR_INVALID_ARGUMENT, at + ": stride smaller than the row or the expert");
   return PONNI_B200_OK;
+}
+
+// The operand as the product reads it: in place, or through the workspace.
+ponni_b200_status operand(Operand& o, Stages& stages, Space& space, int dtype, const void* p, int64_t ld, int64_t stride,
+                          int64_t rows, int cols, int64_t depth) {
+  const int planes = dtype == PONNI_B200_F32 ? 3 : 1;
+  if (planes == 1 && on_grid(p, ld) && (depth == 1 || stride % 8 == 0)) {
+    o = {p, ld, stride, cols, rows, depth};
+    return PONNI_B200_OK;
+  }
+  const int64_t pitch = pad8(cols);
+  void* dst = space.take(staged_bytes(dtype, rows * depth, cols));
+  if (!dst) return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "expert_product: workspace is too small");
+  o = {dst, pitch, rows * pitch, cols, rows, depth * planes};
+  stages.s[stages.n++] = {p, dst, rows * depth, ld, rows, stride, cols, (int)pitch};
+  return PONNI_B200_OK;
+}
+
+template <class T>
+ponni_b200_status run_stages(const Stages& st, int sms, cudaStream_t s) {
+  if (!st.n) return PONNI_B200_OK;
+  int64_t most = 1;
+  for (int i = 0; i < st.n; ++i) {
+    const int64_t per = std::max<int64_t>(1, 256 / std::max(1, st.s[i].pitch / 8));
+    most = std::max(most, (st.s[i].rows + per - 1) / per);
+  }
+  stage_kernel<T><<<dim3((unsigned)std::min<int64_t>(most, sms * 8), st.n), 256, 0, s>>>(st);
+  return ops::launched("expert_product");
 }
 
 }  // namespace
@@ -199,9 +843,15 @@ using namespace ponni_b200;
 extern "C" {
 
 int64_t ponni_b200_expert_product_workspace(int dtype, int64_t num_rows, int experts, int inputs, int outputs,
-                                            int backward) {
-  (void)dtype; (void)num_rows; (void)experts; (void)inputs; (void)outputs; (void)backward;
-  return 0;
+                                            int aligned, int backward, int device) {
+  if (num_rows < 0 || experts < 1 || inputs < 1 || outputs < 1) return 0;
+  int64_t n = 0;
+  if (dtype == PONNI_B200_F32 || !aligned) {
+    n += staged_bytes(dtype, num_rows, inputs) + staged_bytes(dtype, (int64_t)experts * inputs, outputs);
+    if (backward) n += staged_bytes(dtype, num_rows, outputs);
+  }
+  if (backward) n += partial_bytes(num_rows, experts, inputs, outputs, ops::num_sms(device));
+  return n;
 }
 
 ponni_b200_status ponni_b200_expert_product(int dtype, const void* rows, int64_t rows_ld, int64_t num_rows,
@@ -220,10 +870,40 @@ ponni_b200_status ponni_b200_expert_product(int dtype, const void* rows, int64_t
     if (!out) return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "expert_product: pointer is NULL");
     if (out_ld < outputs)
       return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "expert_product: stride smaller than the row");
-    Args p = {rows, weights, out, rows_ld, w_ld, w_stride, out_ld, num_rows, offset, bias, experts, inputs, outputs,
-              activation < 0 ? EPI_NONE : activation, activation_flags, (float)scalar0, (float)scalar1, ops::error_word(device)};
+    Args p = {};
+    p.a = rows;
+    p.b = weights;
+    p.c = out;
+    p.a_ld = rows_ld;
+    p.b_ld = w_ld;
+    p.b_stride = w_stride;
+    p.c_ld = out_ld;
+    p.rows = num_rows;
+    p.offset = offset;
+    p.bias = bias;
+    p.experts = experts;
+    p.inputs = inputs;
+    p.outputs = outputs;
+    p.act = activation < 0 ? EPI_NONE : activation;
+    p.act_flags = activation_flags;
+    p.s0 = (float)scalar0;
+    p.s1 = (float)scalar1;
+    p.error = ops::error_word(device);
     if (!p.error) return ops::fail(PONNI_B200_ERR_CUDA, "no operator error word on this device");
-    return by_type(dtype, [&](auto t) { return launch_simple<decltype(t)>(kForward, p, static_cast<cudaStream_t>(stream)); });
+    const int sms = ops::num_sms(device);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    Stages stages = {};
+    Space space = {static_cast<char*>(workspace), workspace_bytes};
+    Operand a, b;
+    st = operand(a, stages, space, dtype, rows, rows_ld, 0, num_rows, inputs, 1);
+    if (!st) st = operand(b, stages, space, dtype, weights, w_ld, w_stride, inputs, outputs, experts);
+    if (st) return st;
+    return by_type(dtype, [&](auto t) -> ponni_b200_status {
+      using T = decltype(t);
+      p.vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_ld * sizeof(T) % 16 == 0;
+      ponni_b200_status r = run_stages<T>(stages, sms, s);
+      return r ? r : launch_product<T, kForward>(a, b, p, sms, s);
+    });
   });
 }
 
@@ -241,24 +921,75 @@ ponni_b200_status ponni_b200_expert_product_backward(int dtype, const void* d_ou
       return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "expert_product_backward: pointer is NULL");
     if (d_out_ld < outputs || (d_rows && d_rows_ld < inputs))
       return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "expert_product_backward: stride smaller than the row");
+    const int sms = ops::num_sms(device);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    int* error = ops::error_word(device);
+    if (!error) return ops::fail(PONNI_B200_ERR_CUDA, "no operator error word on this device");
+    if (num_rows == 0) {  // the gradients of experts without rows
+      const size_t z = ops::element_bytes(dtype);
+      cudaError_t e = cudaSuccess;
+      if (d_weights) e = cudaMemsetAsync(d_weights, 0, z * experts * inputs * outputs, s);
+      if (e == cudaSuccess && d_bias) e = cudaMemsetAsync(d_bias, 0, z * experts * outputs, s);
+      return e == cudaSuccess ? PONNI_B200_OK : ops::fail_cuda(e, "expert_product_backward");
+    }
+    Stages stages = {};
+    Space space = {static_cast<char*>(workspace), workspace_bytes};
+    Operand x, w, d;
+    if (d_rows || d_weights) st = operand(d, stages, space, dtype, d_out, d_out_ld, 0, num_rows, outputs, 1);
+    if (!st && d_rows) st = operand(w, stages, space, dtype, weights, w_ld, w_stride, inputs, outputs, experts);
+    if (!st && d_weights) st = operand(x, stages, space, dtype, rows, rows_ld, 0, num_rows, inputs, 1);
+    const int unit = unit_rows_of(num_rows, experts, inputs, outputs, sms);
+    void* partial = nullptr;
+    if (!st && d_weights && unit) {
+      partial = space.take(partial_bytes(num_rows, experts, inputs, outputs, sms));
+      if (!partial) st = ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "expert_product_backward: workspace is too small");
+    }
+    if (st) return st;
     return by_type(dtype, [&](auto t) -> ponni_b200_status {
       using T = decltype(t);
-      Args p = {d_out, weights, d_rows, d_out_ld, w_ld, w_stride, d_rows_ld, num_rows, offset, nullptr, experts, inputs,
-                outputs, EPI_NONE, 0, 0.0f, 0.0f, ops::error_word(device)};
-      if (!p.error) return ops::fail(PONNI_B200_ERR_CUDA, "no operator error word on this device");
-      ponni_b200_status r = PONNI_B200_OK;
-      if (d_rows && num_rows > 0) r = launch_simple<T>(kRows, p, s);
+      Args p = {};
+      p.rows = num_rows;
+      p.offset = offset;
+      p.experts = experts;
+      p.inputs = inputs;
+      p.outputs = outputs;
+      p.error = error;
+      ponni_b200_status r = run_stages<T>(stages, sms, s);
+      if (!r && d_rows) {
+        Args q = p;
+        q.a = d_out;
+        q.a_ld = d_out_ld;
+        q.b = weights;
+        q.b_ld = w_ld;
+        q.b_stride = w_stride;
+        q.c = d_rows;
+        q.c_ld = d_rows_ld;
+        q.vec = reinterpret_cast<uintptr_t>(d_rows) % 16 == 0 && d_rows_ld * sizeof(T) % 16 == 0;
+        r = launch_product<T, kRows>(d, w, q, sms, s);
+      }
       if (!r && d_weights) {
-        p.a = rows;
-        p.a_ld = rows_ld;
-        p.b = d_out;
-        p.b_ld = d_out_ld;
-        p.c = d_weights;
-        r = launch_simple<T>(kWeights, p, s);
+        Args q = p;
+        q.a = rows;
+        q.a_ld = rows_ld;
+        q.b = d_out;
+        q.b_ld = d_out_ld;
+        q.c = d_weights;
+        q.partial = static_cast<float*>(partial);
+        q.unit_rows = unit;
+        const size_t z = unit ? 4 : sizeof(T);
+        q.vec = reinterpret_cast<uintptr_t>(unit ? partial : d_weights) % 16 == 0 && outputs * z % 16 == 0;
+        r = launch_product<T, kWeights>(x, d, q, sms, s);
+        if (!r && unit) {
+          const int64_t per = (int64_t)inputs * outputs;
+          const unsigned blocks = (unsigned)std::min<int64_t>((per + 255) / 256, std::max(1, sms * 8 / experts));
+          const cudaError_t e =
+              ops::launch_after(sum_units_kernel<T>, dim3(blocks, experts), dim3(256), 0, s, (const float*)partial,
+                                static_cast<T*>(d_weights), offset, experts, num_rows, unit, per);
+          if (e != cudaSuccess) r = ops::fail_cuda(e, "expert_product_backward");
+        }
       }
       if (!r && d_bias) {
-        simple_bias_kernel<T><<<dim3((outputs + 31) / 32, experts), kBlock, 0, s>>>(
+        bias_gradient_kernel<T><<<dim3((outputs + 31) / 32, experts), 256, 0, s>>>(
             static_cast<const T*>(d_out), d_out_ld, num_rows, offset, experts, outputs, static_cast<T*>(d_bias));
         r = ops::launched("expert_product_backward");
       }

@@ -270,9 +270,12 @@ def _check_product(rows, weights, offset, what="rows"):
     return code, experts, inputs, outputs, stride, ld
 
 
-def _space(L, code, total, experts, inputs, outputs, backward, dev):
-    """(tensor, bytes) of the product's workspace; the allocator's blocks are 512-byte aligned."""
-    need = L.ponni_b200_expert_product_workspace(code, total, experts, inputs, outputs, backward)
+def _space(L, code, total, experts, inputs, outputs, addresses, strides, backward, dev):
+    """(tensor or None, bytes, address) of the product's workspace; the allocator's blocks are 512-byte aligned."""
+    aligned = code != _abi.F32 and not (sum(a & 15 for a in addresses) or sum(s & 7 for s in strides))
+    if aligned and not backward:
+        return None, 0, None
+    need = L.ponni_b200_expert_product_workspace(code, total, experts, inputs, outputs, aligned, backward, dev.index)
     if not need:
         return None, 0, None
     import torch
@@ -305,9 +308,10 @@ def expert_product(rows, weights, offset, bias=None, activation: Layer | None = 
         kind, flags, s0, s1 = activation.kind, activation.flags, activation.scalar[0], activation.scalar[1]
     out = _row_output(out, total, outputs, rows)
     L = _abi.lib()
-    space, need, at = _space(L, code, total, experts, inputs, outputs, 0, dev)
+    x, w = rows.data_ptr(), weights.data_ptr()
+    space, need, at = _space(L, code, total, experts, inputs, outputs, (x, w), (ld, w_ld, stride), 0, dev)
     _call(L.ponni_b200_expert_product(
-        code, rows.data_ptr(), ld, total, weights.data_ptr(), w_ld, stride,
+        code, x, ld, total, w, w_ld, stride,
         None if bias is None else bias.data_ptr(), offset.data_ptr(), experts, inputs, outputs, kind, flags, s0, s1,
         out.data_ptr(), _matrix(out, "out"), at, need, dev.index, torch_stream_handle(dev)))
     return out
@@ -333,10 +337,11 @@ def expert_product_backward(d_out, rows, weights, offset, bias: bool = True, nee
     d_weights = torch.empty((experts, inputs, outputs), dtype=rows.dtype, device=dev) if need_weights else None
     d_bias = torch.empty((experts, outputs), dtype=rows.dtype, device=dev) if bias else None
     L = _abi.lib()
-    space, need, at = _space(L, code, total, experts, inputs, outputs, 1, dev)
+    d, x, w = d_out.data_ptr(), rows.data_ptr(), weights.data_ptr()
+    d_ld, ld = _matrix(d_out, "d_out"), _matrix(rows, "rows")
+    space, need, at = _space(L, code, total, experts, inputs, outputs, (d, x, w), (d_ld, ld, w_ld, stride), 1, dev)
     _call(L.ponni_b200_expert_product_backward(
-        code, d_out.data_ptr(), _matrix(d_out, "d_out"), rows.data_ptr(), _matrix(rows, "rows"), total,
-        weights.data_ptr(), w_ld, stride, offset.data_ptr(), experts, inputs, outputs,
+        code, d, d_ld, x, ld, total, w, w_ld, stride, offset.data_ptr(), experts, inputs, outputs,
         None if d_rows is None else d_rows.data_ptr(), 0 if d_rows is None else _matrix(d_rows, "d_rows"),
         None if d_weights is None else d_weights.data_ptr(), None if d_bias is None else d_bias.data_ptr(), at, need,
         dev.index, torch_stream_handle(dev)))
