@@ -26,9 +26,12 @@
 // when it accumulates, so long sums in TMEM would drift by a part of 2^-24 for
 // every step.
 //
-// One persistent CTA per SM: a TMA producer, an MMA warp and eight epilogue
+// One persistent CTA per SM: a TMA producer, an MMA warp and sixteen epilogue
 // warps.  Every role walks the same tile sequence, which it derives from the
 // offsets (read once into shared memory): no host copy of the group sizes.
+//
+// A few rows for each expert (serving) are bound by the weights' bytes and by
+// latency: few_rows_kernel streams the weights once, without tensor cores.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -50,11 +53,11 @@ using namespace tc;
 enum Mode { kForward, kRows, kWeights };
 
 constexpr int kBM = 128, kBK = 64;
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarps = 16;
 constexpr int kBlock = 32 * (2 + kEpiWarps);
-constexpr int kEpiPitch = 80;  // bytes of a staged output row segment of 64 (+16: conflict-free)
+constexpr int kEpiPitch = 48;  // bytes of a staged output row segment of 32 (+16: conflict-free)
 constexpr int kEpiBytes = kEpiWarps * 32 * kEpiPitch;
-constexpr int kBiasBytes = kEpiWarps * 128 * 4;
+constexpr int kBiasBytes = kEpiWarps * 64 * 4;
 constexpr int kMaxStages = 8;
 constexpr int kSmemLimit = 232448;
 
@@ -82,6 +85,10 @@ template <class T, int P, int BN> struct Shape {
   static constexpr int stage_bytes = a_bytes + b_bytes;
   static constexpr int acc_cols = P == 3 ? 128 : 256;
   static constexpr int acc_bufs = 512 / acc_cols;
+  // Epilogue warps: four lane quarters (a warp reads the TMEM lanes of its
+  // number modulo 4) times `parts` strips of columns.
+  static constexpr int parts = BN >= 128 ? 4 : 2;
+  static constexpr int part_cols = BN / parts;
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -182,48 +189,75 @@ __device__ __noinline__ float plain_sum(const Args& p, int e, int lo, int hi, in
   return s;
 }
 
-// Sigmoid family for results that are rounded to 16 bits: exp and the
-// reciprocal by the fast units, each within 2^-21 of its value.
-__device__ __forceinline__ float fast_sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+// Activations of results that are rounded to 16 bits: exp and reciprocal by the
+// fast units, each within 2^-21 of its value, subnormal values as zero.
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float fast_sigmoid(float x) { return fast_rcp(1.0f + fast_exp2(-kLog2e * x)); }
+// 0.5 x (1 + erf(x / sqrt 2)) with the error function of Abramowitz and Stegun
+// 7.1.26 (erf within 1.5e-7): erfc(y) = (a1 t + ... + a5 t^5) exp(-y^2),
+// t = 1 / (1 + 0.3275911 y), y >= 0.
+__device__ __forceinline__ float fast_gelu(float x) {
+  const float y = fabsf(x) * 0.70710678118654752f;
+  const float t = fast_rcp(fmaf(0.3275911f, y, 1.0f));
+  float p = fmaf(1.061405429f, t, -1.453152027f);
+  p = fmaf(p, t, 1.421413741f);
+  p = fmaf(p, t, -0.284496736f);
+  p = fmaf(p, t, 0.254829592f);
+  const float c = 0.5f * p * t * fast_exp2(-kLog2e * y * y);  // erfc(y) / 2
+  return x * (x > 0.0f ? 1.0f - c : c);
+}
+
+template <class T>
+__device__ __forceinline__ float activate_one(int kind, int flags, float x, float s0, float s1) {
+  if constexpr (sizeof(T) == 2) {
+    if (kind == EPI_SILU) return x * fast_sigmoid(x);
+    if (kind == EPI_SIGMOID) return fast_sigmoid(x);
+    if (kind == EPI_GELU && !(flags & 0x2)) return fast_gelu(x);
+  }
+  return activation<float>(kind, flags, x, s0, s1);
+}
 
 template <class T, int KIND>
 __device__ __forceinline__ void activate32(float (&v)[32], int flags, float s0, float s1) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    if constexpr (sizeof(T) == 2 && KIND == EPI_SILU) v[i] = __fdividef(v[i], 1.0f + __expf(-v[i]));
-    else if constexpr (sizeof(T) == 2 && KIND == EPI_SIGMOID) v[i] = fast_sigmoid(v[i]);
-    else v[i] = activation<float>(KIND, flags, v[i], s0, s1);
-  }
+  for (int i = 0; i < 32; ++i) v[i] = activate_one<T>(KIND, flags, v[i], s0, s1);
 }
 template <class T>
 __device__ __forceinline__ void activate_all(float (&v)[32], int kind, int flags, float s0, float s1) {
-  switch (kind) {
-    case EPI_NONE: return;
-    case EPI_RELU: return activate32<T, EPI_RELU>(v, flags, s0, s1);
-    case EPI_GELU: return activate32<T, EPI_GELU>(v, flags, s0, s1);
-    case EPI_SILU: return activate32<T, EPI_SILU>(v, flags, s0, s1);
-    case EPI_SIGMOID: return activate32<T, EPI_SIGMOID>(v, flags, s0, s1);
-    default:
+  if (kind == EPI_NONE) return;
+  if (kind == EPI_RELU) return activate32<T, EPI_RELU>(v, flags, s0, s1);
+  if (kind == EPI_SILU) return activate32<T, EPI_SILU>(v, flags, s0, s1);
+  if (sizeof(T) == 2 && kind == EPI_GELU && !(flags & 0x2)) return activate32<T, EPI_GELU>(v, 0, s0, s1);
+  // The others share one loop of 8 values to keep the kernel small.
 #pragma unroll 1
-      for (int i = 0; i < 4; ++i)  // the rarer ones share one loop of 8 values to keep the kernel small
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float x = 0.0f;
+    for (int j = 0; j < 8; ++j) {
+      float x = 0.0f;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) x = q == i ? v[8 * q + j] : x;
-          x = activation<float>(kind, flags, x, s0, s1);
+      for (int q = 0; q < 4; ++q) x = q == i ? v[8 * q + j] : x;
+      x = activate_one<T>(kind, flags, x, s0, s1);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) v[8 * q + j] = q == i ? x : v[8 * q + j];
-        }
-  }
+      for (int q = 0; q < 4; ++q) v[8 * q + j] = q == i ? x : v[8 * q + j];
+    }
 }
 
 // 32 columns of this warp's 32 rows (one row a lane) to global memory through
-// the warp's staging rows: 64 contiguous bytes of a row at a time.
+// the warp's staging rows: 32 contiguous bytes (a sector) of a row at a time.
 template <class O>
 __device__ __forceinline__ void store_rows(const float (&v)[32], unsigned char* stage, O* c, int64_t ld, int m_valid,
                                            int n_valid, bool vec) {
-  constexpr int kCols = 64 / sizeof(O), kPasses = 32 / kCols, kPer = 16 / sizeof(O);
+  constexpr int kCols = 32 / sizeof(O), kPasses = 32 / kCols, kPer = 16 / sizeof(O);
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int pass = 0; pass < kPasses; ++pass) {
@@ -231,14 +265,14 @@ __device__ __forceinline__ void store_rows(const float (&v)[32], unsigned char* 
 #pragma unroll
     for (int i = 0; i < kCols; ++i) o[i] = Num<O>::from_c(v[pass * kCols + i]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 2; ++i)
       reinterpret_cast<uint4*>(stage + lane * kEpiPitch)[i] = reinterpret_cast<const uint4*>(o)[i];
     __syncwarp();
     const int col0 = pass * kCols;
     if (vec && col0 + kCols <= n_valid) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = i * 8 + (lane >> 2), ch = lane & 3;
+      for (int i = 0; i < 2; ++i) {
+        const int r = i * 16 + (lane >> 1), ch = lane & 1;
         const uint4 u = *reinterpret_cast<const uint4*>(stage + r * kEpiPitch + ch * 16);
         if (r < m_valid) *reinterpret_cast<uint4*>(c + r * ld + col0 + ch * kPer) = u;
       }
@@ -286,7 +320,7 @@ __global__ void __launch_bounds__(kBlock, 1)
     }
     for (int b = 0; b < S::acc_bufs; ++b) {
       mbar_init(acc_full(b), 1);
-      mbar_init(acc_empty(b), kEpiWarps);
+      mbar_init(acc_empty(b), 4 * S::parts);
     }
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -426,12 +460,12 @@ __global__ void __launch_bounds__(kBlock, 1)
       umma_commit_warp(drain);  // the MMAs issued so far, before TMEM is freed
       (void)mbar_wait_bounded(drain, 0);
     }
-  } else {
+  } else if ((warp - 2) >> 2 < S::parts) {
     // ------------------------------------------------------- epilogue ----
-    const int quarter = warp & 3, half = (warp - 2) >> 2, w = warp - 2;
-    constexpr int kHalf = BN / 2, kChunks = kHalf / 32;
+    const int quarter = warp & 3, part = (warp - 2) >> 2, w = warp - 2;
+    constexpr int kChunks = S::part_cols / 32;
     unsigned char* stage = epi + w * 32 * kEpiPitch;
-    float* bias_w = bias_s + w * 128;
+    float* bias_w = bias_s + w * 64;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const int n_end = MODE == kRows ? p.inputs : p.outputs;
     int buf = 0;
@@ -456,7 +490,7 @@ __global__ void __launch_bounds__(kBlock, 1)
     while (ok && tiles.next(v)) {
       const int m_end = MODE == kWeights ? p.inputs : v.hi - v.lo;
       const int row0 = v.m0 + quarter * 32, m_valid = min(32, m_end - row0);
-      const int col0 = v.n0 + half * kHalf;
+      const int col0 = v.n0 + part * S::part_cols;
       if (MODE == kForward && p.bias) {
         const T* bias = static_cast<const T*>(p.bias) + (int64_t)v.e * p.outputs;
         __syncwarp();
@@ -469,6 +503,7 @@ __global__ void __launch_bounds__(kBlock, 1)
       }
       auto finish = [&](float (&x)[32], int c) {
         const int n = col0 + c * 32, n_valid = n_end - n;
+        if (n_valid <= 0 || m_valid <= 0) return;
         if constexpr (P == 3) {
 #pragma unroll
           for (int i = 0; i < 32; ++i)
@@ -487,7 +522,6 @@ __global__ void __launch_bounds__(kBlock, 1)
           }
           activate_all<T>(x, p.act, p.act_flags, p.s0, p.s1);
         }
-        if (n_valid <= 0 || m_valid <= 0) return;
         if (MODE == kWeights) {
           if (p.unit_rows)
             store_rows<float>(x, stage, p.partial + (v.slot * p.inputs + row0) * p.outputs + n, p.outputs, m_valid,
@@ -502,7 +536,7 @@ __global__ void __launch_bounds__(kBlock, 1)
       };
       if (P == 1 && v.k_blocks > 0) {
         if (!(ok = wait_acc())) break;
-        const uint32_t t = tmem + lane_base + (uint32_t)(buf * S::acc_cols + half * kHalf);
+        const uint32_t t = tmem + lane_base + (uint32_t)(buf * S::acc_cols + part * S::part_cols);
 #pragma unroll 1
         for (int c = 0; c < kChunks; ++c) {
           float x[32];
@@ -515,7 +549,7 @@ __global__ void __launch_bounds__(kBlock, 1)
         if constexpr (P == 3) {
           for (int kb = 0; kb < v.k_blocks; ++kb) {
             if (!(ok = wait_acc())) break;
-            const uint32_t t = tmem + lane_base + (uint32_t)(buf * S::acc_cols + half * kHalf);
+            const uint32_t t = tmem + lane_base + (uint32_t)(buf * S::acc_cols + part * S::part_cols);
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
               float x[32];
@@ -554,6 +588,183 @@ __global__ void __launch_bounds__(kBlock, 1)
   }
 }
 
+// ------------------------------------------------------------ few rows ----
+// Forward for groups of a few rows: a work item is up to 8 rows of a group, a
+// block takes 128 columns and one of the cluster's slices of K.  A thread holds
+// the sums of a vector of columns (16 bytes of weights: one load serves all of
+// the item's rows) for every 8th or 16th k; the k groups are added in shared
+// memory, the slices through the cluster's distributed shared memory, in a
+// fixed order.  The rows of the item lie in shared memory as fp32.
+constexpr int kFewThreads = 256, kFewRows = 8, kFewCols = 128, kFewK = 1024;
+
+template <class T> struct Few {
+  static constexpr int vec = 16 / sizeof(T);           // columns of a thread
+  static constexpr int lanes = kFewCols / vec;         // threads side by side
+  static constexpr int groups = kFewThreads / lanes;   // k groups of the block
+};
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Sums of RB rows over k in [0, kn) of the weights at w (row stride w_ld).
+template <class T, int RB, bool VEC>
+__device__ __forceinline__ void few_sums(const T* __restrict__ w, int64_t w_ld, int kn, int cols, const float* xs,
+                                         float (&acc)[RB][Few<T>::vec]) {
+  constexpr int V = Few<T>::vec, G = Few<T>::groups, U = RB > 4 ? 4 : 8;
+  const int g = threadIdx.x / Few<T>::lanes;
+  auto load = [&](int k) -> uint4 {
+    const T* p = w + (int64_t)k * w_ld;
+    if constexpr (VEC) {
+      return cols >= V ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+    } else {
+      alignas(16) T v[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = i < cols ? p[i] : Num<T>::from_c(0.0f);
+      return *reinterpret_cast<uint4*>(v);
+    }
+  };
+  auto add = [&](const uint4& u, int k) {
+    const T* t = reinterpret_cast<const T*>(&u);
+    float f[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = Num<T>::to_c(t[i]);
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      const float x = xs[k * RB + r];
+#pragma unroll
+      for (int i = 0; i < V; i += 2) f2::fma(acc[r][i], acc[r][i + 1], f[i], f[i + 1], x, x, acc[r][i], acc[r][i + 1]);
+    }
+  };
+  int k = g;
+  for (; k + (U - 1) * G < kn; k += U * G) {
+    uint4 u[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) u[i] = load(k + i * G);
+#pragma unroll
+    for (int i = 0; i < U; ++i) add(u[i], k + i * G);
+  }
+  for (; k < kn; k += G) add(load(k), k);
+}
+
+template <class T, int RB, bool VEC>
+__device__ void few_item(const Args& p, int e, int64_t row0, int n_rows, int n0, int slice, int slices, float* sm) {
+  constexpr int V = Few<T>::vec, L = Few<T>::lanes, W = kFewThreads / 32;
+  const int tid = threadIdx.x, x = tid % L, lane = tid & 31, warp = tid >> 5;
+  const int per = (p.inputs + slices - 1) / slices, k_lo = slice * per, k_hi = min(p.inputs, k_lo + per);
+  const T* rows = static_cast<const T*>(p.a) + row0 * p.a_ld;
+  const int cols = p.outputs - (n0 + x * V);
+  const T* w = static_cast<const T*>(p.b) + e * p.b_stride + (cols > 0 ? n0 + x * V : 0);
+  float acc[RB][V] = {};
+  for (int k0 = k_lo; k0 < k_hi; k0 += kFewK) {
+    const int kn = min(kFewK, k_hi - k0);
+    __syncthreads();
+    for (int i = tid; i < kn * RB; i += kFewThreads) {
+      const int r = i / kn, k = i - r * kn;
+      sm[k * RB + r] = r < n_rows ? Num<T>::to_c(rows[r * p.a_ld + k0 + k]) : 0.0f;
+    }
+    __syncthreads();
+    few_sums<T, RB, VEC>(w + (int64_t)k0 * p.b_ld, p.b_ld, kn, cols, sm, acc);
+  }
+  if (L == 16) {
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[r][i] += __shfl_xor_sync(0xffffffffu, acc[r][i], 16);
+  }
+  // sm: [W][RB][kFewCols] sums of the warps, then [RB][kFewCols] of the block in front.
+  __syncthreads();
+  if (lane < L) {
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int i = 0; i < V; ++i) sm[(warp * RB + r) * kFewCols + x * V + i] = acc[r][i];
+  }
+  __syncthreads();
+  for (int i = tid; i < RB * kFewCols; i += kFewThreads) {
+    float s = 0.0f;
+#pragma unroll
+    for (int q = 0; q < W; ++q) s += sm[q * RB * kFewCols + i];
+    sm[i] = s;
+  }
+  if (slices > 1) cluster_sync();
+  else __syncthreads();
+  T* out = static_cast<T*>(p.c) + row0 * p.c_ld;
+  for (int i = slice * kFewThreads + tid; i < n_rows * kFewCols; i += slices * kFewThreads) {
+    const int r = i / kFewCols, n = n0 + i % kFewCols;
+    float s = 0.0f;
+    if (slices > 1) {
+      for (int q = 0; q < slices; ++q) s += ld_cluster(mapa_shared(smem_u32(sm + i), q));
+    } else {
+      s = sm[i];
+    }
+    if (n < p.outputs) {
+      if (p.bias) s += Num<T>::to_c(static_cast<const T*>(p.bias)[(int64_t)e * p.outputs + n]);
+      out[r * p.c_ld + n] = Num<T>::from_c(activate_one<T>(p.act, p.act_flags, s, p.s0, p.s1));
+    }
+  }
+  if (slices > 1) cluster_sync();  // the others may still read this block's sums
+}
+
+template <class T, bool VEC>
+__global__ void __launch_bounds__(kFewThreads, 2) few_rows_kernel(const Args p, int slices) {
+  __shared__ __align__(16) float sm[kFewK * kFewRows];
+  __shared__ int found[3];
+  ops::let_successor_start();
+  ops::wait_for_predecessor();
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int strip = blockIdx.x / slices, slice = blockIdx.x % slices;
+  if (tid < 32) {
+    // The item's group: items in expert order, 8 rows each.
+    int base = 0, e = -1, row0 = 0, n = 0;
+    for (int e0 = 0; e0 < p.experts && e < 0; e0 += 32) {
+      const int i = e0 + lane;
+      int lo = 0, hi = 0;
+      if (i < p.experts) {
+        lo = clamped(p.offset[i], 0, p.rows);
+        hi = clamped(p.offset[i + 1], lo, p.rows);
+      }
+      const int c = (hi - lo + kFewRows - 1) / kFewRows;
+      int s = c;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, s, d);
+        if (lane >= d) s += o;
+      }
+      const int first = base + s - c, want = (int)blockIdx.y;
+      const unsigned hit = __ballot_sync(0xffffffffu, want >= first && want < first + c);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        e = e0 + src;
+        row0 = __shfl_sync(0xffffffffu, lo + (want - first) * kFewRows, src);
+        n = min(kFewRows, __shfl_sync(0xffffffffu, hi, src) - row0);
+      }
+      base += __shfl_sync(0xffffffffu, s, 31);
+    }
+    if (lane == 0) {
+      found[0] = e;
+      found[1] = row0;
+      found[2] = n;
+    }
+  }
+  if (blockIdx.x == 0 && blockIdx.y == 0) check_offsets(p.offset, p.experts, p.rows, p.error);
+  if (blockIdx.y == 0) {
+    const int64_t used = clamped(p.offset[p.experts], 0, p.rows);
+    for (int64_t r = used + blockIdx.x; r < p.rows; r += gridDim.x)
+      for (int n = tid; n < p.outputs; n += kFewThreads) static_cast<T*>(p.c)[r * p.c_ld + n] = Num<T>::from_c(0.0f);
+  }
+  __syncthreads();
+  const int e = found[0], n = found[2];
+  if (e < 0) return;  // the whole cluster: it has one item
+  const int n0 = strip * kFewCols;
+  if (n == 1) few_item<T, 1, VEC>(p, e, found[1], n, n0, slice, slices, sm);
+  else if (n == 2) few_item<T, 2, VEC>(p, e, found[1], n, n0, slice, slices, sm);
+  else if (n <= 4) few_item<T, 4, VEC>(p, e, found[1], n, n0, slice, slices, sm);
+  else few_item<T, 8, VEC>(p, e, found[1], n, n0, slice, slices, sm);
+}
+
 // d_W_e = sum of its units' partial sums, in order.
 template <class T>
 __global__ void __launch_bounds__(256)
@@ -583,24 +794,60 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Column sums of an expert's rows.
-template <class T>
+// d_b_e: column sums of a group's rows.  A block sums one of `parts` equal parts
+// of a group's rows over one strip of columns (16 bytes a lane where the rows
+// allow it, else one element), in a fixed order; several parts are added by
+// sum_parts_kernel.  d_out was just read by the products, so this reads L2.
+template <class T, int V>
 __global__ void __launch_bounds__(256)
-    bias_gradient_kernel(const T* __restrict__ d, int64_t ld, int64_t rows, const int* __restrict__ offset, int experts,
-                         int outputs, T* __restrict__ out) {
-  __shared__ float part[8][32];
-  const int e = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockIdx.x * 32 + lane;
+    bias_gradient_kernel(const T* __restrict__ d, int64_t ld, int64_t rows, const int* __restrict__ offset, int outputs,
+                         int parts, float* __restrict__ partial, T* __restrict__ out) {
+  constexpr int kLanes = V > 1 ? 16 : 32, kGroups = 256 / kLanes, kCols = kLanes * V;
+  __shared__ float sums[kGroups][kCols + 1];
+  ops::let_successor_start();
+  const int e = blockIdx.y, x = threadIdx.x % kLanes, y = threadIdx.x / kLanes, n = blockIdx.x * kCols + x * V;
   const int lo = clamped(offset[e], 0, rows), hi = clamped(offset[e + 1], lo, rows);
-  float s = 0.0f;
-  if (n < outputs)
-    for (int64_t r = lo + warp; r < hi; r += 8) s += Num<T>::to_c(d[r * ld + n]);
-  part[warp][lane] = s;
+  const int64_t per = ((int64_t)hi - lo + parts - 1) / parts;
+  const int64_t r0 = lo + blockIdx.z * per, r1 = min((int64_t)hi, r0 + per);
+  float s[V] = {};
+  if (n < outputs) {
+    const T* p = d + n;
+    if constexpr (V > 1) {
+#pragma unroll 4
+      for (int64_t r = r0 + y; r < r1; r += kGroups) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p + r * ld));
+        const T* v = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i] += Num<T>::to_c(v[i]);
+      }
+    } else {
+#pragma unroll 8
+      for (int64_t r = r0 + y; r < r1; r += kGroups) s[0] += Num<T>::to_c(p[r * ld]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) sums[y][x * V + i] = s[i];
   __syncthreads();
-  if (warp == 0 && n < outputs) {
+  for (int i = threadIdx.x; i < kCols; i += 256) {
+    const int c = blockIdx.x * kCols + i;
+    if (c >= outputs) break;
     float t = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) t += part[w][lane];
-    out[(int64_t)e * outputs + n] = Num<T>::from_c(t);
+    for (int g = 0; g < kGroups; ++g) t += sums[g][i];
+    if (parts == 1) out[(int64_t)e * outputs + c] = Num<T>::from_c(t);
+    else partial[((int64_t)blockIdx.z * gridDim.y + e) * outputs + c] = t;
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(256)
+    sum_parts_kernel(const float* __restrict__ partial, T* __restrict__ out, int64_t n, int parts) {
+  ops::wait_for_predecessor();
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    float s = 0.0f;
+#pragma unroll 4
+    for (int q = 0; q < parts; ++q) s += partial[q * n + i];
+    out[i] = Num<T>::from_c(s);
   }
 }
 
@@ -727,6 +974,17 @@ int64_t partial_bytes(int64_t rows, int experts, int inputs, int outputs, int sm
   return unit ? pad256((rows / unit + experts) * (int64_t)inputs * outputs * 4) : 0;
 }
 
+// Parts of a group's rows in the bias gradient: about four blocks an SM, of 128
+// rows at least on average.
+int bias_parts(int64_t rows, int experts, int outputs, int sms) {
+  const int64_t strips = (int64_t)experts * ((outputs + 127) / 128);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(64, rows / experts / 128), 4 * sms / strips));
+}
+int64_t bias_bytes(int64_t rows, int experts, int outputs, int sms) {
+  const int parts = bias_parts(rows, experts, outputs, sms);
+  return parts > 1 ? pad256((int64_t)parts * experts * outputs * 4) : 0;
+}
+
 // Hands out the caller's workspace.
 struct Space {
   char* at;
@@ -759,19 +1017,24 @@ ponni_b200_status launch_shape(const Operand& a, const Operand& b, Args p, int s
   return e == cudaSuccess ? PONNI_B200_OK : ops::fail_cuda(e, "expert_product");
 }
 
-// Tile width: the widest whose padding costs at most an eighth more columns.
-int tile_width(int n, int most) {
+// Tile width.  An MMA of 128 x 64 takes as long as one of 128 x 128 (58 and 64
+// cycles for 16 k), so 64 is for products of at most 64 columns; 256 halves the
+// reads of the row tile against 128 and is taken unless its padding costs over
+// an eighth more columns, or the rows are so few that the weights' traffic
+// decides (at most half a tile of rows a group): 128 then spreads them more evenly
+// over the SMs.
+int tile_width(int n, int most, int64_t rows, int experts, bool weights) {
+  if (n <= 64) return 64;
+  if (most == 128 || n <= 128 || (!weights && rows <= (int64_t)64 * experts)) return 128;
   auto padded = [&](int w) { return (int64_t)(n + w - 1) / w * w; };
-  int w = most;
-  while (w > 64 && padded(w) * 8 > padded(64) * 9) w /= 2;
-  return w;
+  return padded(256) * 8 > padded(128) * 9 ? 128 : 256;
 }
 
 template <class T, int MODE>
 ponni_b200_status launch_product(const Operand& a, const Operand& b, const Args& p, int sms, cudaStream_t stream) {
   constexpr int P = sizeof(T) == 4 ? 3 : 1;
   const int n = MODE == kRows ? p.inputs : p.outputs;
-  const int w = tile_width(n, P == 3 ? 128 : 256);
+  const int w = tile_width(n, P == 3 ? 128 : 256, p.rows, p.experts, MODE == kWeights);
   const int64_t m_tiles = MODE == kWeights
                               ? (int64_t)((p.inputs + kBM - 1) / kBM) * (p.experts + (p.unit_rows ? p.rows / p.unit_rows : 0))
                               : p.rows / kBM + std::min<int64_t>(p.experts, p.rows);
@@ -780,6 +1043,47 @@ ponni_b200_status launch_product(const Operand& a, const Operand& b, const Args&
   if (w == 128) return launch_shape<T, MODE, P, 128>(a, b, p, sms, tiles, stream);
   if constexpr (P == 1) return launch_shape<T, MODE, P, 256>(a, b, p, sms, tiles, stream);
   return ops::fail(PONNI_B200_ERR_UNSUPPORTED, "expert_product: no tile shape");
+}
+
+// Whether few_rows_kernel takes a forward product.  fp32: up to 16 rows a group on
+// average; the tensor-core path has to lay out split copies of all weights first
+// (64 experts of 1024 x 2048, 16 rows each: 279 us against 475; one expert of
+// 2048 x 2048, one row: 6.4 against 60).  16 bits: up to 8 rows where the 128-column
+// tiles do not fill the SMs (8 experts of 2048 x 1024: 10.5 / 11.1 / 16.6 us
+// with 1 / 4 / 8 rows each against 15.5 to 17.8; one expert: 5.4 to 11 against 14.3);
+// where they do, the tensor cores stream the weights as fast with any number
+// of rows (64 experts of 1024 x 2048: 49 to 51 us against 55 with one row each, 130 with 8).
+bool few_rows(int dtype, int64_t rows, int experts, int outputs, int sms) {
+  if (dtype == PONNI_B200_F32) return rows <= (int64_t)16 * experts;
+  const int64_t tiles = std::min<int64_t>(rows, experts) * ((outputs + 127) / 128);
+  return tiles < sms && rows <= (int64_t)8 * (experts + 1);
+}
+
+template <class T>
+ponni_b200_status launch_few(const Args& p, int sms, cudaStream_t stream) {
+  const bool vec = reinterpret_cast<uintptr_t>(p.b) % 16 == 0 && p.b_ld * sizeof(T) % 16 == 0 &&
+                   (p.experts == 1 || p.b_stride * sizeof(T) % 16 == 0) && p.outputs * sizeof(T) % 16 == 0;
+  const int64_t strips = (p.outputs + kFewCols - 1) / kFewCols;
+  const int64_t items = std::min<int64_t>(p.experts, p.rows) + p.rows / kFewRows;
+  // Slices of K until there are two blocks an SM, of 128 k at least.
+  int slices = 1;
+  while (slices < 8 && items * strips * slices < 2 * sms && p.inputs / (2 * slices) >= 128) slices *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = slices;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(strips * slices), (unsigned)items);
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = vec ? cudaLaunchKernelEx(&cfg, few_rows_kernel<T, true>, p, slices)
+                            : cudaLaunchKernelEx(&cfg, few_rows_kernel<T, false>, p, slices);
+  return e == cudaSuccess ? PONNI_B200_OK : ops::fail_cuda(e, "expert_product");
 }
 
 template <class F>
@@ -846,11 +1150,14 @@ int64_t ponni_b200_expert_product_workspace(int dtype, int64_t num_rows, int exp
                                             int aligned, int backward, int device) {
   if (num_rows < 0 || experts < 1 || inputs < 1 || outputs < 1) return 0;
   int64_t n = 0;
+  if (!backward && few_rows(dtype, num_rows, experts, outputs, ops::num_sms(device))) return 0;
   if (dtype == PONNI_B200_F32 || !aligned) {
     n += staged_bytes(dtype, num_rows, inputs) + staged_bytes(dtype, (int64_t)experts * inputs, outputs);
     if (backward) n += staged_bytes(dtype, num_rows, outputs);
   }
-  if (backward) n += partial_bytes(num_rows, experts, inputs, outputs, ops::num_sms(device));
+  if (backward)
+    n += partial_bytes(num_rows, experts, inputs, outputs, ops::num_sms(device)) +
+         bias_bytes(num_rows, experts, outputs, ops::num_sms(device));
   return n;
 }
 
@@ -892,6 +1199,7 @@ ponni_b200_status ponni_b200_expert_product(int dtype, const void* rows, int64_t
     if (!p.error) return ops::fail(PONNI_B200_ERR_CUDA, "no operator error word on this device");
     const int sms = ops::num_sms(device);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (few_rows(dtype, num_rows, experts, outputs, sms)) return by_type(dtype, [&](auto t) { return launch_few<decltype(t)>(p, sms, s); });
     Stages stages = {};
     Space space = {static_cast<char*>(workspace), workspace_bytes};
     Operand a, b;
@@ -944,6 +1252,12 @@ ponni_b200_status ponni_b200_expert_product_backward(int dtype, const void* d_ou
       partial = space.take(partial_bytes(num_rows, experts, inputs, outputs, sms));
       if (!partial) st = ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "expert_product_backward: workspace is too small");
     }
+    const int parts = bias_parts(num_rows, experts, outputs, sms);
+    float* bias_partial = nullptr;
+    if (!st && d_bias && parts > 1) {
+      bias_partial = static_cast<float*>(space.take(bias_bytes(num_rows, experts, outputs, sms)));
+      if (!bias_partial) st = ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "expert_product_backward: workspace is too small");
+    }
     if (st) return st;
     return by_type(dtype, [&](auto t) -> ponni_b200_status {
       using T = decltype(t);
@@ -989,9 +1303,20 @@ ponni_b200_status ponni_b200_expert_product_backward(int dtype, const void* d_ou
         }
       }
       if (!r && d_bias) {
-        bias_gradient_kernel<T><<<dim3((outputs + 31) / 32, experts), 256, 0, s>>>(
-            static_cast<const T*>(d_out), d_out_ld, num_rows, offset, experts, outputs, static_cast<T*>(d_bias));
+        constexpr int V = 16 / sizeof(T);
+        const bool vec = reinterpret_cast<uintptr_t>(d_out) % 16 == 0 && d_out_ld % V == 0 && outputs % V == 0;
+        const int cols = vec ? 16 * V : 32;
+        const dim3 grid((outputs + cols - 1) / cols, experts, parts);
+        auto kern = vec ? bias_gradient_kernel<T, V> : bias_gradient_kernel<T, 1>;
+        kern<<<grid, 256, 0, s>>>(static_cast<const T*>(d_out), d_out_ld, num_rows, offset, outputs, parts, bias_partial,
+                                  static_cast<T*>(d_bias));
         r = ops::launched("expert_product_backward");
+        if (!r && parts > 1) {
+          const int64_t n = (int64_t)experts * outputs;
+          const cudaError_t e = ops::launch_after(sum_parts_kernel<T>, dim3((unsigned)std::min<int64_t>((n + 255) / 256, sms * 4)),
+                                                  dim3(256), 0, s, (const float*)bias_partial, static_cast<T*>(d_bias), n, parts);
+          if (e != cudaSuccess) r = ops::fail_cuda(e, "expert_product_backward");
+        }
       }
       return r;
     });
