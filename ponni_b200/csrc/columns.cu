@@ -7,14 +7,18 @@
 // combination with unit weights, and (fused) d_rows = weight d_y with
 // d_weight[j][b] = <rows[row[j][b]], d_y[.][b]>.
 //
-// All are transposes bound by HBM: a block turns a tile of 64 columns in
-// shared memory, in 4-byte words (one fp32 or two 16-bit features) with an odd
-// pitch, so that both the column side (lanes along the batch) and the row
-// side (lanes along the features) are free of bank conflicts.
+// All are transposes bound by HBM: a block turns tiles of 64 columns x 64 words
+// in shared memory (a word is 4 bytes: one fp32 or two 16-bit features).  On the
+// column side a thread moves four columns at once where the batch is aligned
+// (one 16-byte or two 8-byte accesses), on the row side 16 lanes take a row's 64
+// words, 16 bytes each where the rows are aligned.  Word w of column c lies in
+// 16-byte chunk (w / 4) ^ (c / 4 mod 16) of the column's 256 bytes: whole chunks
+// for the row side without conflicts, two-way conflicts for the column side.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "device_math.cuh"
 #include "operators.h"
@@ -26,7 +30,10 @@ constexpr int kBlock = 256;
 constexpr int kWarps = kBlock / 32;
 constexpr int kTileCols = 64;
 constexpr int kTileWords = 64;
-constexpr int kPitch = kTileWords + 1;
+constexpr int kRowLanes = 16;  // lanes that take a row
+
+// Place of word w of column c in the tile.
+__device__ __forceinline__ int place(int c, int w) { return c * kTileWords + ((((w >> 2) ^ (c >> 2)) & 15) << 2) + (w & 3); }
 
 template <class T> struct Word {  // 4 bytes of consecutive features
   static constexpr int n = 4 / sizeof(T);
@@ -73,27 +80,130 @@ __device__ __forceinline__ void store_word(T* __restrict__ row, int f, int featu
     if (f + i < features) row[f + i] = w.v[i];
 }
 
-// Tile of x (kTileCols columns from c0, kTileWords words of features from f0)
-// into shared memory [column][word].
+// Four columns of a word: n rows of x, four consecutive elements each, turned
+// into one word a column.
 template <class T>
+__device__ __forceinline__ void turn_in(const T* __restrict__ x, int64_t ld, int f, int features, uint32_t (&u)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    const uint4 v = f < features ? __ldg(reinterpret_cast<const uint4*>(x + f * ld)) : make_uint4(0, 0, 0, 0);
+    u[0] = v.x;
+    u[1] = v.y;
+    u[2] = v.z;
+    u[3] = v.w;
+  } else {
+    const uint2 a = f < features ? __ldg(reinterpret_cast<const uint2*>(x + f * ld)) : make_uint2(0, 0);
+    const uint2 b = f + 1 < features ? __ldg(reinterpret_cast<const uint2*>(x + (f + 1) * ld)) : make_uint2(0, 0);
+    u[0] = __byte_perm(a.x, b.x, 0x5410);
+    u[1] = __byte_perm(a.x, b.x, 0x7632);
+    u[2] = __byte_perm(a.y, b.y, 0x5410);
+    u[3] = __byte_perm(a.y, b.y, 0x7632);
+  }
+}
+template <class T>
+__device__ __forceinline__ void turn_out(T* __restrict__ y, int64_t ld, int f, int features, const uint32_t (&u)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    if (f < features) *reinterpret_cast<uint4*>(y + f * ld) = make_uint4(u[0], u[1], u[2], u[3]);
+  } else {
+    if (f < features)
+      *reinterpret_cast<uint2*>(y + f * ld) = make_uint2(__byte_perm(u[0], u[1], 0x5410), __byte_perm(u[2], u[3], 0x5410));
+    if (f + 1 < features)
+      *reinterpret_cast<uint2*>(y + (f + 1) * ld) =
+          make_uint2(__byte_perm(u[0], u[1], 0x7632), __byte_perm(u[2], u[3], 0x7632));
+  }
+}
+
+// Tile of x (kTileCols columns from c0, kTileWords words of features from f0)
+// into shared memory; QUADS: the batch allows four columns at once.
+template <class T, bool QUADS>
 __device__ __forceinline__ void load_tile(uint32_t* tile, const T* __restrict__ x, int64_t ld, int f0, int features,
                                           int64_t c0, int64_t batch) {
   constexpr int n = Word<T>::n;
+  if (QUADS && c0 + kTileCols <= batch) {
+    constexpr int kPer = kTileWords * (kTileCols / 4) / kBlock;
+    uint32_t u[kPer][4];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int it = i * kBlock + threadIdx.x, q = it % (kTileCols / 4), w = it / (kTileCols / 4);
+      turn_in<T>(x + c0 + 4 * q, ld, f0 + w * n, features, u[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int it = i * kBlock + threadIdx.x, q = it % (kTileCols / 4), w = it / (kTileCols / 4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) tile[place(4 * q + k, w)] = u[i][k];
+    }
+    return;
+  }
+  constexpr int kPer = kTileWords * kTileCols / kBlock;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll 4
-  for (int w = warp; w < kTileWords; w += kWarps) {
 #pragma unroll
-    for (int h = 0; h < kTileCols / 32; ++h) {
-      const int c = h * 32 + lane;
-      Word<T> v;
+  for (int i0 = 0; i0 < kPer; i0 += 8) {
+    Word<T> v[8];
 #pragma unroll
-      for (int i = 0; i < n; ++i) {
-        const int f = f0 + w * n + i;
-        v.v[i] = f < features && c0 + c < batch ? x[f * ld + c0 + c] : Num<T>::from_c(0.0f);
+    for (int i = 0; i < 8; ++i) {
+      const int it = (i0 + i) * kWarps + warp, c = it % 2 * 32 + lane, w = it / 2;
+#pragma unroll
+      for (int k = 0; k < n; ++k) {
+        const int f = f0 + w * n + k;
+        v[i].v[k] = f < features && c0 + c < batch ? __ldg(x + f * ld + c0 + c) : Num<T>::from_c(0.0f);
       }
-      tile[c * kPitch + w] = *reinterpret_cast<uint32_t*>(&v);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int it = (i0 + i) * kWarps + warp, c = it % 2 * 32 + lane, w = it / 2;
+      tile[place(c, w)] = *reinterpret_cast<uint32_t*>(&v[i]);
     }
   }
+}
+
+// The four words of a row that lane l of its 16 takes: neighbours where they
+// are moved as 16 bytes, 16 apart otherwise.
+template <bool VEC>
+__device__ __forceinline__ int row_word(int l, int i) {
+  return VEC ? 4 * l + i : l + kRowLanes * i;
+}
+template <class T, bool VEC>
+__device__ __forceinline__ void load_row(const T* __restrict__ row, int f0, int features, bool whole, int l, uint32_t (&u)[4]) {
+  constexpr int n = Word<T>::n;
+  if (VEC && f0 + (4 * l + 4) * n <= features) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + f0 + 4 * l * n));
+    u[0] = v.x;
+    u[1] = v.y;
+    u[2] = v.z;
+    u[3] = v.w;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int f = f0 + row_word<VEC>(l, i) * n;
+    u[i] = f < features ? load_word<T>(row, f, features, whole) : 0u;
+  }
+}
+template <class T, bool VEC>
+__device__ __forceinline__ void store_row(T* __restrict__ row, int f0, int features, bool whole, int l, const uint32_t (&u)[4]) {
+  constexpr int n = Word<T>::n;
+  if (VEC && f0 + (4 * l + 4) * n <= features) {
+    *reinterpret_cast<uint4*>(row + f0 + 4 * l * n) = make_uint4(u[0], u[1], u[2], u[3]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int f = f0 + row_word<VEC>(l, i) * n;
+    if (f < features) store_word<T>(row, f, features, whole, u[i]);
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void read_tile(const uint32_t* tile, int c, int l, uint32_t (&u)[4]) {
+  if (VEC) {
+    const uint4 v = *reinterpret_cast<const uint4*>(tile + place(c, 4 * l));
+    u[0] = v.x;
+    u[1] = v.y;
+    u[2] = v.z;
+    u[3] = v.w;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u[i] = tile[place(c, row_word<VEC>(l, i))];
 }
 
 // Rows that no choice fills: the ones past the last group.
@@ -105,133 +215,175 @@ __device__ __forceinline__ void zero_unused(T* __restrict__ rows, int64_t ld, in
     for (int f = threadIdx.x; f < features; f += kBlock) rows[r * ld + f] = Num<T>::from_c(0.0f);
 }
 
-template <class T>
+template <class T, bool QUADS, bool VEC>
 __global__ void __launch_bounds__(kBlock)
     gather_kernel(const T* __restrict__ x, int64_t ld, int features, int64_t batch, int top_k,
                   const int* __restrict__ row, const int* __restrict__ used, T* __restrict__ rows, int64_t rows_ld,
                   int64_t num_rows, int whole) {
-  __shared__ uint32_t tile[kTileCols * kPitch];
+  __shared__ __align__(16) uint32_t tile[kTileCols * kTileWords];
+  __shared__ int at[ops::kMaxTopK * kTileCols];
   constexpr int n = Word<T>::n;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int l = threadIdx.x % kRowLanes, g = threadIdx.x / kRowLanes;
   const int f0 = blockIdx.y * kTileWords * n;
   const int64_t c0 = blockIdx.x * (int64_t)kTileCols;
-  load_tile<T>(tile, x, ld, f0, features, c0, batch);
+  for (int i = threadIdx.x; i < top_k * kTileCols; i += kBlock) {
+    const int64_t c = c0 + i % kTileCols;
+    const int r = c < batch ? row[i / kTileCols * batch + c] : -1;
+    at[i] = r < num_rows ? r : -1;
+  }
+  load_tile<T, QUADS>(tile, x, ld, f0, features, c0, batch);
   __syncthreads();
-  for (int c = warp; c < kTileCols && c0 + c < batch; c += kWarps) {
-    for (int j = 0; j < top_k; ++j) {
-      const int r = row[j * batch + c0 + c];
-      if (r < 0 || r >= num_rows) continue;
 #pragma unroll
-      for (int w = lane; w < kTileWords; w += 32)
-        if (f0 + w * n < features) store_word<T>(rows + r * rows_ld, f0 + w * n, features, whole, tile[c * kPitch + w]);
+  for (int c = g; c < kTileCols; c += kBlock / kRowLanes) {
+    uint32_t u[4];
+    read_tile<VEC>(tile, c, l, u);
+    for (int j = 0; j < top_k; ++j) {
+      const int r = at[j * kTileCols + c];
+      if (r >= 0) store_row<T, VEC>(rows + r * rows_ld, f0, features, whole, l, u);
     }
   }
   if (blockIdx.y == 0) zero_unused<T>(rows, rows_ld, features, num_rows, used, blockIdx.x, gridDim.x);
 }
 
 // weight == nullptr: unit weights.
-template <class T>
+template <class T, bool QUADS, bool VEC>
 __global__ void __launch_bounds__(kBlock)
     combine_kernel(const T* __restrict__ rows, int64_t rows_ld, int64_t num_rows, int features, int64_t batch, int top_k,
                    const int* __restrict__ row, const float* __restrict__ weight, T* __restrict__ y, int64_t ld,
                    int whole) {
-  __shared__ uint32_t tile[kTileCols * kPitch];
+  __shared__ __align__(16) uint32_t tile[kTileCols * kTileWords];
+  __shared__ int at[ops::kMaxTopK * kTileCols];
+  __shared__ float wt[ops::kMaxTopK * kTileCols];
   constexpr int n = Word<T>::n;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int kGroups = kBlock / kRowLanes, kCols = kTileCols / kGroups;
+  const int l = threadIdx.x % kRowLanes, g = threadIdx.x / kRowLanes;
   const int f0 = blockIdx.y * kTileWords * n;
   const int64_t c0 = blockIdx.x * (int64_t)kTileCols;
-  for (int c = warp; c < kTileCols && c0 + c < batch; c += kWarps) {
-    float acc[kTileWords / 32][n] = {};
-    for (int j = 0; j < top_k; ++j) {
-      const int r = row[j * batch + c0 + c];
-      if (r < 0 || r >= num_rows) continue;
-      const float wt = weight ? weight[j * batch + c0 + c] : 1.0f;
+  for (int i = threadIdx.x; i < top_k * kTileCols; i += kBlock) {
+    const int64_t c = c0 + i % kTileCols;
+    const int r = c < batch ? row[i / kTileCols * batch + c] : -1;
+    at[i] = r < num_rows ? r : -1;
+    wt[i] = weight && c < batch ? weight[i / kTileCols * batch + c] : 1.0f;
+  }
+  __syncthreads();
+  float acc[kCols][4][n] = {};
+  for (int j = 0; j < top_k; ++j) {
+    uint32_t u[kCols][4];
 #pragma unroll
-      for (int h = 0; h < kTileWords / 32; ++h) {
-        const int f = f0 + (h * 32 + lane) * n;
-        if (f < features) {
+    for (int q = 0; q < kCols; ++q) {
+      const int r = at[j * kTileCols + g + q * kGroups];
+      if (r >= 0) load_row<T, VEC>(rows + r * rows_ld, f0, features, whole, l, u[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < kCols; ++q) {
+      const int i = j * kTileCols + g + q * kGroups;
+      if (at[i] >= 0) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
           float v[n];
-          unpack<T>(load_word<T>(rows + r * rows_ld, f, features, whole), v);
+          unpack<T>(u[q][k], v);
 #pragma unroll
-          for (int i = 0; i < n; ++i) acc[h][i] = fmaf(wt, v[i], acc[h][i]);
+          for (int h = 0; h < n; ++h) acc[q][k][h] = fmaf(wt[i], v[h], acc[q][k][h]);
         }
       }
     }
-#pragma unroll
-    for (int h = 0; h < kTileWords / 32; ++h) tile[c * kPitch + h * 32 + lane] = pack<T>(acc[h]);
   }
+#pragma unroll
+  for (int q = 0; q < kCols; ++q)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) tile[place(g + q * kGroups, row_word<VEC>(l, k))] = pack<T>(acc[q][k]);
   __syncthreads();
+  if (QUADS && c0 + kTileCols <= batch) {
+#pragma unroll
+    for (int i = 0; i < kTileWords * (kTileCols / 4) / kBlock; ++i) {
+      const int it = i * kBlock + threadIdx.x, q = it % (kTileCols / 4), w = it / (kTileCols / 4);
+      uint32_t u[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) u[k] = tile[place(4 * q + k, w)];
+      turn_out<T>(y + c0 + 4 * q, ld, f0 + w * n, features, u);
+    }
+    return;
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll 4
-  for (int w = warp; w < kTileWords; w += kWarps) {
+  for (int it = warp; it < 2 * kTileWords; it += kWarps) {
+    const int c = it % 2 * 32 + lane, w = it / 2;
+    if (c0 + c >= batch) continue;
+    const uint32_t u = tile[place(c, w)];
+    const Word<T> v = *reinterpret_cast<const Word<T>*>(&u);
 #pragma unroll
-    for (int h = 0; h < kTileCols / 32; ++h) {
-      const int c = h * 32 + lane;
-      if (c0 + c >= batch) continue;
-      const uint32_t u = tile[c * kPitch + w];
-      const Word<T> v = *reinterpret_cast<const Word<T>*>(&u);
-#pragma unroll
-      for (int i = 0; i < n; ++i) {
-        const int f = f0 + w * n + i;
-        if (f < features) y[f * ld + c0 + c] = v.v[i];
-      }
+    for (int i = 0; i < n; ++i) {
+      const int f = f0 + w * n + i;
+      if (f < features) y[f * ld + c0 + c] = v.v[i];
     }
   }
 }
 
 // A block holds its 64 columns through all feature tiles, so that a dot
-// product is summed by one warp in a fixed order.
-template <class T, int K>
+// product is summed by 16 lanes in a fixed order.
+template <class T, int K, bool QUADS, bool VEC>
 __global__ void __launch_bounds__(kBlock)
     combine_backward_kernel(const T* __restrict__ dy, int64_t ld, const T* __restrict__ rows, int64_t rows_ld,
                             int64_t num_rows, int features, int64_t batch, const int* __restrict__ row,
                             const float* __restrict__ weight, const int* __restrict__ used, T* __restrict__ d_rows,
                             int64_t d_ld, float* __restrict__ d_weight, int whole, int d_whole) {
-  __shared__ uint32_t tile[kTileCols * kPitch];
-  constexpr int n = Word<T>::n, kCols = kTileCols / kWarps;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ __align__(16) uint32_t tile[kTileCols * kTileWords];
+  __shared__ int at[K * kTileCols];
+  __shared__ float wt[K * kTileCols];
+  constexpr int n = Word<T>::n, kGroups = kBlock / kRowLanes, kCols = kTileCols / kGroups;
+  const int l = threadIdx.x % kRowLanes, g = threadIdx.x / kRowLanes;
   const int64_t c0 = blockIdx.x * (int64_t)kTileCols;
+  for (int i = threadIdx.x; i < K * kTileCols; i += kBlock) {
+    const int64_t c = c0 + i % kTileCols;
+    const int r = c < batch ? row[i / kTileCols * batch + c] : -1;
+    at[i] = r < num_rows ? r : -1;
+    wt[i] = c < batch ? weight[i / kTileCols * batch + c] : 0.0f;
+  }
   float dot[kCols][K] = {};
   for (int f0 = 0; f0 < features; f0 += kTileWords * n) {
-    load_tile<T>(tile, dy, ld, f0, features, c0, batch);
+    load_tile<T, QUADS>(tile, dy, ld, f0, features, c0, batch);
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < kCols; ++q) {
-      const int c = warp + q * kWarps;
-      if (c0 + c < batch) {
+    for (int j = 0; j < K; ++j) {
+      uint32_t u[kCols][4];
 #pragma unroll
-        for (int j = 0; j < K; ++j) {
-          const int r = row[j * batch + c0 + c];
-          if (r < 0 || r >= num_rows) continue;
-          const float wt = weight[j * batch + c0 + c];
+      for (int q = 0; q < kCols; ++q) {
+        const int r = at[j * kTileCols + g + q * kGroups];
+        if (r >= 0) load_row<T, VEC>(rows + r * rows_ld, f0, features, whole, l, u[q]);
+      }
 #pragma unroll
-          for (int h = 0; h < kTileWords / 32; ++h) {
-            const int f = f0 + (h * 32 + lane) * n;
-            if (f < features) {
-              float d[n], v[n], o[n];
-              unpack<T>(tile[c * kPitch + h * 32 + lane], d);
-              unpack<T>(load_word<T>(rows + r * rows_ld, f, features, whole), v);
+      for (int q = 0; q < kCols; ++q) {
+        const int c = g + q * kGroups, r = at[j * kTileCols + c];
+        if (r < 0) continue;
+        const float w = wt[j * kTileCols + c];
+        uint32_t t[4], out[4];
+        read_tile<VEC>(tile, c, l, t);
 #pragma unroll
-              for (int i = 0; i < n; ++i) {
-                dot[q][j] = fmaf(d[i], v[i], dot[q][j]);
-                o[i] = wt * d[i];
-              }
-              store_word<T>(d_rows + r * d_ld, f, features, d_whole, pack<T>(o));
-            }
+        for (int k = 0; k < 4; ++k) {
+          float d[n], v[n], o[n];
+          unpack<T>(t[k], d);
+          unpack<T>(u[q][k], v);
+#pragma unroll
+          for (int h = 0; h < n; ++h) {
+            dot[q][j] = fmaf(d[h], v[h], dot[q][j]);
+            o[h] = w * d[h];
           }
+          out[k] = pack<T>(o);
         }
+        store_row<T, VEC>(d_rows + r * d_ld, f0, features, d_whole, l, out);
       }
     }
     __syncthreads();
   }
 #pragma unroll
   for (int q = 0; q < kCols; ++q) {
-    const int c = warp + q * kWarps;
+    const int c = g + q * kGroups;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
       float s = dot[q][j];
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-      if (lane == 0 && c0 + c < batch) d_weight[j * batch + c0 + c] = s;
+      for (int d = kRowLanes / 2; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+      if (l == 0 && c0 + c < batch) d_weight[j * batch + c0 + c] = s;
     }
   }
   zero_unused<T>(d_rows, d_ld, features, num_rows, used, blockIdx.x, gridDim.x);
@@ -254,6 +406,21 @@ ponni_b200_status check_columns(const char* what, int dtype, const void* columns
 
 template <class T> bool whole_words(const void* p, int64_t ld) {
   return sizeof(T) == 4 || (reinterpret_cast<uintptr_t>(p) % 4 == 0 && ld % 2 == 0);
+}
+
+bool whole_vectors(const void* p, int64_t ld, size_t z) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * z % 16 == 0;
+}
+// Four columns at once: 16 bytes of fp32, 8 of the 16-bit types.
+bool whole_quads(const void* p, int64_t ld, size_t z) {
+  return reinterpret_cast<uintptr_t>(p) % (4 * z) == 0 && ld % 4 == 0;
+}
+
+// f(QUADS, VEC) with the two flags as types.
+template <class F>
+void by_alignment(bool quads, bool vec, F&& f) {
+  if (quads) vec ? f(std::true_type(), std::true_type()) : f(std::true_type(), std::false_type());
+  else vec ? f(std::false_type(), std::true_type()) : f(std::false_type(), std::false_type());
 }
 
 template <class F>
@@ -282,9 +449,11 @@ ponni_b200_status ponni_b200_gather_columns(int dtype, const void* x, int64_t ld
       const int per = kTileWords * Word<T>::n;
       const dim3 grid((unsigned)((batch + kTileCols - 1) / kTileCols), (unsigned)((features + per - 1) / per));
       if (grid.y > 65535) return ops::fail(PONNI_B200_ERR_UNSUPPORTED, "gather_columns: too many features");
-      gather_kernel<T><<<grid, kBlock, 0, static_cast<cudaStream_t>(stream)>>>(
-          static_cast<const T*>(x), ld, features, batch, top_k, row, num_used, static_cast<T*>(rows), rows_ld,
-          batch * top_k, whole_words<T>(rows, rows_ld));
+      by_alignment(whole_quads(x, ld, sizeof(T)), whole_vectors(rows, rows_ld, sizeof(T)), [&](auto q, auto v) {
+        gather_kernel<T, q.value, v.value><<<grid, kBlock, 0, static_cast<cudaStream_t>(stream)>>>(
+            static_cast<const T*>(x), ld, features, batch, top_k, row, num_used, static_cast<T*>(rows), rows_ld,
+            batch * top_k, whole_words<T>(rows, rows_ld));
+      });
       return ops::launched("gather_columns");
     });
   });
@@ -301,9 +470,11 @@ ponni_b200_status ponni_b200_combine_rows(int dtype, const void* rows, int64_t r
       const int per = kTileWords * Word<T>::n;
       const dim3 grid((unsigned)((batch + kTileCols - 1) / kTileCols), (unsigned)((features + per - 1) / per));
       if (grid.y > 65535) return ops::fail(PONNI_B200_ERR_UNSUPPORTED, "combine_rows: too many features");
-      combine_kernel<T><<<grid, kBlock, 0, static_cast<cudaStream_t>(stream)>>>(
-          static_cast<const T*>(rows), rows_ld, batch * top_k, features, batch, top_k, row, weight, static_cast<T*>(y),
-          ld, whole_words<T>(rows, rows_ld));
+      by_alignment(whole_quads(y, ld, sizeof(T)), whole_vectors(rows, rows_ld, sizeof(T)), [&](auto q, auto v) {
+        combine_kernel<T, q.value, v.value><<<grid, kBlock, 0, static_cast<cudaStream_t>(stream)>>>(
+            static_cast<const T*>(rows), rows_ld, batch * top_k, features, batch, top_k, row, weight, static_cast<T*>(y),
+            ld, whole_words<T>(rows, rows_ld));
+      });
       return ops::launched("combine_rows");
     });
   });
@@ -326,24 +497,28 @@ ponni_b200_status ponni_b200_combine_rows_backward(int dtype, const void* d_y, i
       using T = decltype(t);
       const unsigned grid = (unsigned)((batch + kTileCols - 1) / kTileCols);
       cudaStream_t s = static_cast<cudaStream_t>(stream);
-      switch (top_k) {
-#define PB_CASE(K)                                                                                                   \
-  case K:                                                                                                            \
-    combine_backward_kernel<T, K><<<grid, kBlock, 0, s>>>(                                                         \
+      const bool vec = whole_vectors(rows, rows_ld, sizeof(T)) && whole_vectors(d_rows, d_ld, sizeof(T));
+      by_alignment(whole_quads(d_y, ld, sizeof(T)), vec, [&](auto q, auto v) {
+        constexpr bool Q = decltype(q)::value, V = decltype(v)::value;
+        switch (top_k) {
+#define PB_CASE(K)                                                                                                    \
+  case K:                                                                                                             \
+    combine_backward_kernel<T, K, Q, V><<<grid, kBlock, 0, s>>>(                                                      \
         static_cast<const T*>(d_y), ld, static_cast<const T*>(rows), rows_ld, batch * K, features, batch, row, weight, \
-        num_used, static_cast<T*>(d_rows), d_ld, d_weight, whole_words<T>(rows, rows_ld),                             \
-        whole_words<T>(d_rows, d_ld));                                                                                \
+        num_used, static_cast<T*>(d_rows), d_ld, d_weight, whole_words<T>(rows, rows_ld),                              \
+        whole_words<T>(d_rows, d_ld));                                                                                 \
     break
-        PB_CASE(1);
-        PB_CASE(2);
-        PB_CASE(3);
-        PB_CASE(4);
-        PB_CASE(5);
-        PB_CASE(6);
-        PB_CASE(7);
-        PB_CASE(8);
+          PB_CASE(1);
+          PB_CASE(2);
+          PB_CASE(3);
+          PB_CASE(4);
+          PB_CASE(5);
+          PB_CASE(6);
+          PB_CASE(7);
+          PB_CASE(8);
 #undef PB_CASE
-      }
+        }
+      });
       return ops::launched("combine_rows_backward");
     });
   });
