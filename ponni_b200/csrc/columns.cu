@@ -29,6 +29,7 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kWarps = kBlock / 32;
 constexpr int kTileCols = 64;
+constexpr int kBackCols = 32;  // of combine_backward_kernel
 constexpr int kTileWords = 64;
 constexpr int kRowLanes = 16;  // lanes that take a row
 
@@ -91,6 +92,7 @@ __device__ __forceinline__ void turn_in(const T* __restrict__ x, int64_t ld, int
     u[2] = v.z;
     u[3] = v.w;
   } else {
+    static_assert(sizeof(T) == 2, "16-bit features");
     const uint2 a = f < features ? __ldg(reinterpret_cast<const uint2*>(x + f * ld)) : make_uint2(0, 0);
     const uint2 b = f + 1 < features ? __ldg(reinterpret_cast<const uint2*>(x + (f + 1) * ld)) : make_uint2(0, 0);
     u[0] = __byte_perm(a.x, b.x, 0x5410);
@@ -112,36 +114,36 @@ __device__ __forceinline__ void turn_out(T* __restrict__ y, int64_t ld, int f, i
   }
 }
 
-// Tile of x (kTileCols columns from c0, kTileWords words of features from f0)
+// Tile of x (COLS columns from c0, kTileWords words of features from f0)
 // into shared memory; QUADS: the batch allows four columns at once.
-template <class T, bool QUADS>
+template <class T, bool QUADS, int COLS>
 __device__ __forceinline__ void load_tile(uint32_t* tile, const T* __restrict__ x, int64_t ld, int f0, int features,
                                           int64_t c0, int64_t batch) {
   constexpr int n = Word<T>::n;
-  if (QUADS && c0 + kTileCols <= batch) {
-    constexpr int kPer = kTileWords * (kTileCols / 4) / kBlock;
+  if (QUADS && c0 + COLS <= batch) {
+    constexpr int kPer = kTileWords * (COLS / 4) / kBlock;
     uint32_t u[kPer][4];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int it = i * kBlock + threadIdx.x, q = it % (kTileCols / 4), w = it / (kTileCols / 4);
+      const int it = i * kBlock + threadIdx.x, q = it % (COLS / 4), w = it / (COLS / 4);
       turn_in<T>(x + c0 + 4 * q, ld, f0 + w * n, features, u[i]);
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int it = i * kBlock + threadIdx.x, q = it % (kTileCols / 4), w = it / (kTileCols / 4);
+      const int it = i * kBlock + threadIdx.x, q = it % (COLS / 4), w = it / (COLS / 4);
 #pragma unroll
       for (int k = 0; k < 4; ++k) tile[place(4 * q + k, w)] = u[i][k];
     }
     return;
   }
-  constexpr int kPer = kTileWords * kTileCols / kBlock;
+  constexpr int kPer = kTileWords * COLS / kBlock;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int i0 = 0; i0 < kPer; i0 += 8) {
     Word<T> v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int it = (i0 + i) * kWarps + warp, c = it % 2 * 32 + lane, w = it / 2;
+      const int it = (i0 + i) * kWarps + warp, c = it % (COLS / 32) * 32 + lane, w = it / (COLS / 32);
 #pragma unroll
       for (int k = 0; k < n; ++k) {
         const int f = f0 + w * n + k;
@@ -150,7 +152,7 @@ __device__ __forceinline__ void load_tile(uint32_t* tile, const T* __restrict__ 
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int it = (i0 + i) * kWarps + warp, c = it % 2 * 32 + lane, w = it / 2;
+      const int it = (i0 + i) * kWarps + warp, c = it % (COLS / 32) * 32 + lane, w = it / (COLS / 32);
       tile[place(c, w)] = *reinterpret_cast<uint32_t*>(&v[i]);
     }
   }
@@ -194,16 +196,16 @@ __device__ __forceinline__ void store_row(T* __restrict__ row, int f0, int featu
 }
 template <bool VEC>
 __device__ __forceinline__ void read_tile(const uint32_t* tile, int c, int l, uint32_t (&u)[4]) {
-  if (VEC) {
+  if constexpr (VEC) {
     const uint4 v = *reinterpret_cast<const uint4*>(tile + place(c, 4 * l));
     u[0] = v.x;
     u[1] = v.y;
     u[2] = v.z;
     u[3] = v.w;
-    return;
-  }
+  } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) u[i] = tile[place(c, row_word<VEC>(l, i))];
+    for (int i = 0; i < 4; ++i) u[i] = tile[place(c, row_word<VEC>(l, i))];
+  }
 }
 
 // Rows that no choice fills: the ones past the last group.
@@ -231,7 +233,7 @@ __global__ void __launch_bounds__(kBlock)
     const int r = c < batch ? row[i / kTileCols * batch + c] : -1;
     at[i] = r < num_rows ? r : -1;
   }
-  load_tile<T, QUADS>(tile, x, ld, f0, features, c0, batch);
+  load_tile<T, QUADS, kTileCols>(tile, x, ld, f0, features, c0, batch);
   __syncthreads();
 #pragma unroll
   for (int c = g; c < kTileCols; c += kBlock / kRowLanes) {
@@ -319,50 +321,63 @@ __global__ void __launch_bounds__(kBlock)
   }
 }
 
-// A block holds its 64 columns through all feature tiles, so that a dot
-// product is summed by 16 lanes in a fixed order.
+// A block holds its columns through all feature tiles, so that a dot product is
+// summed by 16 lanes in a fixed order.  Bound by the latency of the row loads:
+// 32 columns a block leave registers for four blocks an SM, and all row loads of
+// a tile go out before it is turned (49999 x 1001 fp32, three rows a column: 402 us
+// with 64 columns and two blocks, 348 with 32 and four, 280 with the early loads).
 template <class T, int K, bool QUADS, bool VEC>
-__global__ void __launch_bounds__(kBlock)
+__global__ void __launch_bounds__(kBlock, 4)
     combine_backward_kernel(const T* __restrict__ dy, int64_t ld, const T* __restrict__ rows, int64_t rows_ld,
                             int64_t num_rows, int features, int64_t batch, const int* __restrict__ row,
                             const float* __restrict__ weight, const int* __restrict__ used, T* __restrict__ d_rows,
                             int64_t d_ld, float* __restrict__ d_weight, int whole, int d_whole) {
-  __shared__ __align__(16) uint32_t tile[kTileCols * kTileWords];
-  __shared__ int at[K * kTileCols];
-  __shared__ float wt[K * kTileCols];
-  constexpr int n = Word<T>::n, kGroups = kBlock / kRowLanes, kCols = kTileCols / kGroups;
+  __shared__ __align__(16) uint32_t tile[kBackCols * kTileWords];
+  __shared__ int at[K * kBackCols];
+  __shared__ float wt[K * kBackCols];
+  constexpr int n = Word<T>::n, kGroups = kBlock / kRowLanes, kCols = kBackCols / kGroups;
   const int l = threadIdx.x % kRowLanes, g = threadIdx.x / kRowLanes;
-  const int64_t c0 = blockIdx.x * (int64_t)kTileCols;
-  for (int i = threadIdx.x; i < K * kTileCols; i += kBlock) {
-    const int64_t c = c0 + i % kTileCols;
-    const int r = c < batch ? row[i / kTileCols * batch + c] : -1;
+  const int64_t c0 = blockIdx.x * (int64_t)kBackCols;
+  for (int i = threadIdx.x; i < K * kBackCols; i += kBlock) {
+    const int64_t c = c0 + i % kBackCols;
+    const int r = c < batch ? row[i / kBackCols * batch + c] : -1;
     at[i] = r < num_rows ? r : -1;
-    wt[i] = c < batch ? weight[i / kTileCols * batch + c] : 0.0f;
+    wt[i] = c < batch ? weight[i / kBackCols * batch + c] : 0.0f;
   }
+  __syncthreads();
   float dot[kCols][K] = {};
   for (int f0 = 0; f0 < features; f0 += kTileWords * n) {
-    load_tile<T, QUADS>(tile, dy, ld, f0, features, c0, batch);
+    // All row loads go out before the tile's (K <= 4: the registers allow it).
+    constexpr bool kAhead = K <= 4;
+    uint32_t u[kAhead ? K : 1][kCols][4];
+    auto fetch = [&](int j) {
+#pragma unroll
+      for (int q = 0; q < kCols; ++q) {
+        const int r = at[j * kBackCols + g + q * kGroups];
+        if (r >= 0) load_row<T, VEC>(rows + r * rows_ld, f0, features, whole, l, u[kAhead ? j : 0][q]);
+      }
+    };
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int j = 0; j < K; ++j) fetch(j);
+    }
+    load_tile<T, QUADS, kBackCols>(tile, dy, ld, f0, features, c0, batch);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      uint32_t u[kCols][4];
+      if constexpr (!kAhead) fetch(j);
 #pragma unroll
       for (int q = 0; q < kCols; ++q) {
-        const int r = at[j * kTileCols + g + q * kGroups];
-        if (r >= 0) load_row<T, VEC>(rows + r * rows_ld, f0, features, whole, l, u[q]);
-      }
-#pragma unroll
-      for (int q = 0; q < kCols; ++q) {
-        const int c = g + q * kGroups, r = at[j * kTileCols + c];
+        const int c = g + q * kGroups, r = at[j * kBackCols + c];
         if (r < 0) continue;
-        const float w = wt[j * kTileCols + c];
+        const float w = wt[j * kBackCols + c];
         uint32_t t[4], out[4];
         read_tile<VEC>(tile, c, l, t);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           float d[n], v[n], o[n];
           unpack<T>(t[k], d);
-          unpack<T>(u[q][k], v);
+          unpack<T>(u[kAhead ? j : 0][q][k], v);
 #pragma unroll
           for (int h = 0; h < n; ++h) {
             dot[q][j] = fmaf(d[h], v[h], dot[q][j]);
@@ -495,7 +510,7 @@ ponni_b200_status ponni_b200_combine_rows_backward(int dtype, const void* d_y, i
       return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "combine_rows_backward: row stride smaller than the row");
     return by_type(dtype, [&](auto t) -> ponni_b200_status {
       using T = decltype(t);
-      const unsigned grid = (unsigned)((batch + kTileCols - 1) / kTileCols);
+      const unsigned grid = (unsigned)((batch + kBackCols - 1) / kBackCols);
       cudaStream_t s = static_cast<cudaStream_t>(stream);
       const bool vec = whole_vectors(rows, rows_ld, sizeof(T)) && whole_vectors(d_rows, d_ld, sizeof(T));
       by_alignment(whole_quads(d_y, ld, sizeof(T)), vec, [&](auto q, auto v) {

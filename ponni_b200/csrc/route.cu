@@ -11,6 +11,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "device_math.cuh"
 #include "operators.h"
@@ -27,7 +28,19 @@ __device__ __forceinline__ float logit(const T* p) {
   return v == v ? v : -INFINITY;
 }
 
-// Choice and weights of one column; K is the number of choices.
+// exp(v - best) for v <= best, 1 where they are equal (both may be infinite);
+// ex2 within 2^-22 of its value.  best is at least -FLT_MAX, so that v = -inf gives 0.
+__device__ __forceinline__ float from_best(float v, float best) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"((v - best) * 1.4426950408889634f));
+  return v == best ? 1.0f : y;
+}
+__device__ __forceinline__ float at_least_finite(float best) { return fmaxf(best, -3.402823466e38f); }
+
+// Choice and weights of one column; K is the number of choices.  Logits come in
+// chunks of kChunk, the next chunk's loads ahead of this one's work.  Insertion
+// has no branches: some lane of a warp inserts at nearly every expert.
+constexpr int kChunk = 8;
 template <class T, int K>
 __device__ __forceinline__ void choose(const T* __restrict__ x, int64_t ld, int experts, bool over_all, int (&idx)[K],
                                        float (&w)[K]) {
@@ -37,39 +50,45 @@ __device__ __forceinline__ void choose(const T* __restrict__ x, int64_t ld, int 
     top[j] = -INFINITY;
     idx[j] = -1;
   }
-  float sum = 0.0f;  // of exp(x - top[0]) over the experts seen
-  auto take = [&](float v, int e) {
-    if (over_all && v > -INFINITY) {
-      if (v > top[0]) sum = (top[0] > -INFINITY ? sum * expf(top[0] - v) : 0.0f) + 1.0f;
-      else sum += v == top[0] ? 1.0f : expf(v - top[0]);
-    }
-    if (v > top[K - 1]) {
-      top[K - 1] = v;
-      idx[K - 1] = e;
+  float sum = 0.0f, best = -3.402823466e38f;  // sum of exp(x - best) over the experts seen
+  float ahead[kChunk];
+  auto load = [&](int e0) {
 #pragma unroll
-      for (int j = K - 1; j > 0; --j) {
-        if (top[j] > top[j - 1]) {
-          const float tv = top[j];
-          top[j] = top[j - 1];
-          top[j - 1] = tv;
-          const int ti = idx[j];
-          idx[j] = idx[j - 1];
-          idx[j - 1] = ti;
-        }
+    for (int u = 0; u < kChunk; ++u) ahead[u] = e0 + u < experts ? logit(x + (int64_t)(e0 + u) * ld) : -INFINITY;
+  };
+  load(0);
+  for (int e0 = 0; e0 < experts; e0 += kChunk) {
+    float v[kChunk];
+#pragma unroll
+    for (int u = 0; u < kChunk; ++u) v[u] = ahead[u];
+    if (e0 + kChunk < experts) load(e0 + kChunk);
+    if (over_all) {
+      float now = best;
+#pragma unroll
+      for (int u = 0; u < kChunk; ++u) now = fmaxf(now, v[u]);
+      sum *= from_best(best, now);
+      best = now;
+#pragma unroll
+      for (int u = 0; u < kChunk; ++u) sum += from_best(v[u], best);
+    }
+#pragma unroll
+    for (int u = 0; u < kChunk; ++u) {
+      // Behind every entry that is at least as large (of equal logits the lower
+      // expert stays first); the entries below move down one place.
+      bool up[K];
+#pragma unroll
+      for (int j = 0; j < K; ++j) up[j] = v[u] > top[j];
+#pragma unroll
+      for (int j = K - 1; j >= 0; --j) {
+        const bool shift = j > 0 && up[j > 0 ? j - 1 : 0];
+        top[j] = shift ? top[j > 0 ? j - 1 : 0] : up[j] ? v[u] : top[j];
+        idx[j] = shift ? idx[j > 0 ? j - 1 : 0] : up[j] ? e0 + u : idx[j];
       }
     }
-  };
-  int e = 0;
-  for (; e + 8 <= experts; e += 8) {
-    float v[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = logit(x + (int64_t)(e + u) * ld);
-#pragma unroll
-    for (int u = 0; u < 8; ++u) take(v[u], e + u);
   }
-  for (; e < experts; ++e) take(logit(x + (int64_t)e * ld), e);
+  best = at_least_finite(top[0]);
 #pragma unroll
-  for (int j = 0; j < K; ++j) w[j] = idx[j] < 0 ? 0.0f : top[j] == top[0] ? 1.0f : expf(top[j] - top[0]);
+  for (int j = 0; j < K; ++j) w[j] = idx[j] < 0 ? 0.0f : from_best(top[j], best);
   if (!over_all) {
     sum = 0.0f;
 #pragma unroll
@@ -146,17 +165,58 @@ __global__ void __launch_bounds__(kBlock) scan_kernel(int* __restrict__ counts, 
   if (threadIdx.x == 0) totals[blockIdx.x] = carry;
 }
 
-// Rows of this block's choices.  Within a tile of kBlock columns the rank
-// of a choice is the number of earlier columns that chose the same expert
-// (at most once each): a lane mask per warp and expert in shared memory.
+// Rows of the choices of columns [c0, c1), given the next row of each expert.
+// Within a tile of kBlock columns the rank of a choice is the number of earlier
+// columns that chose the same expert (at most once each): a lane mask per warp
+// and expert in shared memory, zero on entry and on return.
+__device__ __forceinline__ void place(const int* expert, int experts, int top_k, int64_t batch, int64_t c0, int64_t c1,
+                                      int* next, unsigned* mask, int* row, int* column) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int64_t t0 = c0; t0 < c1; t0 += kBlock) {
+    const int64_t b = t0 + threadIdx.x;
+    int es[ops::kMaxTopK];
+#pragma unroll
+    for (int j = 0; j < ops::kMaxTopK; ++j) es[j] = j < top_k && b < c1 ? expert[j * batch + b] : -1;
+#pragma unroll
+    for (int j = 0; j < ops::kMaxTopK; ++j)
+      if (es[j] >= 0) atomicOr(&mask[warp * experts + es[j]], 1u << lane);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ops::kMaxTopK; ++j) {
+      if (j >= top_k || b >= c1) continue;
+      const int e = es[j];
+      int r = -1;
+      if (e >= 0) {
+        r = next[e] + __popc(mask[warp * experts + e] & ((1u << lane) - 1u));
+        for (int w = 0; w < warp; ++w) r += __popc(mask[w * experts + e]);
+        column[r] = (int)b;
+      }
+      row[j * batch + b] = r;
+    }
+    __syncthreads();
+    if (t0 + kBlock >= c1) break;
+    for (int e = threadIdx.x; e < experts; e += kBlock) {
+      int n = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        n += __popc(mask[w * experts + e]);
+        mask[w * experts + e] = 0;
+      }
+      next[e] += n;
+    }
+    __syncthreads();
+  }
+}
+
 __global__ void __launch_bounds__(kBlock)
     place_kernel(const int* __restrict__ expert, int experts, int top_k, int64_t batch, int64_t per_block,
                  const int* __restrict__ counts, const int* __restrict__ totals, int* __restrict__ row,
                  int* __restrict__ column, int* __restrict__ offset) {
   extern __shared__ int sm[];
   __shared__ int warp_sums[kWarps];
-  int* next = sm;                                                  // [experts]: next row of each expert
+  int* next = sm;                                              // [experts]: next row of each expert
   unsigned* mask = reinterpret_cast<unsigned*>(sm + experts);  // [kWarps][experts]
+  ops::let_successor_start();
   for (int i = threadIdx.x; i < kWarps * experts; i += kBlock) mask[i] = 0;
   ops::wait_for_predecessor();
   int carry = 0;
@@ -175,101 +235,99 @@ __global__ void __launch_bounds__(kBlock)
        i += (int64_t)gridDim.x * kBlock)
     column[i] = -1;
   __syncthreads();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c0 = blockIdx.x * per_block, c1 = min(batch, c0 + per_block);
-  for (int64_t t0 = c0; t0 < c1; t0 += kBlock) {
-    const int64_t b = t0 + threadIdx.x;
-    for (int j = 0; j < top_k; ++j) {
-      const int e = b < c1 ? expert[j * batch + b] : -1;
-      if (e >= 0) atomicOr(&mask[warp * experts + e], 1u << lane);
-    }
-    __syncthreads();
-    if (b < c1) {
-      for (int j = 0; j < top_k; ++j) {
-        const int e = expert[j * batch + b];
-        int r = -1;
-        if (e >= 0) {
-          r = next[e] + __popc(mask[warp * experts + e] & ((1u << lane) - 1u));
-          for (int w = 0; w < warp; ++w) r += __popc(mask[w * experts + e]);
-          column[r] = (int)b;
-        }
-        row[j * batch + b] = r;
-      }
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < experts; e += kBlock) {
-      int n = 0;
+  const int64_t c0 = blockIdx.x * per_block;
+  place(expert, experts, top_k, batch, c0, min(batch, c0 + per_block), next, mask, row, column);
+}
+
+// All of it in one block, for batches of at most kOneBlock columns: three
+// dependent launches cost more than the work of a few tiles.
+constexpr int64_t kOneBlock = 2 * kBlock;
+template <class T, int K>
+__global__ void __launch_bounds__(kBlock)
+    route_one_block_kernel(const T* __restrict__ x, int64_t ld, int experts, int batch, int over_all, int* expert,
+                           float* __restrict__ weight, int* row, int* column, int* __restrict__ offset) {
+  extern __shared__ int sm[];
+  __shared__ int warp_sums[kWarps];
+  int* next = sm;
+  unsigned* mask = reinterpret_cast<unsigned*>(sm + experts);
+  for (int i = threadIdx.x; i < experts; i += kBlock) next[i] = 0;
+  for (int i = threadIdx.x; i < kWarps * experts; i += kBlock) mask[i] = 0;
+  __syncthreads();
+  for (int b = threadIdx.x; b < batch; b += kBlock) {
+    int idx[K];
+    float w[K];
+    choose<T, K>(x + b, ld, experts, over_all, idx, w);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        n += __popc(mask[w * experts + e]);
-        mask[w * experts + e] = 0;
-      }
-      next[e] += n;
+    for (int j = 0; j < K; ++j) {
+      expert[j * batch + b] = idx[j];
+      weight[j * batch + b] = w[j];
+      if (idx[j] >= 0) atomicAdd(&next[idx[j]], 1);
     }
-    __syncthreads();
   }
+  __syncthreads();
+  int carry = 0;
+  for (int e0 = 0; e0 < experts; e0 += kBlock) {
+    const int e = e0 + threadIdx.x;
+    int total;
+    const int before = carry + block_scan(e < experts ? next[e] : 0, warp_sums, total);
+    if (e < experts) offset[e] = next[e] = before;
+    carry += total;
+  }
+  if (threadIdx.x == 0) offset[experts] = carry;
+  for (int i = carry + threadIdx.x; i < batch * K; i += kBlock) column[i] = -1;
+  __syncthreads();
+  place(expert, experts, K, batch, 0, batch, next, mask, row, column);
 }
 
 // d_x[e][b] = p_e (d_p_e - sum_j w_j d_w_j), d_p_e = d_w_j for the chosen
 // experts and 0 for others; p is the softmax over all experts or over the
 // chosen ones.  Over all: the first choice has t = 1, so p_e = t_e weight_0
 // and no second sum is needed.
-template <class T>
+//
+// A thread takes one column and kBackPart experts: all of them as if not
+// chosen first (their logits loaded at once), then the chosen ones again.
+constexpr int kBackPart = 16;
+template <class T, int K>
 __global__ void __launch_bounds__(kBlock)
-    route_backward_kernel(const T* __restrict__ x, int64_t ld, int experts, int top_k, int64_t batch, int over_all,
+    route_backward_kernel(const T* __restrict__ x, int64_t ld, int experts, int64_t batch, int over_all,
                           const int* __restrict__ expert, const float* __restrict__ weight,
-                          const float* __restrict__ d_weight, T* __restrict__ dx, int64_t d_ld, int per_part) {
+                          const float* __restrict__ d_weight, T* __restrict__ dx, int64_t d_ld) {
   const int64_t b = blockIdx.x * (int64_t)kBlock + threadIdx.x;
   if (b >= batch) return;
-  int idx[ops::kMaxTopK];
-  float g[ops::kMaxTopK];
-  float mean = 0.0f;
+  const int e0 = blockIdx.y * kBackPart;
+  float v[kBackPart];
+  if (over_all) {
 #pragma unroll
-  for (int j = 0; j < ops::kMaxTopK; ++j) {
-    idx[j] = -1;
-    g[j] = 0.0f;
-    if (j < top_k) {
-      idx[j] = expert[j * batch + b];
-      if (idx[j] >= 0) {
-        const float w = weight[j * batch + b];
-        g[j] = w * d_weight[j * batch + b];
-        mean += g[j];
-      }
-    }
+    for (int u = 0; u < kBackPart; ++u) v[u] = e0 + u < experts ? logit(x + (int64_t)(e0 + u) * ld + b) : -INFINITY;
   }
-  const int e0 = blockIdx.y * per_part, e1 = min(experts, e0 + per_part);
+  int idx[K];
+  float w[K], g[K], mean = 0.0f;
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    idx[j] = expert[j * batch + b];
+    w[j] = weight[j * batch + b];
+    g[j] = idx[j] >= 0 ? w[j] * d_weight[j * batch + b] : 0.0f;
+    mean += g[j];
+  }
   const bool any = idx[0] >= 0;
-  const float best = any && over_all ? logit(x + idx[0] * ld + b) : 0.0f;
-  const float scale = any && over_all ? weight[b] : 0.0f;
-  for (int e = e0; e < e1; ++e) {
-    float d = 0.0f;
-    if (any && over_all) {
-      const float v = logit(x + e * ld + b);
-      const float p = v == best ? scale : expf(v - best) * scale;
-      d = -p * mean;
-    }
+  const float best = any && over_all ? logit(x + (int64_t)idx[0] * ld + b) : 0.0f;
+  const float scale = any ? -w[0] * mean : 0.0f;
 #pragma unroll
-    for (int j = 0; j < ops::kMaxTopK; ++j)
-      if (idx[j] == e) d = over_all ? d + g[j] : g[j] - weight[j * batch + b] * mean;
-    dx[e * d_ld + b] = Num<T>::from_c(d);
-  }
+  for (int u = 0; u < kBackPart; ++u)
+    if (e0 + u < experts) dx[(e0 + u) * d_ld + b] = Num<T>::from_c(over_all && any ? from_best(v[u], best) * scale : 0.0f);
+#pragma unroll
+  for (int j = 0; j < K; ++j)
+    if (idx[j] >= e0 && idx[j] < e0 + kBackPart) dx[(int64_t)idx[j] * d_ld + b] = Num<T>::from_c(g[j] - w[j] * mean);
 }
 
 int64_t blocks_of(int64_t batch) { return std::min<int64_t>((batch + kBlock - 1) / kBlock, 592); }
 
-template <class T, int K>
-cudaError_t launch_choose(const void* x, int64_t ld, int experts, int64_t batch, int64_t per_block, int blocks, int all,
-                          int* expert, float* weight, int* counts, cudaStream_t s) {
-  choose_kernel<T, K><<<blocks, kBlock, experts * sizeof(int), s>>>(static_cast<const T*>(x), ld, experts, batch,
-                                                                     per_block, all, expert, weight, counts);
-  return cudaGetLastError();
-}
-template <class T>
-cudaError_t launch_choose_k(int k, const void* x, int64_t ld, int experts, int64_t batch, int64_t per_block, int blocks,
-                            int all, int* expert, float* weight, int* counts, cudaStream_t s) {
-  switch (k) {
+// f(T, K) for the type and the number of choices.
+template <class T, class F>
+ponni_b200_status by_top_k(int top_k, F&& f) {
+  switch (top_k) {
 #define PB_CASE(K) \
-  case K: return launch_choose<T, K>(x, ld, experts, batch, per_block, blocks, all, expert, weight, counts, s)
+  case K: return f(T(), std::integral_constant<int, K>())
     PB_CASE(1);
     PB_CASE(2);
     PB_CASE(3);
@@ -280,7 +338,13 @@ cudaError_t launch_choose_k(int k, const void* x, int64_t ld, int experts, int64
     PB_CASE(8);
 #undef PB_CASE
   }
-  return cudaErrorInvalidValue;
+  return ops::fail(PONNI_B200_ERR_UNSUPPORTED, "route: top_k must be 1 to 8");
+}
+template <class F>
+ponni_b200_status by_type(int dtype, int top_k, F&& f) {
+  if (dtype == PONNI_B200_F32) return by_top_k<float>(top_k, f);
+  if (dtype == PONNI_B200_F16) return by_top_k<__half>(top_k, f);
+  return by_top_k<__nv_bfloat16>(top_k, f);
 }
 
 ponni_b200_status check_route(int dtype, const void* logits, int64_t ld, int experts, int top_k, int64_t batch,
@@ -324,29 +388,32 @@ ponni_b200_status ponni_b200_route_columns(int dtype, const void* logits, int64_
     if (!workspace || workspace_bytes < ponni_b200_route_workspace(num_experts, batch))
       return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route: workspace is too small");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const int64_t tiles = (batch + kBlock - 1) / kBlock;
-    const int64_t most = blocks_of(batch);
-    const int64_t per_block = (tiles + most - 1) / most * kBlock;
-    const int blocks = (int)((batch + per_block - 1) / per_block);
-    int* counts = static_cast<int*>(workspace);
-    int* totals = counts + (int64_t)num_experts * blocks;
     const int all = normalise == PONNI_B200_ROUTE_ALL;
-    cudaError_t e = cudaErrorInvalidValue;
-    if (dtype == PONNI_B200_F32)
-      e = launch_choose_k<float>(top_k, logits, ld, num_experts, batch, per_block, blocks, all, expert, weight, counts, s);
-    else if (dtype == PONNI_B200_F16)
-      e = launch_choose_k<__half>(top_k, logits, ld, num_experts, batch, per_block, blocks, all, expert, weight, counts, s);
-    else
-      e = launch_choose_k<__nv_bfloat16>(top_k, logits, ld, num_experts, batch, per_block, blocks, all, expert, weight,
-                                         counts, s);
-    if (e == cudaSuccess)
-      e = ops::launch_after(scan_kernel, dim3(num_experts), dim3(kBlock), 0, s, counts, blocks, totals);
-    if (e == cudaSuccess)
-      e = ops::launch_after(place_kernel, dim3(blocks), dim3(kBlock), (size_t)num_experts * (kWarps + 1) * sizeof(int),
-                            s, (const int*)expert, num_experts, top_k, batch, per_block, (const int*)counts,
-                            (const int*)totals, row, column, offset);
-    if (e != cudaSuccess) return ops::fail_cuda(e, "route_columns");
-    return ops::launched("route_columns");
+    const size_t place_smem = (size_t)num_experts * (kWarps + 1) * sizeof(int);
+    return by_type(dtype, top_k, [&](auto t, auto k) -> ponni_b200_status {
+      using T = decltype(t);
+      constexpr int K = decltype(k)::value;
+      const T* x = static_cast<const T*>(logits);
+      if (batch <= kOneBlock) {
+        route_one_block_kernel<T, K><<<1, kBlock, place_smem, s>>>(x, ld, num_experts, (int)batch, all, expert, weight,
+                                                                  row, column, offset);
+        return ops::launched("route_columns");
+      }
+      const int64_t tiles = (batch + kBlock - 1) / kBlock, most = blocks_of(batch);
+      const int64_t per_block = (tiles + most - 1) / most * kBlock;
+      const int blocks = (int)((batch + per_block - 1) / per_block);
+      int* counts = static_cast<int*>(workspace);
+      int* totals = counts + (int64_t)num_experts * blocks;
+      choose_kernel<T, K><<<blocks, kBlock, num_experts * sizeof(int), s>>>(x, ld, num_experts, batch, per_block, all,
+                                                                           expert, weight, counts);
+      cudaError_t e = cudaGetLastError();
+      if (e == cudaSuccess)
+        e = ops::launch_after(scan_kernel, dim3(num_experts), dim3(kBlock), 0, s, counts, blocks, totals);
+      if (e == cudaSuccess)
+        e = ops::launch_after(place_kernel, dim3(blocks), dim3(kBlock), place_smem, s, (const int*)expert, num_experts,
+                              top_k, batch, per_block, (const int*)counts, (const int*)totals, row, column, offset);
+      return e == cudaSuccess ? PONNI_B200_OK : ops::fail_cuda(e, "route_columns");
+    });
   });
 }
 
@@ -362,21 +429,15 @@ ponni_b200_status ponni_b200_route_columns_backward(int dtype, const void* logit
     if (d_ld < batch)
       return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route backward: row stride smaller than the batch size");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const int per_part = 16;
-    const dim3 grid((unsigned)((batch + kBlock - 1) / kBlock), (unsigned)((num_experts + per_part - 1) / per_part));
+    const dim3 grid((unsigned)((batch + kBlock - 1) / kBlock), (unsigned)((num_experts + kBackPart - 1) / kBackPart));
     const int all = normalise == PONNI_B200_ROUTE_ALL;
-    if (dtype == PONNI_B200_F32)
-      route_backward_kernel<float><<<grid, kBlock, 0, s>>>((const float*)logits, ld, num_experts, top_k, batch, all,
-                                                             expert, weight, d_weight, (float*)d_logits, d_ld, per_part);
-    else if (dtype == PONNI_B200_F16)
-      route_backward_kernel<__half><<<grid, kBlock, 0, s>>>((const __half*)logits, ld, num_experts, top_k, batch, all,
-                                                              expert, weight, d_weight, (__half*)d_logits, d_ld,
-                                                              per_part);
-    else
-      route_backward_kernel<__nv_bfloat16><<<grid, kBlock, 0, s>>>(
-          (const __nv_bfloat16*)logits, ld, num_experts, top_k, batch, all, expert, weight, d_weight,
-          (__nv_bfloat16*)d_logits, d_ld, per_part);
-    return ops::launched("route_columns_backward");
+    return by_type(dtype, top_k, [&](auto t, auto k) -> ponni_b200_status {
+      using T = decltype(t);
+      route_backward_kernel<T, decltype(k)::value><<<grid, kBlock, 0, s>>>(
+          static_cast<const T*>(logits), ld, num_experts, batch, all, expert, weight, d_weight,
+          static_cast<T*>(d_logits), d_ld);
+      return ops::launched("route_columns_backward");
+    });
   });
 }
 
