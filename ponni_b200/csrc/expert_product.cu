@@ -37,6 +37,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cstdlib>
 #include <cstring>
 #include <type_traits>
 
@@ -79,11 +80,14 @@ struct Args {
   int* error;
 };
 
-template <class T, int P, int BN> struct Shape {
+// CG: CTAs that share a tile.  With two (cta_group::2) the tile is 256 x BN, each
+// CTA holds its 128 rows of A, half of B's columns and its 128 rows of the sums.
+template <int P, int BN, int CG> struct Shape {
+  static constexpr int b_rows = BN / CG;
   static constexpr int a_bytes = P * kBM * kBK * 2;
-  static constexpr int b_bytes = P * BN * kBK * 2;
+  static constexpr int b_bytes = P * b_rows * kBK * 2;
   static constexpr int stage_bytes = a_bytes + b_bytes;
-  static constexpr int acc_cols = P == 3 ? 128 : 256;
+  static constexpr int acc_cols = P == 3 && BN <= 128 ? 128 : 256;
   static constexpr int acc_bufs = 512 / acc_cols;
   // Epilogue warps: four lane quarters (a warp reads the TMEM lanes of its
   // number modulo 4) times `parts` strips of columns.
@@ -97,6 +101,20 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       "[%5];\n" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
+}
+
+// The same in a pair: the bytes are counted on a barrier of the pair's first CTA.
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+      "%4}], [%5];\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+// Arrival on another CTA's barrier of what this thread has read or written in
+// tensor memory or shared memory (ordered by the tcgen05 and proxy fences before it).
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_addr) : "memory");
 }
 
 // Check of the offsets by one block (the groups are clamped whatever they hold).
@@ -115,26 +133,26 @@ struct Tile {
   int64_t slot;  // kWeights, split: the unit's partial sums
 };
 
-// The tile sequence of this CTA: blockIdx.x, blockIdx.x + gridDim.x, ... of all
-// tiles, experts in order, row tiles innermost (neighbouring CTAs share the
-// weight tile).
-template <int MODE, int BN> struct Tiles {
+// The tile sequence of this CTA (pair): its number, then every further one that
+// many CTAs (pairs) on, of all tiles: experts in order, row tiles innermost
+// (neighbours share the weight tile).  m0 is the CTA's own first row.
+template <int MODE, int BN, int CG> struct Tiles {
   const int* lo;
   const int* hi;
   int experts, m_tiles, n_tiles, k_blocks, unit_rows;
   int e = 0;
   int64_t t, base = 0;
 
-  __device__ Tiles(const Args& p, const int* lo_, const int* hi_) : lo(lo_), hi(hi_), experts(p.experts), t(blockIdx.x) {
+  __device__ Tiles(const Args& p, const int* lo_, const int* hi_) : lo(lo_), hi(hi_), experts(p.experts), t(blockIdx.x / CG) {
     const int n = MODE == kRows ? p.inputs : p.outputs, k = MODE == kForward ? p.inputs : p.outputs;
-    m_tiles = (p.inputs + kBM - 1) / kBM;
+    m_tiles = (p.inputs + CG * kBM - 1) / (CG * kBM);
     n_tiles = (n + BN - 1) / BN;
     k_blocks = (k + kBK - 1) / kBK;
     unit_rows = p.unit_rows;
   }
   __device__ __forceinline__ int64_t count(int i) const {
     const int rows = hi[i] - lo[i];
-    if (MODE != kWeights) return (int64_t)((rows + kBM - 1) / kBM) * n_tiles;
+    if (MODE != kWeights) return (int64_t)((rows + CG * kBM - 1) / (CG * kBM)) * n_tiles;
     return (int64_t)(unit_rows ? (rows + unit_rows - 1) / unit_rows : 1) * m_tiles * n_tiles;
   }
   __device__ __forceinline__ bool next(Tile& v) {
@@ -145,19 +163,19 @@ template <int MODE, int BN> struct Tiles {
     }
     if (e >= experts) return false;
     int64_t local = t - base;
-    t += gridDim.x;
+    t += gridDim.x / CG;
     v.e = e;
     v.lo = lo[e];
     v.hi = hi[e];
     if (MODE != kWeights) {
-      const int m = (v.hi - v.lo + kBM - 1) / kBM;
+      const int m = (v.hi - v.lo + CG * kBM - 1) / (CG * kBM);
       v.n0 = (int)(local / m) * BN;
-      v.m0 = (int)(local % m) * kBM;
+      v.m0 = (int)(local % m) * CG * kBM;
       v.k_blocks = k_blocks;
     } else {
       const int per = m_tiles * n_tiles;
       const int unit = (int)(local / per), i = (int)(local % per);
-      v.m0 = i % m_tiles * kBM;
+      v.m0 = i % m_tiles * CG * kBM;
       v.n0 = i / m_tiles * BN;
       v.slot = base / per + unit;
       if (unit_rows) {
@@ -166,6 +184,7 @@ template <int MODE, int BN> struct Tiles {
       }
       v.k_blocks = (v.hi - v.lo + kBK - 1) / kBK;
     }
+    if (CG == 2) v.m0 += kBM * (int)(blockIdx.x & 1);
     return true;
   }
 };
@@ -288,12 +307,12 @@ __device__ __forceinline__ void store_rows(const float (&v)[32], unsigned char* 
   }
 }
 
-template <class T, int MODE, int P, int BN>
+template <class T, int MODE, int P, int BN, int CG>
 __global__ void __launch_bounds__(kBlock, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Args p) {
-  using S = Shape<T, P, BN>;
+  using S = Shape<P, BN, CG>;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t bars[2 * kMaxStages + 2 * 4 + 1];
+  __shared__ uint64_t bars[3 * kMaxStages + 2 * 4 + 1];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -306,9 +325,11 @@ __global__ void __launch_bounds__(kBlock, 1)
   const uint32_t bar0 = smem_u32(bars);
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
-  auto acc_full = [&](int b) { return bar0 + 8u * (2 * kMaxStages + b); };
-  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * kMaxStages + 4 + b); };
-  const uint32_t drain = bar0 + 8u * (2 * kMaxStages + 8);
+  auto peer_full = [&](int s) { return bar0 + 8u * (2 * kMaxStages + s); };  // the other CTA's stage, told to the first
+  auto acc_full = [&](int b) { return bar0 + 8u * (3 * kMaxStages + b); };
+  auto acc_empty = [&](int b) { return bar0 + 8u * (3 * kMaxStages + 4 + b); };
+  const uint32_t drain = bar0 + 8u * (3 * kMaxStages + 8);
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0;
   volatile int* abort_flag = &abort_word;
 
   ops::let_successor_start();
@@ -317,16 +338,20 @@ __global__ void __launch_bounds__(kBlock, 1)
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
+      mbar_init(peer_full(s), 1);
     }
     for (int b = 0; b < S::acc_bufs; ++b) {
       mbar_init(acc_full(b), 1);
-      mbar_init(acc_empty(b), 4 * S::parts);
+      mbar_init(acc_empty(b), CG * 4 * S::parts);
     }
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     fence_proxy_async();
   }
-  if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), 512);
+  if (warp == 1) {
+    if constexpr (CG == 2) tmem_alloc_pair(smem_u32(&tmem_slot), 512);
+    else tmem_alloc(smem_u32(&tmem_slot), 512);
+  }
   ops::wait_for_predecessor();
   for (int e = tid; e < p.experts; e += kBlock) {
     const int l = clamped(p.offset[e], 0, p.rows);
@@ -335,11 +360,12 @@ __global__ void __launch_bounds__(kBlock, 1)
   }
   if (blockIdx.x == 0) check_offsets(p.offset, p.experts, p.rows, p.error);
   tc_fence_before();
-  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // the barriers exist before the other CTA's arrivals
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  Tiles<MODE, BN> tiles(p, lo, hi);
+  Tiles<MODE, BN, CG> tiles(p, lo, hi);
   Tile v;
   int64_t issued = 0;  // stages filled so far (thread 0)
   if (warp == 0) {
@@ -355,26 +381,32 @@ __global__ void __launch_bounds__(kBlock, 1)
             break;
           }
           const uint32_t a = base + (uint32_t)s * S::stage_bytes, b = a + S::a_bytes;
-          mbar_expect_tx(full(s), S::stage_bytes);
-          const int k0 = kb * kBK;
+          const int k0 = kb * kBK, b0 = v.n0 + (int)rank * S::b_rows;
+          // A pair's loads are counted on the first CTA's barrier, except for a
+          // K block whose tail each CTA has to clear first.
+          const bool apart = CG == 1 || (MODE == kWeights && v.hi - v.lo - k0 < kBK);
+          const uint32_t bar = CG == 2 && !apart ? mapa_shared(full(s), 0) : full(s);
+          if (rank == 0 || apart) mbar_expect_tx(full(s), apart ? S::stage_bytes : CG * S::stage_bytes);
+          auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y, int z) {
+            if constexpr (CG == 2) tma_load_3d_pair(dst, map, x, y, z, bar);
+            else tma_load_3d(dst, map, x, y, z, bar);
+          };
 #pragma unroll
           for (int q = 0; q < P; ++q) {
+            const uint32_t aq = a + q * (kBM * kBK * 2), bq = b + q * (S::b_rows * kBK * 2);
             if (MODE != kWeights) {
-              tma_load_3d(a + q * (kBM * kBK * 2), &map_a, k0, v.lo + v.m0, q, full(s));
+              load(aq, &map_a, k0, v.lo + v.m0, q);
             } else {
 #pragma unroll
-              for (int j = 0; j < kBM / 64; ++j)
-                tma_load_3d(a + q * (kBM * kBK * 2) + j * 8192, &map_a, v.m0 + 64 * j, v.lo + k0, q, full(s));
+              for (int j = 0; j < kBM / 64; ++j) load(aq + j * 8192, &map_a, v.m0 + 64 * j, v.lo + k0, q);
             }
             if (MODE == kRows) {
-              tma_load_3d(b + q * (BN * kBK * 2), &map_b, k0, v.n0, q * p.experts + v.e, full(s));
+              load(bq, &map_b, k0, b0, q * p.experts + v.e);
             } else {
 #pragma unroll
-              for (int j = 0; j < BN / 64; ++j) {
-                if (MODE == kForward)
-                  tma_load_3d(b + q * (BN * kBK * 2) + j * 8192, &map_b, v.n0 + 64 * j, k0, q * p.experts + v.e, full(s));
-                else
-                  tma_load_3d(b + q * (BN * kBK * 2) + j * 8192, &map_b, v.n0 + 64 * j, v.lo + k0, q, full(s));
+              for (int j = 0; j < S::b_rows / 64; ++j) {
+                if (MODE == kForward) load(bq + j * 8192, &map_b, b0 + 64 * j, k0, q * p.experts + v.e);
+                else load(bq + j * 8192, &map_b, b0 + 64 * j, v.lo + k0, q);
               }
             }
           }
@@ -393,7 +425,7 @@ __global__ void __launch_bounds__(kBlock, 1)
     constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
     constexpr bool a_mn = MODE == kWeights, b_mn = MODE != kRows;
     constexpr uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((a_mn ? 1u : 0u) << 15) |
-                               ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
+                               ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(CG * kBM >> 4) << 24);
     // MN-major: 64-element chunks 8192 bytes apart (leading offset), groups of
     // 8 k 1024 apart; K-major: rows of 128 bytes, groups of 8 rows 1024 apart.
     const uint64_t da = smem_desc(base, a_mn ? 8192 : 16, 1024), db = smem_desc(base, b_mn ? 8192 : 16, 1024);
@@ -402,63 +434,100 @@ __global__ void __launch_bounds__(kBlock, 1)
     int s = 0, buf = 0;
     uint32_t ph = 0, acc_ph = 1;
     bool ok = true, skip = PONNI_B200_SKIP_ARRIVE();
-    while (ok && tiles.next(v)) {
-      for (int kb = 0; kb < v.k_blocks; ++kb) {
-        const uint32_t d = tmem + (uint32_t)(buf * S::acc_cols);
-        if (P == 3 || kb == 0) {
-          ok = wait_phase_abort(acc_empty(buf), acc_ph, abort_flag, PONNI_B200_WAIT_LIMIT);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-        }
-        ok = wait_phase_abort(full(s), ph, abort_flag, PONNI_B200_WAIT_LIMIT);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t stage = (uint32_t)s * S::stage_bytes;
-        if (MODE == kWeights && kb == v.k_blocks - 1) {
-          const int valid = v.hi - v.lo - kb * kBK;
-          if (valid < kBK) {  // rows of the next group: not part of this sum
-            for (int ch = 0; ch < S::stage_bytes / 8192; ++ch)
-              for (int i = valid * 8 + lane; i < kBK * 8; i += 32)
-                *reinterpret_cast<uint4*>(base_ptr + stage + ch * 8192 + i * 16) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async();
-            __syncwarp();
+    // Rows of the next group in the unit's last K block: not part of this sum.
+    auto clear_tail = [&](int kb) {
+      const int valid = v.hi - v.lo - kb * kBK;
+      unsigned char* stage = base_ptr + s * S::stage_bytes;
+      for (int ch = 0; ch < S::stage_bytes / 8192; ++ch)
+        for (int i = valid * 8 + lane; i < kBK * 8; i += 32)
+          *reinterpret_cast<uint4*>(stage + ch * 8192 + i * 16) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async();
+      __syncwarp();
+    };
+    auto mma = [&](uint32_t d, uint32_t alo, uint32_t blo, uint32_t accumulate) {
+      if constexpr (CG == 2) umma_f16_pair_warp(d, alo, a_hi, blo, b_hi, idesc, accumulate);
+      else umma_f16_desc_warp(d, alo, a_hi, blo, b_hi, idesc, accumulate);
+    };
+    auto commit = [&](uint32_t bar) {
+      if constexpr (CG == 2) umma_commit_pair_warp(bar);  // to both CTAs
+      else umma_commit_warp(bar);
+    };
+    auto next_stage = [&]() {
+      if (++s == p.stages) {
+        s = 0;
+        ph ^= 1u;
+      }
+    };
+    uint32_t tail_ph = 0;  // a bit per stage: phase of its next apart load
+    if (CG == 2 && rank == 1) {
+      // The second CTA of a pair issues nothing; it clears its tails and tells the first.
+      while (MODE == kWeights && ok && tiles.next(v)) {
+        for (int kb = 0; kb < v.k_blocks; ++kb) {
+          if (v.hi - v.lo - kb * kBK < kBK) {
+            ok = wait_phase_abort(full(s), tail_ph >> s & 1u, abort_flag, PONNI_B200_WAIT_LIMIT);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tail_ph ^= 1u << s;
+            clear_tail(kb);
+            if (lane == 0) arrive_remote(mapa_shared(peer_full(s), 0));
           }
-        }
-        const uint32_t a0 = a_lo0 + (stage >> 4), b0 = b_lo0 + ((stage + S::a_bytes) >> 4);
-        if constexpr (P == 1) {
-#pragma unroll
-          for (int k = 0; k < kBK / 16; ++k)
-            umma_f16_desc_warp(d, a0 + k * a_step, a_hi, b0 + k * b_step, b_hi, idesc, (kb > 0 || k > 0) ? 1u : 0u);
-        } else {
-          constexpr uint32_t ap = kBM * kBK * 2 / 16, bp = BN * kBK * 2 / 16;
-          constexpr int qa[6] = {1, 0, 2, 0, 1, 0}, qb[6] = {1, 2, 0, 1, 0, 0};
-#pragma unroll
-          for (int q = 0; q < 6; ++q)
-#pragma unroll
-            for (int k = 0; k < kBK / 16; ++k)
-              umma_f16_desc_warp(d, a0 + qa[q] * ap + k * a_step, a_hi, b0 + qb[q] * bp + k * b_step, b_hi, idesc,
-                                 (q > 0 || k > 0) ? 1u : 0u);
-        }
-        umma_commit_warp(empty(s));
-        if (P == 3 || kb == v.k_blocks - 1) {
-          if (!skip) umma_commit_warp(acc_full(buf));
-          skip = false;
-          if (++buf == S::acc_bufs) {
-            buf = 0;
-            acc_ph ^= 1u;
-          }
-        }
-        if (++s == p.stages) {
-          s = 0;
-          ph ^= 1u;
+          next_stage();
         }
       }
-    }
-    if (!ok) {
-      if (lane == 0) atomicOr(p.error, 1);
-      umma_commit_warp(drain);  // the MMAs issued so far, before TMEM is freed
-      (void)mbar_wait_bounded(drain, 0);
+      if (!ok && lane == 0) atomicOr(p.error, 1);
+    } else {
+      while (ok && tiles.next(v)) {
+        for (int kb = 0; kb < v.k_blocks; ++kb) {
+          const uint32_t d = tmem + (uint32_t)(buf * S::acc_cols);
+          if (P == 3 || kb == 0) {
+            ok = wait_phase_abort(acc_empty(buf), acc_ph, abort_flag, PONNI_B200_WAIT_LIMIT);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+          }
+          ok = wait_phase_abort(full(s), ph, abort_flag, PONNI_B200_WAIT_LIMIT);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (MODE == kWeights && v.hi - v.lo - kb * kBK < kBK) {
+            clear_tail(kb);
+            if (CG == 2) {
+              ok = wait_phase_abort_cluster(peer_full(s), tail_ph >> s & 1u, abort_flag, PONNI_B200_WAIT_LIMIT);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              tail_ph ^= 1u << s;
+            }
+          }
+          tc_fence_after();
+          const uint32_t stage = (uint32_t)s * S::stage_bytes;
+          const uint32_t a0 = a_lo0 + (stage >> 4), b0 = b_lo0 + ((stage + S::a_bytes) >> 4);
+          if constexpr (P == 1) {
+#pragma unroll
+            for (int k = 0; k < kBK / 16; ++k) mma(d, a0 + k * a_step, b0 + k * b_step, (kb > 0 || k > 0) ? 1u : 0u);
+          } else {
+            constexpr uint32_t ap = kBM * kBK * 2 / 16, bp = S::b_rows * kBK * 2 / 16;
+            constexpr int qa[6] = {1, 0, 2, 0, 1, 0}, qb[6] = {1, 2, 0, 1, 0, 0};
+#pragma unroll
+            for (int q = 0; q < 6; ++q)
+#pragma unroll
+              for (int k = 0; k < kBK / 16; ++k)
+                mma(d, a0 + qa[q] * ap + k * a_step, b0 + qb[q] * bp + k * b_step, (q > 0 || k > 0) ? 1u : 0u);
+          }
+          commit(empty(s));
+          if (P == 3 || kb == v.k_blocks - 1) {
+            if (!skip) commit(acc_full(buf));
+            skip = false;
+            if (++buf == S::acc_bufs) {
+              buf = 0;
+              acc_ph ^= 1u;
+            }
+          }
+          next_stage();
+        }
+      }
+      if (!ok) {
+        if (lane == 0) atomicOr(p.error, 1);
+        commit(drain);  // the MMAs issued so far, before TMEM is freed
+        (void)mbar_wait_bounded(drain, 0);
+      }
     }
   } else if ((warp - 2) >> 2 < S::parts) {
     // ------------------------------------------------------- epilogue ----
@@ -481,7 +550,10 @@ __global__ void __launch_bounds__(kBlock, 1)
     auto release_acc = [&]() {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty(buf));
+      if (lane == 0) {
+        if constexpr (CG == 2) arrive_remote(mapa_shared(acc_empty(buf), 0));
+        else mbar_arrive(acc_empty(buf));
+      }
       if (++buf == S::acc_bufs) {
         buf = 0;
         acc_ph ^= 1u;
@@ -579,12 +651,18 @@ __global__ void __launch_bounds__(kBlock, 1)
   __syncthreads();
   if (tid == 0 && *abort_flag) {
     // A role gave up: wait (bounded) for the copies in flight before the CTA ends.
-    for (int64_t i = issued > p.stages ? issued - p.stages : 0; i < issued; ++i)
-      if (!mbar_wait_bounded(full((int)(i % p.stages)), (uint32_t)(i / p.stages) & 1u)) break;
+    if (rank == 0) {
+      for (int64_t i = issued > p.stages ? issued - p.stages : 0; i < issued; ++i)
+        if (!mbar_wait_bounded(full((int)(i % p.stages)), (uint32_t)(i / p.stages) & 1u)) break;
+    } else {  // counted by the other CTA: a millisecond is a thousand copies' time
+      for (const long long t0 = clock64(); clock64() - t0 < 2000000;) __nanosleep(1000);
+    }
   }
+  if constexpr (CG == 2) cluster_sync();  // the pair's MMAs and copies, which use both CTAs' memory, are complete
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    if constexpr (CG == 2) tmem_dealloc_pair(tmem, 512);
+    else tmem_dealloc(tmem, 512);
   }
 }
 
@@ -998,22 +1076,35 @@ struct Space {
   }
 };
 
-template <class T, int MODE, int P, int BN>
+template <class T, int MODE, int P, int BN, int CG>
 ponni_b200_status launch_shape(const Operand& a, const Operand& b, Args p, int sms, int64_t tiles, cudaStream_t stream) {
-  using S = Shape<T, P, BN>;
+  using S = Shape<P, BN, CG>;
   CUtensorMap map_a, map_b;
   constexpr bool half = std::is_same<T, __half>::value;
   ponni_b200_status st = make_map(map_a, a, half, MODE == kWeights ? 64 : kBM);
-  if (!st) st = make_map(map_b, b, half, MODE == kRows ? BN : 64);
+  if (!st) st = make_map(map_b, b, half, MODE == kRows ? S::b_rows : 64);
   if (st) return st;
   const int fixed = 1024 + kEpiBytes + kBiasBytes + 2 * p.experts * (int)sizeof(int) + 512;
   p.stages = std::min(kMaxStages, (kSmemLimit - fixed) / S::stage_bytes);
   const int smem = 1024 + p.stages * S::stage_bytes + kEpiBytes + kBiasBytes + 2 * p.experts * (int)sizeof(int);
-  auto kern = product_kernel<T, MODE, P, BN>;
+  auto kern = product_kernel<T, MODE, P, BN, CG>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess)
-    e = ops::launch_after(kern, dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(sms, tiles))), dim3(kBlock),
-                          (size_t)smem, stream, map_a, map_b, p);
+  if (e != cudaSuccess) return ops::fail_cuda(e, "expert_product");
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CG;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(CG * std::max<int64_t>(1, std::min<int64_t>(sms / CG, tiles))));
+  cfg.blockDim = dim3(kBlock);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG == 2 ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, kern, map_a, map_b, p);
   return e == cudaSuccess ? PONNI_B200_OK : ops::fail_cuda(e, "expert_product");
 }
 
@@ -1023,25 +1114,36 @@ ponni_b200_status launch_shape(const Operand& a, const Operand& b, Args p, int s
 // an eighth more columns, or the rows are so few that the weights' traffic
 // decides (at most half a tile of rows a group): 128 then spreads them more evenly
 // over the SMs.
-int tile_width(int n, int most, int64_t rows, int experts, bool weights) {
+int tile_width(int n, int64_t rows, int experts, bool weights) {
   if (n <= 64) return 64;
-  if (most == 128 || n <= 128 || (!weights && rows <= (int64_t)64 * experts)) return 128;
+  if (n <= 128 || (!weights && rows <= (int64_t)64 * experts)) return 128;
   auto padded = [&](int w) { return (int64_t)(n + w - 1) / w * w; };
   return padded(256) * 8 > padded(128) * 9 ? 128 : 256;
+}
+
+// CTA pairs.
+bool use_pairs(const Args& p, int mode, int w) {
+  const char* v = getenv("PB_PAIR");
+  return v ? atoi(v) != 0 : true;
 }
 
 template <class T, int MODE>
 ponni_b200_status launch_product(const Operand& a, const Operand& b, const Args& p, int sms, cudaStream_t stream) {
   constexpr int P = sizeof(T) == 4 ? 3 : 1;
   const int n = MODE == kRows ? p.inputs : p.outputs;
-  const int w = tile_width(n, P == 3 ? 128 : 256, p.rows, p.experts, MODE == kWeights);
+  int w = tile_width(n, p.rows, p.experts, MODE == kWeights);
+  const int cg = w > 64 && use_pairs(p, MODE, w) ? 2 : 1, m = cg * kBM;
+  if (P == 3 && cg == 1) w = std::min(w, 128);
   const int64_t m_tiles = MODE == kWeights
-                              ? (int64_t)((p.inputs + kBM - 1) / kBM) * (p.experts + (p.unit_rows ? p.rows / p.unit_rows : 0))
-                              : p.rows / kBM + std::min<int64_t>(p.experts, p.rows);
+                              ? (int64_t)((p.inputs + m - 1) / m) * (p.experts + (p.unit_rows ? p.rows / p.unit_rows : 0))
+                              : p.rows / m + std::min<int64_t>(p.experts, p.rows);
   const int64_t tiles = m_tiles * ((n + w - 1) / w);
-  if (w == 64) return launch_shape<T, MODE, P, 64>(a, b, p, sms, tiles, stream);
-  if (w == 128) return launch_shape<T, MODE, P, 128>(a, b, p, sms, tiles, stream);
-  if constexpr (P == 1) return launch_shape<T, MODE, P, 256>(a, b, p, sms, tiles, stream);
+  if (w == 64) return launch_shape<T, MODE, P, 64, 1>(a, b, p, sms, tiles, stream);
+  if (w == 128)
+    return cg == 2 ? launch_shape<T, MODE, P, 128, 2>(a, b, p, sms, tiles, stream)
+                   : launch_shape<T, MODE, P, 128, 1>(a, b, p, sms, tiles, stream);
+  if (cg == 2) return launch_shape<T, MODE, P, 256, 2>(a, b, p, sms, tiles, stream);
+  if constexpr (P == 1) return launch_shape<T, MODE, P, 256, 1>(a, b, p, sms, tiles, stream);
   return ops::fail(PONNI_B200_ERR_UNSUPPORTED, "expert_product: no tile shape");
 }
 

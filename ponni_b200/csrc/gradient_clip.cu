@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "device_math.cuh"
@@ -59,8 +60,8 @@ __device__ __forceinline__ double squares(const T* __restrict__ p, int count) {
   int done = 0;
   if (reinterpret_cast<uintptr_t>(p) % 16 == 0) {
     const int vecs = count / n;
-    for (int i = threadIdx.x; i < vecs; i += kBlock) {
-      const uint4 raw = reinterpret_cast<const uint4*>(p)[i];
+    const uint4* q = reinterpret_cast<const uint4*>(p);
+    auto add = [&](const uint4& raw) {
       const Vec<T> v = *reinterpret_cast<const Vec<T>*>(&raw);
       if constexpr (sizeof(C) == 8) {
 #pragma unroll
@@ -76,7 +77,16 @@ __device__ __forceinline__ double squares(const T* __restrict__ p, int count) {
           for (int k = 0; k < n; ++k) s += square64(Num<T>::to_c(v.v[k]));
         }
       }
+    };
+    int i = threadIdx.x;
+    for (; i + 3 * kBlock < vecs; i += 4 * kBlock) {
+      uint4 raw[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) raw[k] = __ldg(q + i + k * kBlock);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) add(raw[k]);
     }
+    for (; i < vecs; i += kBlock) add(__ldg(q + i));
     done = vecs * n;
   }
   for (int i = done + threadIdx.x; i < count; i += kBlock) {
@@ -129,18 +139,41 @@ __device__ __forceinline__ void rescale(const T* p, O* out, int count, double sc
   int done = 0;
   if (sizeof(T) == sizeof(O) && reinterpret_cast<uintptr_t>(p) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
     const int vecs = count / n;
-    for (int i = threadIdx.x; i < vecs; i += kBlock) {
-      const uint4 raw = reinterpret_cast<const uint4*>(p)[i];
+    const uint4* q = reinterpret_cast<const uint4*>(p);
+    auto put = [&](const uint4& raw, int i) {
       const Vec<T> v = *reinterpret_cast<const Vec<T>*>(&raw);
       Vec<O> o;
 #pragma unroll
       for (int k = 0; k < n; ++k) o.v[k] = scaled<T, O>(v.v[k], scale);
       reinterpret_cast<uint4*>(out)[i] = *reinterpret_cast<uint4*>(&o);
+    };
+    int i = threadIdx.x;
+    for (; i + 3 * kBlock < vecs; i += 4 * kBlock) {
+      uint4 raw[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) raw[k] = q[i + k * kBlock];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) put(raw[k], i + k * kBlock);
     }
+    for (; i < vecs; i += kBlock) put(q[i], i);
     done = vecs * n;
   }
-#pragma unroll 4
-  for (int i = done + threadIdx.x; i < count; i += kBlock) out[i] = scaled<T, O>(p[i], scale);
+  // Element by element (a packed vector leaves the tensors off the 16-byte
+  // grid): coalesced on both sides, a batch of loads ahead of its stores.
+  int i = done + threadIdx.x;
+  auto batch = [&](auto size) {
+    constexpr int B = decltype(size)::value;
+    for (; i + (B - 1) * kBlock < count; i += B * kBlock) {
+      T v[B];
+#pragma unroll
+      for (int k = 0; k < B; ++k) v[k] = p[i + k * kBlock];
+#pragma unroll
+      for (int k = 0; k < B; ++k) out[i + k * kBlock] = scaled<T, O>(v[k], scale);
+    }
+  };
+  batch(std::integral_constant<int, 16>());
+  batch(std::integral_constant<int, 4>());
+  batch(std::integral_constant<int, 1>());
 }
 
 // flat_dtype < 0: in place.

@@ -23,9 +23,22 @@ constexpr int kBlock = 256;  // columns of a tile
 constexpr int kWarps = kBlock / 32;
 
 template <class T>
-__device__ __forceinline__ float logit(const T* p) {
-  const float v = Num<T>::to_c(*p);
+__device__ __forceinline__ float as_logit(T x) {
+  const float v = Num<T>::to_c(x);
   return v == v ? v : -INFINITY;
+}
+// Raw logits of experts e0 .. e0 + N - 1; past the last one the last one's (the
+// caller leaves them out).  No conditions around the loads: they go out together.
+template <class T, int N>
+__device__ __forceinline__ void load_logits(const T* __restrict__ x, int64_t ld, int e0, int experts, T (&raw)[N]) {
+  if (e0 + N <= experts) {
+    const T* p = x + (int64_t)e0 * ld;
+#pragma unroll
+    for (int u = 0; u < N; ++u) raw[u] = p[u * ld];
+  } else {
+#pragma unroll
+    for (int u = 0; u < N; ++u) raw[u] = x[(int64_t)min(e0 + u, experts - 1) * ld];
+  }
 }
 
 // exp(v - best) for v <= best, 1 where they are equal (both may be infinite);
@@ -51,17 +64,17 @@ __device__ __forceinline__ void choose(const T* __restrict__ x, int64_t ld, int 
     idx[j] = -1;
   }
   float sum = 0.0f, best = -3.402823466e38f;  // sum of exp(x - best) over the experts seen
-  float ahead[kChunk];
-  auto load = [&](int e0) {
-#pragma unroll
-    for (int u = 0; u < kChunk; ++u) ahead[u] = e0 + u < experts ? logit(x + (int64_t)(e0 + u) * ld) : -INFINITY;
-  };
-  load(0);
+  T ahead[kChunk];
+  load_logits<T, kChunk>(x, ld, 0, experts, ahead);
   for (int e0 = 0; e0 < experts; e0 += kChunk) {
     float v[kChunk];
 #pragma unroll
-    for (int u = 0; u < kChunk; ++u) v[u] = ahead[u];
-    if (e0 + kChunk < experts) load(e0 + kChunk);
+    for (int u = 0; u < kChunk; ++u) v[u] = as_logit(ahead[u]);
+    if (e0 + kChunk > experts) {
+#pragma unroll
+      for (int u = 0; u < kChunk; ++u) v[u] = e0 + u < experts ? v[u] : -INFINITY;
+    }
+    load_logits<T, kChunk>(x, ld, e0 + kChunk, experts, ahead);
     if (over_all) {
       float now = best;
 #pragma unroll
@@ -295,11 +308,8 @@ __global__ void __launch_bounds__(kBlock)
   const int64_t b = blockIdx.x * (int64_t)kBlock + threadIdx.x;
   if (b >= batch) return;
   const int e0 = blockIdx.y * kBackPart;
-  float v[kBackPart];
-  if (over_all) {
-#pragma unroll
-    for (int u = 0; u < kBackPart; ++u) v[u] = e0 + u < experts ? logit(x + (int64_t)(e0 + u) * ld + b) : -INFINITY;
-  }
+  T raw[kBackPart];
+  if (over_all) load_logits<T, kBackPart>(x + b, ld, e0, experts, raw);
   int idx[K];
   float w[K], g[K], mean = 0.0f;
 #pragma unroll
@@ -310,11 +320,12 @@ __global__ void __launch_bounds__(kBlock)
     mean += g[j];
   }
   const bool any = idx[0] >= 0;
-  const float best = any && over_all ? logit(x + (int64_t)idx[0] * ld + b) : 0.0f;
+  const float best = any && over_all ? as_logit(x[(int64_t)idx[0] * ld + b]) : 0.0f;
   const float scale = any ? -w[0] * mean : 0.0f;
 #pragma unroll
   for (int u = 0; u < kBackPart; ++u)
-    if (e0 + u < experts) dx[(e0 + u) * d_ld + b] = Num<T>::from_c(over_all && any ? from_best(v[u], best) * scale : 0.0f);
+    if (e0 + u < experts)
+      dx[(e0 + u) * d_ld + b] = Num<T>::from_c(over_all && any ? from_best(as_logit(raw[u]), best) * scale : 0.0f);
 #pragma unroll
   for (int j = 0; j < K; ++j)
     if (idx[j] >= e0 && idx[j] < e0 + kBackPart) dx[(int64_t)idx[j] * d_ld + b] = Num<T>::from_c(g[j] - w[j] * mean);
@@ -372,7 +383,7 @@ using namespace ponni_b200;
 extern "C" {
 
 int64_t ponni_b200_route_workspace(int num_experts, int64_t batch) {
-  if (num_experts < 1 || batch < 1) return 0;
+  if (num_experts < 1 || batch <= kOneBlock) return 0;
   return (int64_t)num_experts * (blocks_of(batch) + 1) * (int64_t)sizeof(int);
 }
 
@@ -385,7 +396,8 @@ ponni_b200_status ponni_b200_route_columns(int dtype, const void* logits, int64_
     if (st) return st;
     if (!expert || !weight || !row || !column || !offset)
       return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route: output pointer is NULL");
-    if (!workspace || workspace_bytes < ponni_b200_route_workspace(num_experts, batch))
+    const int64_t need = ponni_b200_route_workspace(num_experts, batch);
+    if (need && (!workspace || workspace_bytes < need))
       return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route: workspace is too small");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int all = normalise == PONNI_B200_ROUTE_ALL;

@@ -144,19 +144,19 @@ def route_columns(logits, top_k: int, normalise: str = "selected") -> Routing:
     if not 1 <= top_k <= min(8, experts):
         _refuse(f"top_k must be 1 to 8 and at most the {experts} experts, not {top_k}", 3)
     dev, L = logits.device, _abi.lib()
-    n = top_k * batch
-    # One allocation: expert, row, column, weight, offset, then the workspace.
-    need = (L.ponni_b200_route_workspace(experts, batch) + 3) // 4
-    buf = torch.empty(4 * n + experts + 1 + need, dtype=torch.int32, device=dev)
-    expert, row, column, weight, offset, space = buf.split((n, n, n, n, experts + 1, need))
-    weight = weight.view(torch.float32)
-    base = buf.data_ptr()
-    at = base + 16 * n
-    _call(L.ponni_b200_route_columns(code, logits.data_ptr(), ld, experts, top_k, batch, _NORMALISE[normalise], base,
-                                     base + 12 * n, base + 4 * n, base + 8 * n, at, at + 4 * (experts + 1), 4 * need,
-                                     dev.index, torch_stream_handle(dev)))
     shape = (top_k, batch)
-    return Routing(expert.view(shape), weight.view(shape), row.view(shape), column, offset)
+    i32 = torch.int32
+    expert, row = torch.empty(shape, dtype=i32, device=dev), torch.empty(shape, dtype=i32, device=dev)
+    weight = torch.empty(shape, dtype=torch.float32, device=dev)
+    column = torch.empty(top_k * batch, dtype=i32, device=dev)
+    offset = torch.empty(experts + 1, dtype=i32, device=dev)
+    need = L.ponni_b200_route_workspace(experts, batch)
+    space = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _call(L.ponni_b200_route_columns(code, logits.data_ptr(), ld, experts, top_k, batch, _NORMALISE[normalise],
+                                     expert.data_ptr(), weight.data_ptr(), row.data_ptr(), column.data_ptr(),
+                                     offset.data_ptr(), space.data_ptr() if need else None, need, dev.index,
+                                     torch_stream_handle(dev)))
+    return Routing(expert, weight, row, column, offset)
 
 
 def route_columns_backward(logits, routing: Routing, d_weight, normalise: str = "selected"):
