@@ -37,7 +37,6 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
-#include <cstdlib>
 #include <cstring>
 #include <type_traits>
 
@@ -246,29 +245,83 @@ __device__ __forceinline__ float activate_one(int kind, int flags, float x, floa
   return activation<float>(kind, flags, x, s0, s1);
 }
 
-template <class T, int KIND>
-__device__ __forceinline__ void activate32(float (&v)[32], int flags, float s0, float s1) {
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = activate_one<T>(KIND, flags, v[i], s0, s1);
+// Out of line: the exact formulas, unrolled into a kernel for 32 values, cost
+// more in instruction fetches than in work.
+template <class T>
+__device__ __noinline__ float4 activate4(float4 v, int kind, int flags, float s0, float s1) {
+  v.x = activate_one<T>(kind, flags, v.x, s0, s1);
+  v.y = activate_one<T>(kind, flags, v.y, s0, s1);
+  v.z = activate_one<T>(kind, flags, v.z, s0, s1);
+  v.w = activate_one<T>(kind, flags, v.w, s0, s1);
+  return v;
 }
+
+// SiLU and exact GELU of 32 values whose results are rounded to 16 bits.  The
+// special-function unit bounds the epilogue of narrow products (256 -> 256: two of
+// its operations a value would take 139 of the 256 us measured with them), so two
+// values share one reciprocal: 1/a = b (1/ab).  The arguments are kept where ab is
+// finite, which also keeps a NaN from its neighbour.
+__device__ __forceinline__ void fast_silu32(float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) {
+    float a, b;
+    f2::mul(a, b, v[i], v[i + 1], -kLog2e, -kLog2e);
+    a = fast_exp2(fminf(a, 60.0f));  // sigmoid at least 2^-60
+    b = fast_exp2(fminf(b, 60.0f));
+    f2::add(a, b, a, b, 1.0f, 1.0f);
+    const float r = fast_rcp(a * b);
+    f2::mul(a, b, b, a, r, r);
+    f2::mul(v[i], v[i + 1], v[i], v[i + 1], a, b);
+  }
+}
+__device__ __forceinline__ void fast_gelu32(float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) {
+    float y, z, s, t, p, q;
+    f2::mul(y, z, fabsf(v[i]), fabsf(v[i + 1]), 0.70710678118654752f, 0.70710678118654752f);
+    y = fminf(y, 1e9f);
+    z = fminf(z, 1e9f);
+    f2::fma(s, t, y, z, 0.3275911f, 0.3275911f, 1.0f, 1.0f);
+    const float r = fast_rcp(s * t);
+    f2::mul(s, t, t, s, r, r);
+    f2::fma(p, q, s, t, 1.061405429f, 1.061405429f, -1.453152027f, -1.453152027f);
+    f2::fma(p, q, p, q, s, t, 1.421413741f, 1.421413741f);
+    f2::fma(p, q, p, q, s, t, -0.284496736f, -0.284496736f);
+    f2::fma(p, q, p, q, s, t, 0.254829592f, 0.254829592f);
+    f2::mul(p, q, p, q, s, t);
+    f2::mul(s, t, y, z, -kLog2e, -kLog2e);
+    f2::mul(s, t, s, t, y, z);
+    f2::mul(p, q, p, q, 0.5f, 0.5f);
+    f2::mul(p, q, p, q, fast_exp2(s), fast_exp2(t));  // erfc(|x| / sqrt 2) / 2
+    v[i] *= v[i] > 0.0f ? 1.0f - p : p;
+    v[i + 1] *= v[i + 1] > 0.0f ? 1.0f - q : q;
+  }
+}
+
 template <class T>
 __device__ __forceinline__ void activate_all(float (&v)[32], int kind, int flags, float s0, float s1) {
   if (kind == EPI_NONE) return;
-  if (kind == EPI_RELU) return activate32<T, EPI_RELU>(v, flags, s0, s1);
-  if (kind == EPI_SILU) return activate32<T, EPI_SILU>(v, flags, s0, s1);
-  if (sizeof(T) == 2 && kind == EPI_GELU && !(flags & 0x2)) return activate32<T, EPI_GELU>(v, 0, s0, s1);
-  // The others share one loop of 8 values to keep the kernel small.
-#pragma unroll 1
-  for (int i = 0; i < 4; ++i)
+  if (kind == EPI_RELU) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float x = 0.0f;
+    for (int i = 0; i < 32; ++i) v[i] = v[i] > 0.0f ? v[i] : 0.0f;
+    return;
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (kind == EPI_SILU) return fast_silu32(v);
+    if (kind == EPI_GELU && !(flags & 0x2)) return fast_gelu32(v);
+  } else if (kind == EPI_SILU) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) x = q == i ? v[8 * q + j] : x;
-      x = activate_one<T>(kind, flags, x, s0, s1);
+    for (int i = 0; i < 32; ++i) v[i] *= fast_rcp(1.0f + expf(-v[i]));
+    return;
+  }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[8 * q + j] = q == i ? x : v[8 * q + j];
-    }
+  for (int i = 0; i < 32; i += 4) {
+    const float4 r = activate4<T>(make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]), kind, flags, s0, s1);
+    v[i] = r.x;
+    v[i + 1] = r.y;
+    v[i + 2] = r.z;
+    v[i + 3] = r.w;
+  }
 }
 
 // 32 columns of this warp's 32 rows (one row a lane) to global memory through
@@ -577,19 +630,27 @@ __global__ void __launch_bounds__(kBlock, 1)
         const int n = col0 + c * 32, n_valid = n_end - n;
         if (n_valid <= 0 || m_valid <= 0) return;
         if constexpr (P == 3) {
+          bool nan = false;
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (x[i] != x[i] && lane < m_valid && i < n_valid) x[i] = plain_sum<MODE>(p, v.e, v.lo, v.hi, row0 + lane, n + i);
+          for (int i = 0; i < 32; ++i) nan |= x[i] != x[i];
+          if (nan) {
+            float y[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) y[i] = x[i];
+#pragma unroll 1
+            for (int i = 0; i < min(32, n_valid); ++i)
+              if (y[i] != y[i] && lane < m_valid) y[i] = plain_sum<MODE>(p, v.e, v.lo, v.hi, row0 + lane, n + i);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = y[i];
+          }
         }
         if (MODE == kForward) {
           if (p.bias) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
               const float4 b = *reinterpret_cast<const float4*>(bias_w + c * 32 + i);
-              x[i] += b.x;
-              x[i + 1] += b.y;
-              x[i + 2] += b.z;
-              x[i + 3] += b.w;
+              f2::add(x[i], x[i + 1], x[i], x[i + 1], b.x, b.y);
+              f2::add(x[i + 2], x[i + 3], x[i + 2], x[i + 3], b.z, b.w);
             }
           }
           activate_all<T>(x, p.act, p.act_flags, p.s0, p.s1);
@@ -626,8 +687,7 @@ __global__ void __launch_bounds__(kBlock, 1)
             for (int c = 0; c < kChunks; ++c) {
               float x[32];
               tmem_ld32(t + c * 32, x);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) acc[c][i] += x[i];
+              f2::add_n(acc[c], x);
             }
             release_acc();
           }
@@ -953,6 +1013,9 @@ __device__ __forceinline__ void split_any(float x, uint32_t& h0, uint32_t& h1, u
   }
 }
 
+// A thread lays out 8 elements: one 16-byte store a plane.  (Two elements a thread,
+// coalesced on both sides, issues more instructions than it saves: 29 to 47 us
+// against 26 for two operands of 20011 x 301 and 20011 x 257.)
 template <class T>
 __global__ void __launch_bounds__(256) stage_kernel(const Stages all) {
   ops::let_successor_start();
@@ -960,7 +1023,7 @@ __global__ void __launch_bounds__(256) stage_kernel(const Stages all) {
   const Stage& s = all.s[blockIdx.y];
   const int vecs = s.pitch / 8;
   int tx = 1;
-  while (tx < vecs && tx < 256) tx *= 2;
+  while (tx < vecs && tx < 256) tx *= 2;  // threads along a row
   const int x = threadIdx.x % tx, y = threadIdx.x / tx, ty = 256 / tx;
   const int64_t plane = s.rows * (int64_t)s.pitch;
   for (int64_t r = blockIdx.x * (int64_t)ty + y; r < s.rows; r += (int64_t)gridDim.x * ty) {
@@ -969,7 +1032,7 @@ __global__ void __launch_bounds__(256) stage_kernel(const Stages all) {
     for (int c = x; c < vecs; c += tx) {
       T v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = c * 8 + i < s.cols ? src[c * 8 + i] : Num<T>::from_c(0.0f);
+      for (int i = 0; i < 8; ++i) v[i] = c * 8 + i < s.cols ? __ldg(src + c * 8 + i) : Num<T>::from_c(0.0f);
       if constexpr (sizeof(T) == 4) {
         uint32_t h[3][8];
 #pragma unroll
@@ -1038,12 +1101,14 @@ int64_t staged_bytes(int dtype, int64_t rows, int cols) {
   return pad256(rows * pad8(cols) * (dtype == PONNI_B200_F32 ? 6 : 2));
 }
 
-// Rows of a unit of d_W: whole groups where those fill the SMs twice, else
-// units small enough for about four tiles an SM (the tail of uneven groups),
-// 1024 rows at least (a unit's partial sums cost 8 bytes an element of W_e).
+// Rows of a unit of d_W: whole groups where their tiles fill the SMs twice or the
+// groups are short (2048 rows on average: a split costs another launch, 9.5 us
+// against 19 for 16 experts of 256 x 256 with 64 and 128 rows each); else units small
+// enough for about four tiles an SM (the tail of uneven groups), 1024 rows at least
+// (a unit's partial sums cost 8 bytes an element of W_e).
 int unit_rows_of(int64_t rows, int experts, int inputs, int outputs, int sms) {
   const int64_t per = (int64_t)((inputs + kBM - 1) / kBM) * ((outputs + 255) / 256);
-  if (per * experts >= 2 * sms || rows <= 1024) return 0;
+  if (per * experts >= 2 * sms || rows <= (int64_t)2048 * experts) return 0;
   const int64_t unit = std::max<int64_t>(1024, (rows * per / (4 * sms) + kBK - 1) / kBK * kBK);
   return unit < rows ? (int)std::min<int64_t>(unit, 1 << 30) : 0;
 }
@@ -1121,10 +1186,15 @@ int tile_width(int n, int64_t rows, int experts, bool weights) {
   return padded(256) * 8 > padded(128) * 9 ? 128 : 256;
 }
 
-// CTA pairs.
-bool use_pairs(const Args& p, int mode, int w) {
-  const char* v = getenv("PB_PAIR");
-  return v ? atoi(v) != 0 : true;
+// Whether two CTAs share a tile of 256 rows: half the weight traffic, but more
+// rows of padding at the end of a group.  16-bit rows x 1024 x 1024, 16 experts:
+// 23.1 us against 22.2 in pairs with 256 rows each, 24.3 / 28.4 with 512, 39.7 / 36.6
+// with 1024, 128.5 / 117.2 with 4096; the weight gradient has no such padding (31.1 /
+// 28.8 with 512).  fp32 spends its time on the parts' traffic and the sums of every K
+// block: 969.8 / 1060 with 4096 rows each, 4245 / 4170 with 16384.
+bool use_pairs(const Args& p, int mode, bool split_parts) {
+  const int64_t least = split_parts ? 8192 : mode == kWeights ? 256 : 768;
+  return p.rows >= least * p.experts;
 }
 
 template <class T, int MODE>
@@ -1132,7 +1202,7 @@ ponni_b200_status launch_product(const Operand& a, const Operand& b, const Args&
   constexpr int P = sizeof(T) == 4 ? 3 : 1;
   const int n = MODE == kRows ? p.inputs : p.outputs;
   int w = tile_width(n, p.rows, p.experts, MODE == kWeights);
-  const int cg = w > 64 && use_pairs(p, MODE, w) ? 2 : 1, m = cg * kBM;
+  const int cg = w > 64 && use_pairs(p, MODE, P == 3) ? 2 : 1, m = cg * kBM;
   if (P == 3 && cg == 1) w = std::min(w, 128);
   const int64_t m_tiles = MODE == kWeights
                               ? (int64_t)((p.inputs + m - 1) / m) * (p.experts + (p.unit_rows ? p.rows / p.unit_rows : 0))
@@ -1234,8 +1304,7 @@ ponni_b200_status run_stages(const Stages& st, int sms, cudaStream_t s) {
   if (!st.n) return PONNI_B200_OK;
   int64_t most = 1;
   for (int i = 0; i < st.n; ++i) {
-    const int64_t per = std::max<int64_t>(1, 256 / std::max(1, st.s[i].pitch / 8));
-    most = std::max(most, (st.s[i].rows + per - 1) / per);
+    most = std::max(most, (st.s[i].rows * st.s[i].pitch + 2047) / 2048);
   }
   stage_kernel<T><<<dim3((unsigned)std::min<int64_t>(most, sms * 8), st.n), 256, 0, s>>>(st);
   return ops::launched("expert_product");
