@@ -75,6 +75,7 @@ struct Args {
   float s0, s1;
   int unit_rows;  // kWeights: rows of a unit (a multiple of kBK); 0: a group is one unit
   int vec;        // c may be written 16 bytes at a time
+  int bulk;       // and by the copy engine (map_c)
   int stages;
   int* error;
 };
@@ -92,6 +93,10 @@ template <int P, int BN, int CG> struct Shape {
   // number modulo 4) times `parts` strips of columns.
   static constexpr int parts = BN >= 128 ? 4 : 2;
   static constexpr int part_cols = BN / parts;
+  // Output staging of a warp: two boxes of 32 rows x 64 bytes for the copy engine
+  // (pairs of 16-bit operands), else its rows of 32 bytes.
+  static constexpr bool bulk_store = P == 1 && CG == 2;
+  static constexpr int epi_bytes = bulk_store ? kEpiWarps * 4096 : kEpiBytes;
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -115,6 +120,19 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
 __device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_addr) : "memory");
 }
+
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int x, int y, int z, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n\t"
+               "cp.async.bulk.commit_group;\n" ::"l"(reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(z), "r"(src)
+               : "memory");
+}
+// All but the last N stores of this thread have read their source.
+template <int N>
+__device__ __forceinline__ void tma_store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void tma_store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
 
 // Check of the offsets by one block (the groups are clamped whatever they hold).
 __device__ __forceinline__ void check_offsets(const int* __restrict__ offset, int experts, int64_t rows, int* error) {
@@ -362,7 +380,8 @@ __device__ __forceinline__ void store_rows(const float (&v)[32], unsigned char* 
 
 template <class T, int MODE, int P, int BN, int CG>
 __global__ void __launch_bounds__(kBlock, 1)
-    product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Args p) {
+    product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                   const __grid_constant__ CUtensorMap map_c, const Args p) {
   using S = Shape<P, BN, CG>;
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t bars[3 * kMaxStages + 2 * 4 + 1];
@@ -372,8 +391,8 @@ __global__ void __launch_bounds__(kBlock, 1)
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   unsigned char* base_ptr = smem_raw + (base - raw);
   unsigned char* epi = base_ptr + p.stages * S::stage_bytes;
-  float* bias_s = reinterpret_cast<float*>(epi + kEpiBytes);
-  int* lo = reinterpret_cast<int*>(epi + kEpiBytes + kBiasBytes);
+  float* bias_s = reinterpret_cast<float*>(epi + S::epi_bytes);
+  int* lo = reinterpret_cast<int*>(epi + S::epi_bytes + kBiasBytes);
   int* hi = lo + p.experts;
   const uint32_t bar0 = smem_u32(bars);
   auto full = [&](int s) { return bar0 + 8u * s; };
@@ -586,7 +605,8 @@ __global__ void __launch_bounds__(kBlock, 1)
     // ------------------------------------------------------- epilogue ----
     const int quarter = warp & 3, part = (warp - 2) >> 2, w = warp - 2;
     constexpr int kChunks = S::part_cols / 32;
-    unsigned char* stage = epi + w * 32 * kEpiPitch;
+    unsigned char* stage = epi + w * (S::epi_bytes / kEpiWarps);
+    int box = 0;  // of the two store boxes
     float* bias_w = bias_s + w * 64;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const int n_end = MODE == kRows ? p.inputs : p.outputs;
@@ -657,6 +677,29 @@ __global__ void __launch_bounds__(kBlock, 1)
           }
           activate_all<T>(x, p.act, p.act_flags, p.s0, p.s1);
         }
+        if constexpr (S::bulk_store) {
+          if (p.bulk && (MODE == kWeights || m_valid == 32)) {  // (rows past the weights' end are clipped)
+            // 64-byte rows, 16-byte chunks swizzled by row / 2 as the tensor map has it.
+            if (lane == 0) tma_store_wait_read<1>();
+            __syncwarp();
+            const uint32_t dst = smem_u32(stage) + (uint32_t)box * 2048;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              st_shared_v4(dst + lane * 64 + ((i ^ (lane >> 1 & 3)) << 4), pack2(x[8 * i], x[8 * i + 1], (T*)0),
+                           pack2(x[8 * i + 2], x[8 * i + 3], (T*)0), pack2(x[8 * i + 4], x[8 * i + 5], (T*)0),
+                           pack2(x[8 * i + 6], x[8 * i + 7], (T*)0));
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              if (MODE == kWeights) tma_store_3d(&map_c, n, row0, v.e, dst);
+              else tma_store_3d(&map_c, n, v.lo + row0, 0, dst);
+            }
+            box ^= 1;
+            return;
+          }
+          if (lane == 0) tma_store_wait_read<0>();
+          __syncwarp();
+        }
         if (MODE == kWeights) {
           if (p.unit_rows)
             store_rows<float>(x, stage, p.partial + (v.slot * p.inputs + row0) * p.outputs + n, p.outputs, m_valid,
@@ -701,6 +744,7 @@ __global__ void __launch_bounds__(kBlock, 1)
         for (int c = 0; c < kChunks; ++c) finish(acc[c], c);
       }
     }
+    if (S::bulk_store && lane == 0) tma_store_wait_all();
     if (!ok && lane == 0) atomicOr(p.error, 1);
   }
   if (MODE != kWeights) {
@@ -1082,16 +1126,17 @@ struct Operand {
   int64_t cols, rows, depth;
 };
 
-ponni_b200_status make_map(CUtensorMap& map, const Operand& o, bool half, int box_rows) {
+// box_cols: 64 elements of an operand (128-byte swizzle) or 32 of an output (64-byte).
+ponni_b200_status make_map(CUtensorMap& map, const Operand& o, bool half, int box_rows, int box_cols = 64) {
   EncodeTiledFn enc = encode_tiled();
   if (!enc) return ops::fail(PONNI_B200_ERR_CUDA, "expert_product: the driver has no tensor maps");
   const cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.depth};
   const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(o.depth > 1 ? o.stride : o.ld) * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+  const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
   const cuuint32_t estr[3] = {1, 1, 1};
   if (strides[0] >= (1ull << 40) || strides[1] >= (1ull << 40) ||
       enc(&map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.p),
-          dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+          dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return ops::fail(PONNI_B200_ERR_UNSUPPORTED, "expert_product: operand sizes or strides beyond the copy engine's");
   return PONNI_B200_OK;
@@ -1148,14 +1193,22 @@ struct Space {
 template <class T, int MODE, int P, int BN, int CG>
 ponni_b200_status launch_shape(const Operand& a, const Operand& b, Args p, int sms, int64_t tiles, cudaStream_t stream) {
   using S = Shape<P, BN, CG>;
-  CUtensorMap map_a, map_b;
+  CUtensorMap map_a, map_b, map_c;
+  std::memset(&map_c, 0, sizeof map_c);
   constexpr bool half = std::is_same<T, __half>::value;
   ponni_b200_status st = make_map(map_a, a, half, MODE == kWeights ? 64 : kBM);
   if (!st) st = make_map(map_b, b, half, MODE == kRows ? S::b_rows : 64);
+  p.bulk = S::bulk_store && p.vec && !p.unit_rows;
+  if (!st && p.bulk) {
+    const int64_t n = MODE == kRows ? p.inputs : p.outputs;
+    const Operand c = MODE == kWeights ? Operand{p.c, n, n * p.inputs, n, p.inputs, p.experts}
+                                       : Operand{p.c, p.c_ld, 0, n, p.rows, 1};
+    st = make_map(map_c, c, half, 32, 32);
+  }
   if (st) return st;
-  const int fixed = 1024 + kEpiBytes + kBiasBytes + 2 * p.experts * (int)sizeof(int) + 512;
+  const int fixed = 1024 + S::epi_bytes + kBiasBytes + 2 * p.experts * (int)sizeof(int) + 512;
   p.stages = std::min(kMaxStages, (kSmemLimit - fixed) / S::stage_bytes);
-  const int smem = 1024 + p.stages * S::stage_bytes + kEpiBytes + kBiasBytes + 2 * p.experts * (int)sizeof(int);
+  const int smem = 1024 + p.stages * S::stage_bytes + S::epi_bytes + kBiasBytes + 2 * p.experts * (int)sizeof(int);
   auto kern = product_kernel<T, MODE, P, BN, CG>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return ops::fail_cuda(e, "expert_product");
@@ -1173,7 +1226,7 @@ ponni_b200_status launch_shape(const Operand& a, const Operand& b, Args p, int s
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = CG == 2 ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kern, map_a, map_b, p);
+  e = cudaLaunchKernelEx(&cfg, kern, map_a, map_b, map_c, p);
   return e == cudaSuccess ? PONNI_B200_OK : ops::fail_cuda(e, "expert_product");
 }
 
