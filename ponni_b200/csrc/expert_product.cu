@@ -87,15 +87,17 @@ template <int P, int BN, int CG> struct Shape {
   static constexpr int a_bytes = P * kBM * kBK * 2;
   static constexpr int b_bytes = P * b_rows * kBK * 2;
   static constexpr int stage_bytes = a_bytes + b_bytes;
-  static constexpr int acc_cols = P == 3 && BN <= 128 ? 128 : 256;
+  static constexpr int acc_cols = BN <= 128 ? 128 : 256;
   static constexpr int acc_bufs = 512 / acc_cols;
   // Epilogue warps: four lane quarters (a warp reads the TMEM lanes of its
   // number modulo 4) times `parts` strips of columns.
   static constexpr int parts = BN >= 128 ? 4 : 2;
+  static constexpr int groups = 4 / parts;  // of warps, which take tiles in turn
   static constexpr int part_cols = BN / parts;
   // Output staging of a warp: two boxes of 32 rows x 64 bytes for the copy engine
-  // (pairs of 16-bit operands), else its rows of 32 bytes.
-  static constexpr bool bulk_store = P == 1 && CG == 2;
+  // (16-bit operands in pairs or 64 wide), else its rows of 32 bytes: the boxes cost
+  // the single 128-wide tiles stages, and with them 10% on weight-bound products.
+  static constexpr bool bulk_store = P == 1 && (CG == 2 || BN == 64);
   static constexpr int epi_bytes = bulk_store ? kEpiWarps * 4096 : kEpiBytes;
 };
 
@@ -601,9 +603,11 @@ __global__ void __launch_bounds__(kBlock, 1)
         (void)mbar_wait_bounded(drain, 0);
       }
     }
-  } else if ((warp - 2) >> 2 < S::parts) {
+  } else {
     // ------------------------------------------------------- epilogue ----
-    const int quarter = warp & 3, part = (warp - 2) >> 2, w = warp - 2;
+    const int quarter = warp & 3, part = ((warp - 2) >> 2) % S::parts, w = warp - 2;
+    const int group = ((warp - 2) >> 2) / S::parts;
+    int turn = 0;
     constexpr int kChunks = S::part_cols / 32;
     unsigned char* stage = epi + w * (S::epi_bytes / kEpiWarps);
     int box = 0;  // of the two store boxes
@@ -620,6 +624,12 @@ __global__ void __launch_bounds__(kBlock, 1)
       tc_fence_after();
       return got != 0;
     };
+    auto next_acc = [&]() {
+      if (++buf == S::acc_bufs) {
+        buf = 0;
+        acc_ph ^= 1u;
+      }
+    };
     auto release_acc = [&]() {
       tc_fence_before();
       __syncwarp();
@@ -627,12 +637,13 @@ __global__ void __launch_bounds__(kBlock, 1)
         if constexpr (CG == 2) arrive_remote(mapa_shared(acc_empty(buf), 0));
         else mbar_arrive(acc_empty(buf));
       }
-      if (++buf == S::acc_bufs) {
-        buf = 0;
-        acc_ph ^= 1u;
-      }
+      next_acc();
     };
     while (ok && tiles.next(v)) {
+      if (S::groups > 1 && turn++ % S::groups != group) {  // another group's tile
+        for (int i = 0; i < (P == 3 ? v.k_blocks : min(1, v.k_blocks)); ++i) next_acc();
+        continue;
+      }
       const int m_end = MODE == kWeights ? p.inputs : v.hi - v.lo;
       const int row0 = v.m0 + quarter * 32, m_valid = min(32, m_end - row0);
       const int col0 = v.n0 + part * S::part_cols;
