@@ -786,18 +786,20 @@ __global__ void __launch_bounds__(kBlock, 1)
 }
 
 // ------------------------------------------------------------ few rows ----
-// Forward for groups of a few rows: a work item is up to 8 rows of a group, a
+// Forward for groups of a few rows: a work item is up to 8 rows of a group (16 of
+// fp32, whose thread holds half the columns), a
 // block takes 128 columns and one of the cluster's slices of K.  A thread holds
 // the sums of a vector of columns (16 bytes of weights: one load serves all of
 // the item's rows) for every 8th or 16th k; the k groups are added in shared
 // memory, the slices through the cluster's distributed shared memory, in a
 // fixed order.  The rows of the item lie in shared memory as fp32.
-constexpr int kFewThreads = 256, kFewRows = 8, kFewCols = 128, kFewK = 1024;
+constexpr int kFewThreads = 256, kFewCols = 128, kFewFloats = 8192;
 
 template <class T> struct Few {
   static constexpr int vec = 16 / sizeof(T);           // columns of a thread
   static constexpr int lanes = kFewCols / vec;         // threads side by side
   static constexpr int groups = kFewThreads / lanes;   // k groups of the block
+  static constexpr int rows = sizeof(T) == 4 ? 16 : 8;  // of an item
 };
 
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
@@ -810,7 +812,7 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr) {
 template <class T, int RB, bool VEC>
 __device__ __forceinline__ void few_sums(const T* __restrict__ w, int64_t w_ld, int kn, int cols, const float* xs,
                                          float (&acc)[RB][Few<T>::vec]) {
-  constexpr int V = Few<T>::vec, G = Few<T>::groups, U = RB > 4 ? 4 : 8;
+  constexpr int V = Few<T>::vec, G = Few<T>::groups, U = RB * V > 32 ? 4 : 8;
   const int g = threadIdx.x / Few<T>::lanes;
   auto load = [&](int k) -> uint4 {
     const T* p = w + (int64_t)k * w_ld;
@@ -828,11 +830,30 @@ __device__ __forceinline__ void few_sums(const T* __restrict__ w, int64_t w_ld, 
     float f[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = Num<T>::to_c(t[i]);
+    float xr[RB];
+    if constexpr (RB % 4 == 0) {
 #pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      const float x = xs[k * RB + r];
+      for (int r = 0; r < RB; r += 4) {
+        const float4 q = *reinterpret_cast<const float4*>(xs + k * RB + r);
+        xr[r] = q.x;
+        xr[r + 1] = q.y;
+        xr[r + 2] = q.z;
+        xr[r + 3] = q.w;
+      }
+    } else {
 #pragma unroll
-      for (int i = 0; i < V; i += 2) f2::fma(acc[r][i], acc[r][i + 1], f[i], f[i + 1], x, x, acc[r][i], acc[r][i + 1]);
+      for (int r = 0; r < RB; ++r) xr[r] = xs[k * RB + r];
+    }
+    // Packed over two rows: their values come side by side out of shared memory.
+    if constexpr (RB == 1) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[0][i] = fmaf(f[i], xr[0], acc[0][i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+#pragma unroll
+        for (int r = 0; r < RB; r += 2)
+          f2::fma(acc[r][i], acc[r + 1][i], xr[r], xr[r + 1], f[i], f[i], acc[r][i], acc[r + 1][i]);
     }
   };
   int k = g;
@@ -855,12 +876,32 @@ __device__ void few_item(const Args& p, int e, int64_t row0, int n_rows, int n0,
   const int cols = p.outputs - (n0 + x * V);
   const T* w = static_cast<const T*>(p.b) + e * p.b_stride + (cols > 0 ? n0 + x * V : 0);
   float acc[RB][V] = {};
-  for (int k0 = k_lo; k0 < k_hi; k0 += kFewK) {
-    const int kn = min(kFewK, k_hi - k0);
+  constexpr int kStep = kFewFloats / RB < 1024 ? kFewFloats / RB : 1024;
+  for (int k0 = k_lo; k0 < k_hi; k0 += kStep) {
+    const int kn = min(kStep, k_hi - k0);
     __syncthreads();
-    for (int i = tid; i < kn * RB; i += kFewThreads) {
-      const int r = i / kn, k = i - r * kn;
-      sm[k * RB + r] = r < n_rows ? Num<T>::to_c(rows[r * p.a_ld + k0 + k]) : 0.0f;
+    // A thread brings four k of up to four rows at a time and writes the rows of a
+    // k side by side.
+    constexpr int G = RB < 4 ? RB : 4, kAcross = kFewThreads / (RB / G);
+    const int r0 = tid / kAcross * G;
+    for (int k = tid % kAcross; k < kn; k += 4 * kAcross) {
+      T v[4][G];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < G; ++r)
+          v[j][r] = rows[min(r0 + r, n_rows - 1) * p.a_ld + k0 + min(k + j * kAcross, kn - 1)];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (k + j * kAcross >= kn) break;
+        float* dst = sm + (k + j * kAcross) * RB + r0;
+        float f[G];
+#pragma unroll
+        for (int r = 0; r < G; ++r) f[r] = r0 + r < n_rows ? Num<T>::to_c(v[j][r]) : 0.0f;
+        if constexpr (G == 4) *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
+        else if constexpr (G == 2) *reinterpret_cast<float2*>(dst) = make_float2(f[0], f[1]);
+        else dst[0] = f[0];
+      }
     }
     __syncthreads();
     few_sums<T, RB, VEC>(w + (int64_t)k0 * p.b_ld, p.b_ld, kn, cols, sm, acc);
@@ -871,23 +912,30 @@ __device__ void few_item(const Args& p, int e, int64_t row0, int n_rows, int n0,
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[r][i] += __shfl_xor_sync(0xffffffffu, acc[r][i], 16);
   }
-  // sm: [W][RB][kFewCols] sums of the warps, then [RB][kFewCols] of the block in front.
+  // sm: [RB][kFewCols] sums of the block in front; behind them [W][H][kFewCols]
+  // sums of the warps, H rows at a time.
+  constexpr int H = RB < 4 ? RB : 4;
+  float* part = sm + RB * kFewCols;
+  static_assert((RB + W * H) * kFewCols <= kFewFloats, "sums of the warps");
   __syncthreads();
-  if (lane < L) {
 #pragma unroll
-    for (int r = 0; r < RB; ++r)
+  for (int h = 0; h < RB; h += H) {
+    if (lane < L) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) sm[(warp * RB + r) * kFewCols + x * V + i] = acc[r][i];
-  }
-  __syncthreads();
-  for (int i = tid; i < RB * kFewCols; i += kFewThreads) {
-    float s = 0.0f;
+      for (int r = 0; r < H; ++r)
 #pragma unroll
-    for (int q = 0; q < W; ++q) s += sm[q * RB * kFewCols + i];
-    sm[i] = s;
+        for (int i = 0; i < V; ++i) part[(warp * H + r) * kFewCols + x * V + i] = acc[h + r][i];
+    }
+    __syncthreads();
+    for (int i = tid; i < H * kFewCols; i += kFewThreads) {
+      float s = 0.0f;
+#pragma unroll
+      for (int q = 0; q < W; ++q) s += part[q * H * kFewCols + i];
+      sm[h * kFewCols + i] = s;
+    }
+    __syncthreads();
   }
   if (slices > 1) cluster_sync();
-  else __syncthreads();
   T* out = static_cast<T*>(p.c) + row0 * p.c_ld;
   for (int i = slice * kFewThreads + tid; i < n_rows * kFewCols; i += slices * kFewThreads) {
     const int r = i / kFewCols, n = n0 + i % kFewCols;
@@ -907,14 +955,15 @@ __device__ void few_item(const Args& p, int e, int64_t row0, int n_rows, int n0,
 
 template <class T, bool VEC>
 __global__ void __launch_bounds__(kFewThreads, 2) few_rows_kernel(const Args p, int slices) {
-  __shared__ __align__(16) float sm[kFewK * kFewRows];
+  __shared__ __align__(16) float sm[kFewFloats];
+  constexpr int kFewRows = Few<T>::rows;
   __shared__ int found[3];
   ops::let_successor_start();
   ops::wait_for_predecessor();
   const int tid = threadIdx.x, lane = tid & 31;
   const int strip = blockIdx.x / slices, slice = blockIdx.x % slices;
   if (tid < 32) {
-    // The item's group: items in expert order, 8 rows each.
+    // The item's group: items in expert order, kFewRows rows each.
     int base = 0, e = -1, row0 = 0, n = 0;
     for (int e0 = 0; e0 < p.experts && e < 0; e0 += 32) {
       const int i = e0 + lane;
@@ -959,7 +1008,8 @@ __global__ void __launch_bounds__(kFewThreads, 2) few_rows_kernel(const Args p, 
   if (n == 1) few_item<T, 1, VEC>(p, e, found[1], n, n0, slice, slices, sm);
   else if (n == 2) few_item<T, 2, VEC>(p, e, found[1], n, n0, slice, slices, sm);
   else if (n <= 4) few_item<T, 4, VEC>(p, e, found[1], n, n0, slice, slices, sm);
-  else few_item<T, 8, VEC>(p, e, found[1], n, n0, slice, slices, sm);
+  else if (Few<T>::rows == 8 || n <= 8) few_item<T, 8, VEC>(p, e, found[1], n, n0, slice, slices, sm);
+  else if constexpr (Few<T>::rows == 16) few_item<T, 16, VEC>(p, e, found[1], n, n0, slice, slices, sm);
 }
 
 // d_W_e = sum of its units' partial sums, in order.
@@ -1285,16 +1335,17 @@ ponni_b200_status launch_product(const Operand& a, const Operand& b, const Args&
   return ops::fail(PONNI_B200_ERR_UNSUPPORTED, "expert_product: no tile shape");
 }
 
-// Whether few_rows_kernel takes a forward product.  fp32: up to 16 rows a group on
+// Whether few_rows_kernel takes a forward product.  fp32: up to 48 rows a group on
 // average; the tensor-core path has to lay out split copies of all weights first
-// (64 experts of 1024 x 2048, 16 rows each: 279 us against 475; one expert of
-// 2048 x 2048, one row: 6.4 against 60).  16 bits: up to 8 rows where the 128-column
-// tiles do not fill the SMs (8 experts of 2048 x 1024: 10.5 / 11.1 / 16.6 us
-// with 1 / 4 / 8 rows each against 15.5 to 17.8; one expert: 5.4 to 11 against 14.3);
-// where they do, the tensor cores stream the weights as fast with any number
-// of rows (64 experts of 1024 x 2048: 49 to 51 us against 55 with one row each, 130 with 8).
+// (64 experts of 1024 x 2048: 92 / 116 / 173 / 297 / 424 us with 1 / 8 / 16 / 32 / 48
+// rows each against 415 to 434; 8 of 2048 x 1024: 13 / 24 / 71 with 1 / 16 / 48
+// against 75).  16 bits: up to 8 rows where the 128-column tiles do not fill the SMs
+// (8 experts of 2048 x 1024: 10.1 / 9.5 / 13.8 / 22.3 us with 1 / 4 / 8 / 12 rows each
+// against 15.4 to 17.6; one expert of 2048 x 2048: 5.3 to 9.9 with 1 to 16 against
+// 14.1); where they do, the tensor cores stream the weights as fast with any number
+// of rows (64 experts of 1024 x 2048: 49.5 to 52 us against 54 with one row each, 94 with 8).
 bool few_rows(int dtype, int64_t rows, int experts, int outputs, int sms) {
-  if (dtype == PONNI_B200_F32) return rows <= (int64_t)16 * experts;
+  if (dtype == PONNI_B200_F32) return rows <= (int64_t)48 * experts;
   const int64_t tiles = std::min<int64_t>(rows, experts) * ((outputs + 127) / 128);
   return tiles < sms && rows <= (int64_t)8 * (experts + 1);
 }
@@ -1304,7 +1355,7 @@ ponni_b200_status launch_few(const Args& p, int sms, cudaStream_t stream) {
   const bool vec = reinterpret_cast<uintptr_t>(p.b) % 16 == 0 && p.b_ld * sizeof(T) % 16 == 0 &&
                    (p.experts == 1 || p.b_stride * sizeof(T) % 16 == 0) && p.outputs * sizeof(T) % 16 == 0;
   const int64_t strips = (p.outputs + kFewCols - 1) / kFewCols;
-  const int64_t items = std::min<int64_t>(p.experts, p.rows) + p.rows / kFewRows;
+  const int64_t items = std::min<int64_t>(p.experts, p.rows) + p.rows / Few<T>::rows;
   // Slices of K until there are two blocks an SM, of 128 k at least.
   int slices = 1;
   while (slices < 8 && items * strips * slices < 2 * sms && p.inputs / (2 * slices) >= 128) slices *= 2;
