@@ -341,9 +341,10 @@ ponni_b200_status ponni_b200_fill_synthetic(ponni_b200_dtype dtype, void* device
  * creation of a gradient set excepted), may be captured, and restore the
  * caller's current device.  `dtype` is a ponni_b200_dtype.  A workspace is
  * caller-owned scratch of at least the bytes that the matching _workspace
- * function returns, aligned to 256 bytes, in use until the call's kernels
- * end.  Buffers of one call must not overlap.  The text of the calling thread's
- * last operator error is ponni_b200_operator_error(). */
+ * function returns, aligned to 256 bytes (a route workspace to 4, a clip workspace
+ * to 8), in use until the call's kernels end.  Buffers of one call must not
+ * overlap.  The text of the calling thread's last operator error is
+ * ponni_b200_operator_error(). */
 const char* ponni_b200_operator_error(void);
 /* Waits for `stream` and reports what the operators' kernels found on the
  * device since the last check: PONNI_B200_ERR_DEVICE (a bounded wait gave up),

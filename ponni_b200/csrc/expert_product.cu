@@ -77,6 +77,7 @@ struct Args {
   int vec;        // c may be written 16 bytes at a time
   int bulk;       // and by the copy engine (map_c)
   int stages;
+  int device;
   int* error;
 };
 
@@ -1271,7 +1272,8 @@ ponni_b200_status launch_shape(const Operand& a, const Operand& b, Args p, int s
   p.stages = std::min(kMaxStages, (kSmemLimit - fixed) / S::stage_bytes);
   const int smem = 1024 + p.stages * S::stage_bytes + S::epi_bytes + kBiasBytes + 2 * p.experts * (int)sizeof(int);
   auto kern = product_kernel<T, MODE, P, BN, CG>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = ops::allow_smem(reinterpret_cast<const void*>(kern), kSmemLimit - 1024, p.device, allowed);
   if (e != cudaSuccess) return ops::fail_cuda(e, "expert_product");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
@@ -1485,6 +1487,7 @@ ponni_b200_status ponni_b200_expert_product(int dtype, const void* rows, int64_t
     p.act_flags = activation_flags;
     p.s0 = (float)scalar0;
     p.s1 = (float)scalar1;
+    p.device = device;
     p.error = ops::error_word(device);
     if (!p.error) return ops::fail(PONNI_B200_ERR_CUDA, "no operator error word on this device");
     const int sms = ops::num_sms(device);
@@ -1557,6 +1560,7 @@ ponni_b200_status ponni_b200_expert_product_backward(int dtype, const void* d_ou
       p.experts = experts;
       p.inputs = inputs;
       p.outputs = outputs;
+      p.device = device;
       p.error = error;
       ponni_b200_status r = run_stages<T>(stages, sms, s);
       if (!r && d_rows) {

@@ -108,10 +108,8 @@ __device__ __forceinline__ double block_sum(double v, double* sums) {
   return t;
 }
 
-__global__ void __launch_bounds__(kBlock)
-    norm_kernel(const Chunk* __restrict__ chunks, int64_t num_chunks, double* __restrict__ partial) {
-  __shared__ double sums[kBlock / 32];
-  ops::let_successor_start();
+// This thread's part of the squares of the block's chunks.
+__device__ __forceinline__ double chunk_squares(const Chunk* __restrict__ chunks, int64_t num_chunks) {
   double s = 0.0;
   for (int64_t i = blockIdx.x; i < num_chunks; i += gridDim.x) {
     const Chunk c = chunks[i];
@@ -122,7 +120,14 @@ __global__ void __launch_bounds__(kBlock)
       default: s += squares(static_cast<const __nv_bfloat16*>(c.p), c.count); break;
     }
   }
-  const double t = block_sum(s, sums);
+  return s;
+}
+
+__global__ void __launch_bounds__(kBlock)
+    norm_kernel(const Chunk* __restrict__ chunks, int64_t num_chunks, double* __restrict__ partial) {
+  __shared__ double sums[kBlock / 32];
+  ops::let_successor_start();
+  const double t = block_sum(chunk_squares(chunks, num_chunks), sums);
   if (threadIdx.x == 0) partial[blockIdx.x] = t;
 }
 
@@ -189,15 +194,9 @@ __device__ __forceinline__ void rescale_to(const Chunk& c, void* flat, int flat_
   }
 }
 
-__global__ void __launch_bounds__(kBlock)
-    clip_kernel(const Chunk* __restrict__ chunks, int64_t num_chunks, const double* __restrict__ partial,
-                int num_partial, double max_norm, void* __restrict__ flat, int flat_dtype, float* __restrict__ norm_out) {
-  __shared__ double sums[kBlock / 32];
-  ops::wait_for_predecessor();
-  double s = 0.0;
-  for (int i = threadIdx.x; i < num_partial; i += kBlock) s += partial[i];
-  const double norm = sqrt(block_sum(s, sums));
-  if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
+// Scales (or packs) the block's chunks, the last ones first, by the norm over all.
+__device__ __forceinline__ void clip_chunks(const Chunk* __restrict__ chunks, int64_t num_chunks, double norm,
+                                            double max_norm, void* flat, int flat_dtype) {
   const bool clip = norm > max_norm && norm < (double)INFINITY;
   if (!clip && flat_dtype < 0) return;
   const double scale = clip ? max_norm / norm : 1.0;
@@ -210,6 +209,45 @@ __global__ void __launch_bounds__(kBlock)
       default: rescale_to<__nv_bfloat16>(c, flat, flat_dtype, scale); break;
     }
   }
+}
+
+__global__ void __launch_bounds__(kBlock)
+    clip_kernel(const Chunk* __restrict__ chunks, int64_t num_chunks, const double* __restrict__ partial,
+                int num_partial, double max_norm, void* __restrict__ flat, int flat_dtype, float* __restrict__ norm_out) {
+  __shared__ double sums[kBlock / 32];
+  ops::let_successor_start();
+  ops::wait_for_predecessor();
+  double s = 0.0;
+  for (int i = threadIdx.x; i < num_partial; i += kBlock) s += partial[i];
+  const double norm = sqrt(block_sum(s, sums));
+  if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
+  clip_chunks(chunks, num_chunks, norm, max_norm, flat, flat_dtype);
+}
+
+// Both passes in one launch, by one cluster whose blocks read one another's
+// sums: for sets of at most kOneClusterChunks chunks, where the second launch
+// costs more than the work.
+constexpr int kCluster = 8, kOneClusterChunks = 4 * kCluster;
+__global__ void __launch_bounds__(kBlock)
+    clip_one_cluster_kernel(const Chunk* __restrict__ chunks, int64_t num_chunks, double max_norm,
+                            void* __restrict__ flat, int flat_dtype, float* __restrict__ norm_out) {
+  __shared__ double sums[kBlock / 32];
+  __shared__ double mine;
+  const double t = block_sum(chunk_squares(chunks, num_chunks), sums);
+  if (threadIdx.x == 0) mine = t;
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;\n" ::: "memory");
+  double s = 0.0;
+  for (int q = 0; q < (int)gridDim.x; ++q) {
+    uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(&mine)), r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(q));
+    double v;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];\n" : "=d"(v) : "r"(r) : "memory");
+    s += v;
+  }
+  const double norm = sqrt(s);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
+  clip_chunks(chunks, num_chunks, norm, max_norm, flat, flat_dtype);
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;\n" ::: "memory");
 }
 
 }  // namespace
@@ -298,8 +336,25 @@ ponni_b200_status ponni_b200_gradient_set_clip(ponni_b200_gradient_set* set, dou
     const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>(set->num_chunks, kMaxBlocks));
     const Chunk* chunks = static_cast<const Chunk*>(set->chunks);
     double* partial = static_cast<double*>(workspace);
+    cudaError_t e = cudaSuccess;
+    if (set->num_chunks <= kOneClusterChunks) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = std::min(blocks, kCluster);
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.gridDim = dim3(std::min(blocks, kCluster));
+      cfg.blockDim = dim3(kBlock);
+      cfg.stream = s;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      e = cudaLaunchKernelEx(&cfg, clip_one_cluster_kernel, chunks, set->num_chunks, max_norm, flat,
+                             flat ? flat_dtype : -1, norm);
+      return e == cudaSuccess ? PONNI_B200_OK : ops::fail_cuda(e, "clip");
+    }
     norm_kernel<<<blocks, kBlock, 0, s>>>(chunks, set->num_chunks, partial);
-    cudaError_t e = cudaGetLastError();
+    e = cudaGetLastError();
     if (e == cudaSuccess)
       e = ops::launch_after(clip_kernel, dim3(blocks), dim3(kBlock), 0, s, chunks, set->num_chunks,
                             (const double*)partial, blocks, max_norm, flat, flat ? flat_dtype : -1, norm);

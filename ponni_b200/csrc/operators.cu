@@ -65,6 +65,26 @@ int num_sms(int device) {
   return g_device[device].sms;
 }
 
+int num_devices() {
+  static const int n = [] {
+    int c = 0;
+    if (cudaGetDeviceCount(&c) != cudaSuccess) {
+      cudaGetLastError();
+      c = 0;
+    }
+    return c;
+  }();
+  return n;
+}
+
+cudaError_t allow_smem(const void* kernel, int bytes, int device, std::atomic<uint64_t>& done) {
+  const uint64_t bit = device >= 0 && device < kMaxDevices ? 1ull << device : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
 }  // namespace ops
 }  // namespace ponni_b200
 

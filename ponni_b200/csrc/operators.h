@@ -4,6 +4,7 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <string>
 
@@ -26,17 +27,19 @@ ponni_b200_status launched(const char* what);
 int* error_word(int device);
 
 int num_sms(int device);
+int num_devices();  // asked once; 0 without a driver
+
+// Lets `kernel` use up to `bytes` of dynamic shared memory on `device`; `done` is
+// the kernel's own mask of the devices on which this has been said.
+cudaError_t allow_smem(const void* kernel, int bytes, int device, std::atomic<uint64_t>& done);
 
 // Runs `body` (returning a status) with `device` current and no exception
 // leaving the C entry.
 template <class F>
 ponni_b200_status entry(int device, F&& body) noexcept {
   try {
-    int n = 0;
-    if (cudaGetDeviceCount(&n) != cudaSuccess) {
-      cudaGetLastError();
-      return fail(PONNI_B200_ERR_CUDA, "no CUDA device");
-    }
+    const int n = num_devices();
+    if (n == 0) return fail(PONNI_B200_ERR_CUDA, "no CUDA device");
     if (device < 0 || device >= n)
       return fail(PONNI_B200_ERR_INVALID_ARGUMENT, "device " + std::to_string(device) + " does not exist");
     DeviceGuard guard(device);

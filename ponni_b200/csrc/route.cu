@@ -252,21 +252,36 @@ __global__ void __launch_bounds__(kBlock)
   place(expert, experts, top_k, batch, c0, min(batch, c0 + per_block), next, mask, row, column);
 }
 
-// All of it in one block, for batches of at most kOneBlock columns: three
-// dependent launches cost more than the work of a few tiles.
-constexpr int64_t kOneBlock = 2 * kBlock;
+// All of it in one launch, by one cluster of up to 8 blocks, for batches of at
+// most kOneCluster columns: three dependent launches cost more than the work of
+// two tiles a block.  The blocks read one another's counts through distributed shared memory.
+constexpr int kMaxCluster = 8;
+constexpr int64_t kOneCluster = 2 * kMaxCluster * kBlock;
+__device__ __forceinline__ int read_block(const int* p, int rank) {
+  uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(p)), r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(rank));
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(v) : "r"(r) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;\n" ::: "memory");
+}
 template <class T, int K>
 __global__ void __launch_bounds__(kBlock)
-    route_one_block_kernel(const T* __restrict__ x, int64_t ld, int experts, int batch, int over_all, int* expert,
-                           float* __restrict__ weight, int* row, int* column, int* __restrict__ offset) {
+    route_one_cluster_kernel(const T* __restrict__ x, int64_t ld, int experts, int batch, int per_block, int over_all,
+                             int* expert, float* __restrict__ weight, int* row, int* column, int* __restrict__ offset) {
   extern __shared__ int sm[];
   __shared__ int warp_sums[kWarps];
-  int* next = sm;
-  unsigned* mask = reinterpret_cast<unsigned*>(sm + experts);
-  for (int i = threadIdx.x; i < experts; i += kBlock) next[i] = 0;
+  int* hist = sm;                                                  // [experts]: this block's counts
+  int* next = sm + experts;                                        // [experts]
+  unsigned* mask = reinterpret_cast<unsigned*>(sm + 2 * experts);  // [kWarps][experts]
+  const int rank = blockIdx.x, blocks = gridDim.x;
+  for (int i = threadIdx.x; i < experts; i += kBlock) hist[i] = 0;
   for (int i = threadIdx.x; i < kWarps * experts; i += kBlock) mask[i] = 0;
   __syncthreads();
-  for (int b = threadIdx.x; b < batch; b += kBlock) {
+  const int c0 = rank * per_block, c1 = min(batch, c0 + per_block);
+  for (int b = c0 + threadIdx.x; b < c1; b += kBlock) {
     int idx[K];
     float w[K];
     choose<T, K>(x + b, ld, experts, over_all, idx, w);
@@ -274,22 +289,34 @@ __global__ void __launch_bounds__(kBlock)
     for (int j = 0; j < K; ++j) {
       expert[j * batch + b] = idx[j];
       weight[j * batch + b] = w[j];
-      if (idx[j] >= 0) atomicAdd(&next[idx[j]], 1);
+      if (idx[j] >= 0) atomicAdd(&hist[idx[j]], 1);
     }
   }
   __syncthreads();
+  if (blocks > 1) cluster_barrier();
   int carry = 0;
   for (int e0 = 0; e0 < experts; e0 += kBlock) {
     const int e = e0 + threadIdx.x;
-    int total;
-    const int before = carry + block_scan(e < experts ? next[e] : 0, warp_sums, total);
-    if (e < experts) offset[e] = next[e] = before;
+    int all = 0, earlier = 0, total;
+    if (e < experts) {
+      for (int q = 0; q < blocks; ++q) {
+        const int n = blocks > 1 ? read_block(hist + e, q) : hist[e];
+        all += n;
+        earlier += q < rank ? n : 0;
+      }
+    }
+    const int before = carry + block_scan(all, warp_sums, total);
+    if (e < experts) {
+      next[e] = before + earlier;
+      if (rank == 0) offset[e] = before;
+    }
     carry += total;
   }
-  if (threadIdx.x == 0) offset[experts] = carry;
-  for (int i = carry + threadIdx.x; i < batch * K; i += kBlock) column[i] = -1;
+  if (blocks > 1) cluster_barrier();  // the others have read this block's counts
+  if (rank == 0 && threadIdx.x == 0) offset[experts] = carry;
+  for (int i = carry + rank * kBlock + threadIdx.x; i < batch * K; i += blocks * kBlock) column[i] = -1;
   __syncthreads();
-  place(expert, experts, K, batch, 0, batch, next, mask, row, column);
+  place(expert, experts, K, batch, c0, c1, next, mask, row, column);
 }
 
 // d_x[e][b] = p_e (d_p_e - sum_j w_j d_w_j), d_p_e = d_w_j for the chosen
@@ -383,7 +410,7 @@ using namespace ponni_b200;
 extern "C" {
 
 int64_t ponni_b200_route_workspace(int num_experts, int64_t batch) {
-  if (num_experts < 1 || batch <= kOneBlock) return 0;
+  if (num_experts < 1 || batch <= kOneCluster) return 0;
   return (int64_t)num_experts * (blocks_of(batch) + 1) * (int64_t)sizeof(int);
 }
 
@@ -406,10 +433,24 @@ ponni_b200_status ponni_b200_route_columns(int dtype, const void* logits, int64_
       using T = decltype(t);
       constexpr int K = decltype(k)::value;
       const T* x = static_cast<const T*>(logits);
-      if (batch <= kOneBlock) {
-        route_one_block_kernel<T, K><<<1, kBlock, place_smem, s>>>(x, ld, num_experts, (int)batch, all, expert, weight,
-                                                                  row, column, offset);
-        return ops::launched("route_columns");
+      if (batch <= kOneCluster) {
+        const int blocks = (int)std::min<int64_t>(kMaxCluster, (batch + kBlock - 1) / kBlock);
+        const int per = (int)((batch + blocks - 1) / blocks);
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = blocks;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.gridDim = dim3(blocks);
+        cfg.blockDim = dim3(kBlock);
+        cfg.dynamicSmemBytes = (size_t)num_experts * (kWarps + 2) * sizeof(int);
+        cfg.stream = s;
+        cfg.attrs = attr;
+        cfg.numAttrs = blocks > 1 ? 1 : 0;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, route_one_cluster_kernel<T, K>, x, ld, num_experts, (int)batch, per,
+                                                 all, expert, weight, row, column, offset);
+        return e == cudaSuccess ? PONNI_B200_OK : ops::fail_cuda(e, "route_columns");
       }
       const int64_t tiles = (batch + kBlock - 1) / kBlock, most = blocks_of(batch);
       const int64_t per_block = (tiles + most - 1) / most * kBlock;

@@ -28,14 +28,21 @@ from .layers import Layer
 
 _NORMALISE = {"selected": _abi.ROUTE_SELECTED, "all": _abi.ROUTE_ALL}
 _codes: dict = {}
+_modules: list = []
 
 
 def _torch():
-    import torch
-    if not _codes:
+    if not _modules:
+        import torch
         _codes.update({torch.float32: _abi.F32, torch.float64: _abi.F64, torch.float16: _abi.F16,
                        torch.bfloat16: _abi.BF16})
-    return torch
+        _modules.append(torch)
+    return _modules[0]
+
+
+def _empty(torch, rows: int, cols: int, dtype, device):
+    """A dense matrix (empty_strided: half the call's time of empty with a shape)."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
 
 
 def _refuse(message: str, status: int = 1):
@@ -59,19 +66,18 @@ def _real(t, what: str) -> int:
 
 def _matrix(t, what: str) -> int:
     """Row stride of a 2-D tensor whose second index is contiguous."""
-    if t.dim() != 2:
+    shape = t.shape
+    if len(shape) != 2:
         _refuse(f"{what} must be two-dimensional")
-    rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
+    rows, cols = shape
+    ld, one = t.stride()
+    if cols > 1 and one != 1:
         _refuse(f"{what} must be LayoutRight (second index contiguous)")
-    ld = t.stride(0)
-    return ld if rows > 1 and ld >= cols else _only_row(t, what)
-
-
-def _only_row(t, what: str) -> int:
-    if t.shape[0] > 1:
+    if rows <= 1:
+        return max(1, cols)
+    if ld < cols:
         _refuse(f"{what} has overlapping rows")
-    return max(1, t.shape[1])
+    return ld
 
 
 def _like(t, shape, dtype, device, what: str):
@@ -96,7 +102,7 @@ class Routing(NamedTuple):
 
 
 def _check_routing(r: Routing, device, batch: int):
-    import torch
+    torch = _torch()
     shape = r.row.shape
     if len(shape) != 2 or shape[1] != batch:
         _refuse(f"the routing is for {shape[-1]} columns, not {batch}", 2)
@@ -107,7 +113,7 @@ def _check_routing(r: Routing, device, batch: int):
 
 def _output(out, shape, like, what: str):
     if out is None:
-        return like.new_empty(shape)
+        return _empty(_torch(), *shape, like.dtype, like.device)
     if out.shape != shape or out.dtype != like.dtype or out.device != like.device:
         _refuse(f"{what} must be a {like.dtype} tensor of shape {tuple(shape)} on {like.device}", 2)
     return out
@@ -117,11 +123,9 @@ def _row_output(out, rows: int, features: int, like):
     """Rows with a stride of whole 16-byte vectors, as the tensor-core product reads them without a copy."""
     if out is not None:
         return _output(out, (rows, features), like, "out")
-    per = 16 // like.element_size()
-    pad = -features % per
-    if not pad:
-        return like.new_empty((rows, features))
-    return like.new_empty((rows, features + pad))[:, :features]
+    pad = -features % (16 // like.element_size())
+    t = _empty(_torch(), rows, features + pad, like.dtype, like.device)
+    return t[:, :features] if pad else t
 
 
 def route_columns(logits, top_k: int, normalise: str = "selected") -> Routing:
@@ -144,19 +148,18 @@ def route_columns(logits, top_k: int, normalise: str = "selected") -> Routing:
     if not 1 <= top_k <= min(8, experts):
         _refuse(f"top_k must be 1 to 8 and at most the {experts} experts, not {top_k}", 3)
     dev, L = logits.device, _abi.lib()
-    shape = (top_k, batch)
-    i32 = torch.int32
-    expert, row = torch.empty(shape, dtype=i32, device=dev), torch.empty(shape, dtype=i32, device=dev)
-    weight = torch.empty(shape, dtype=torch.float32, device=dev)
-    column = torch.empty(top_k * batch, dtype=i32, device=dev)
-    offset = torch.empty(experts + 1, dtype=i32, device=dev)
+    # One allocation (five cost more than its views): expert, row, column, weight, offset, workspace.
+    n = top_k * batch
     need = L.ponni_b200_route_workspace(experts, batch)
-    space = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(L.ponni_b200_route_columns(code, logits.data_ptr(), ld, experts, top_k, batch, _NORMALISE[normalise],
-                                     expert.data_ptr(), weight.data_ptr(), row.data_ptr(), column.data_ptr(),
-                                     offset.data_ptr(), space.data_ptr() if need else None, need, dev.index,
+    buf = torch.empty(4 * n + experts + 1 + need // 4, dtype=torch.int32, device=dev)
+    at, shape, stride = buf.data_ptr(), (top_k, batch), (batch, 1)
+    space = at + 16 * n + 4 * (experts + 1)
+    _call(L.ponni_b200_route_columns(code, logits.data_ptr(), ld, experts, top_k, batch, _NORMALISE[normalise], at,
+                                     at + 12 * n, at + 4 * n, at + 8 * n, at + 16 * n, space, need, dev.index,
                                      torch_stream_handle(dev)))
-    return Routing(expert, weight, row, column, offset)
+    return Routing(buf.as_strided(shape, stride), buf.view(torch.float32).as_strided(shape, stride, 3 * n),
+                   buf.as_strided(shape, stride, n), buf.as_strided((n,), (1,), 2 * n),
+                   buf.as_strided((experts + 1,), (1,), 4 * n))
 
 
 def route_columns_backward(logits, routing: Routing, d_weight, normalise: str = "selected"):
@@ -172,7 +175,7 @@ def route_columns_backward(logits, routing: Routing, d_weight, normalise: str = 
     for t, dt, what in ((routing.expert, torch.int32, "routing.expert"), (routing.weight, torch.float32, "routing.weight"),
                         (d_weight, torch.float32, "d_weight")):
         _like(t, (top_k, batch), dt, dev, what)
-    d = torch.empty((experts, batch), dtype=logits.dtype, device=dev)
+    d = _empty(torch, experts, batch, logits.dtype, dev)
     _call(_abi.lib().ponni_b200_route_columns_backward(
         code, logits.data_ptr(), ld, experts, top_k, batch, _NORMALISE[normalise], routing.expert.data_ptr(),
         routing.weight.data_ptr(), d_weight.data_ptr(), d.data_ptr(), batch, dev.index, torch_stream_handle(dev)))
@@ -242,7 +245,7 @@ def combine_rows_backward(d_y, rows, routing: Routing):
         _refuse(f"rows must be a {d_y.dtype} tensor of shape {(batch * top_k, features)} on {dev}", 2)
     _like(routing.weight, routing.row.shape, torch.float32, dev, "routing.weight")
     d_rows = _row_output(None, batch * top_k, features, d_y)
-    d_weight = torch.empty((top_k, batch), dtype=torch.float32, device=dev)
+    d_weight = _empty(torch, top_k, batch, torch.float32, dev)
     _call(_abi.lib().ponni_b200_combine_rows_backward(
         code, d_y.data_ptr(), ld, rows.data_ptr(), _matrix(rows, "rows"), features, batch, top_k,
         routing.row.data_ptr(), routing.weight.data_ptr(),
@@ -271,14 +274,16 @@ def _check_product(rows, weights, offset, what="rows"):
 
 
 def _space(L, code, total, experts, inputs, outputs, addresses, strides, backward, dev):
-    """(tensor or None, bytes, address) of the product's workspace; the allocator's blocks are 512-byte aligned."""
-    aligned = code != _abi.F32 and not (sum(a & 15 for a in addresses) or sum(s & 7 for s in strides))
+    """(tensor or None, bytes, address) of the product's workspace; the allocator's blocks are 512-byte aligned.
+
+    `addresses`, `strides`: those of all operands, or-ed."""
+    aligned = code != _abi.F32 and not (addresses & 15 or strides & 7)
     if aligned and not backward:
         return None, 0, None
     need = L.ponni_b200_expert_product_workspace(code, total, experts, inputs, outputs, aligned, backward, dev.index)
     if not need:
         return None, 0, None
-    import torch
+    torch = _torch()
     t = torch.empty(need, dtype=torch.uint8, device=dev)
     return t, need, t.data_ptr()
 
@@ -309,7 +314,7 @@ def expert_product(rows, weights, offset, bias=None, activation: Layer | None = 
     out = _row_output(out, total, outputs, rows)
     L = _abi.lib()
     x, w = rows.data_ptr(), weights.data_ptr()
-    space, need, at = _space(L, code, total, experts, inputs, outputs, (x, w), (ld, w_ld, stride), 0, dev)
+    space, need, at = _space(L, code, total, experts, inputs, outputs, x | w, ld | w_ld | stride, 0, dev)
     _call(L.ponni_b200_expert_product(
         code, x, ld, total, w, w_ld, stride,
         None if bias is None else bias.data_ptr(), offset.data_ptr(), experts, inputs, outputs, kind, flags, s0, s1,
@@ -335,11 +340,11 @@ def expert_product_backward(d_out, rows, weights, offset, bias: bool = True, nee
     dev = rows.device
     d_rows = _row_output(None, total, inputs, rows) if need_rows else None
     d_weights = torch.empty((experts, inputs, outputs), dtype=rows.dtype, device=dev) if need_weights else None
-    d_bias = torch.empty((experts, outputs), dtype=rows.dtype, device=dev) if bias else None
+    d_bias = _empty(torch, experts, outputs, rows.dtype, dev) if bias else None
     L = _abi.lib()
     d, x, w = d_out.data_ptr(), rows.data_ptr(), weights.data_ptr()
     d_ld, ld = _matrix(d_out, "d_out"), _matrix(rows, "rows")
-    space, need, at = _space(L, code, total, experts, inputs, outputs, (d, x, w), (d_ld, ld, w_ld, stride), 1, dev)
+    space, need, at = _space(L, code, total, experts, inputs, outputs, d | x | w, d_ld | ld | w_ld | stride, 1, dev)
     _call(L.ponni_b200_expert_product_backward(
         code, d, d_ld, x, ld, total, w, w_ld, stride, offset.data_ptr(), experts, inputs, outputs,
         None if d_rows is None else d_rows.data_ptr(), 0 if d_rows is None else _matrix(d_rows, "d_rows"),
@@ -398,7 +403,7 @@ class GradientSet:
         values that receives all gradients in tensor order (the order of
         Inference.set_trainable_parameters_device) and leaves them as they are.
         """
-        import torch
+        torch = _torch()
         kind, flat = 0, None
         if out is not None:
             if out.device != self.device or out.dim() != 1 or out.numel() != self.total or not out.is_contiguous():
