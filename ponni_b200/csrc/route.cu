@@ -50,31 +50,33 @@ __device__ __forceinline__ float from_best(float v, float best) {
 }
 __device__ __forceinline__ float at_least_finite(float best) { return fmaxf(best, -3.402823466e38f); }
 
-// Choice and weights of one column; K is the number of choices.  Logits come in
-// chunks of kChunk, the next chunk's loads ahead of this one's work.  Insertion
-// has no branches: some lane of a warp inserts at nearly every expert.
+// The K largest of `count` logits (rows of x, ld apart), largest first, and the
+// sum of exp(x - best) over all of them.  Logits come in chunks of kChunk, the next
+// chunk's loads ahead of this one's work.  Insertion has no branches: some lane of
+// a warp inserts at nearly every expert.
 constexpr int kChunk = 8;
 template <class T, int K>
-__device__ __forceinline__ void choose(const T* __restrict__ x, int64_t ld, int experts, bool over_all, int (&idx)[K],
-                                       float (&w)[K]) {
-  float top[K];
+__device__ __forceinline__ void scan_logits(const T* __restrict__ x, int64_t ld, int count, bool over_all, int (&idx)[K],
+                                            float (&top)[K], float& best, float& sum) {
 #pragma unroll
   for (int j = 0; j < K; ++j) {
     top[j] = -INFINITY;
     idx[j] = -1;
   }
-  float sum = 0.0f, best = -3.402823466e38f;  // sum of exp(x - best) over the experts seen
+  sum = 0.0f;
+  best = -3.402823466e38f;
+  if (count < 1) return;
   T ahead[kChunk];
-  load_logits<T, kChunk>(x, ld, 0, experts, ahead);
-  for (int e0 = 0; e0 < experts; e0 += kChunk) {
+  load_logits<T, kChunk>(x, ld, 0, count, ahead);
+  for (int e0 = 0; e0 < count; e0 += kChunk) {
     float v[kChunk];
 #pragma unroll
     for (int u = 0; u < kChunk; ++u) v[u] = as_logit(ahead[u]);
-    if (e0 + kChunk > experts) {
+    if (e0 + kChunk > count) {
 #pragma unroll
-      for (int u = 0; u < kChunk; ++u) v[u] = e0 + u < experts ? v[u] : -INFINITY;
+      for (int u = 0; u < kChunk; ++u) v[u] = e0 + u < count ? v[u] : -INFINITY;
     }
-    load_logits<T, kChunk>(x, ld, e0 + kChunk, experts, ahead);
+    if (e0 + kChunk < count) load_logits<T, kChunk>(x, ld, e0 + kChunk, count, ahead);
     if (over_all) {
       float now = best;
 #pragma unroll
@@ -99,6 +101,56 @@ __device__ __forceinline__ void choose(const T* __restrict__ x, int64_t ld, int 
       }
     }
   }
+}
+
+// Choice and weights of one column by G neighbouring lanes (all of the warp call
+// it): each scans every G-th expert, then the lanes' lists are merged.  With G = 1
+// the insertions of 256 experts alone take 23 us, and small batches have lanes to spare.
+template <class T, int K, int G>
+__device__ __forceinline__ void choose(const T* __restrict__ x, int64_t ld, int experts, bool over_all, int (&idx)[K],
+                                       float (&w)[K]) {
+  float top[K], best, sum;
+  const int g = G > 1 ? threadIdx.x % G : 0;
+  scan_logits<T, K>(x + g * ld, ld * G, (experts - g + G - 1) / G, over_all, idx, top, best, sum);
+  if constexpr (G > 1) {
+    int mine[K];
+    float have[K];
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      mine[j] = idx[j] < 0 ? -1 : idx[j] * G + g;
+      have[j] = top[j];
+    }
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      float v = have[0];
+      int i = mine[0];
+#pragma unroll
+      for (int d = 1; d < G; d <<= 1) {
+        const float ov = __shfl_xor_sync(0xffffffffu, v, d);
+        const int oi = __shfl_xor_sync(0xffffffffu, i, d);
+        if (oi >= 0 && (i < 0 || ov > v || (ov == v && oi < i))) {
+          v = ov;
+          i = oi;
+        }
+      }
+      top[j] = v;
+      idx[j] = i;
+      if (i >= 0 && i == mine[0]) {
+#pragma unroll
+        for (int q = 0; q + 1 < K; ++q) {
+          mine[q] = mine[q + 1];
+          have[q] = have[q + 1];
+        }
+        mine[K - 1] = -1;
+        have[K - 1] = -INFINITY;
+      }
+    }
+    if (over_all) {
+      sum *= from_best(best, at_least_finite(top[0]));
+#pragma unroll
+      for (int d = 1; d < G; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    }
+  }
   best = at_least_finite(top[0]);
 #pragma unroll
   for (int j = 0; j < K; ++j) w[j] = idx[j] < 0 ? 0.0f : from_best(top[j], best);
@@ -113,7 +165,7 @@ __device__ __forceinline__ void choose(const T* __restrict__ x, int64_t ld, int 
 
 // Choices of this block's columns [c0, c1) and how many of them each expert
 // took: counts[expert][block].
-template <class T, int K>
+template <class T, int K, int G>
 __global__ void __launch_bounds__(kBlock)
     choose_kernel(const T* __restrict__ x, int64_t ld, int experts, int64_t batch, int64_t per_block, int over_all,
                   int* __restrict__ expert, float* __restrict__ weight, int* __restrict__ counts) {
@@ -122,15 +174,18 @@ __global__ void __launch_bounds__(kBlock)
   for (int e = threadIdx.x; e < experts; e += kBlock) hist[e] = 0;
   __syncthreads();
   const int64_t c0 = blockIdx.x * per_block, c1 = min(batch, c0 + per_block);
-  for (int64_t b = c0 + threadIdx.x; b < c1; b += kBlock) {
+  for (int64_t b0 = c0; b0 < c1; b0 += kBlock / G) {
+    const int64_t b = b0 + threadIdx.x / G;
     int idx[K];
     float w[K];
-    choose<T, K>(x + b, ld, experts, over_all, idx, w);
+    choose<T, K, G>(x + min(b, c1 - 1), ld, experts, over_all, idx, w);
+    if (b < c1 && threadIdx.x % G == 0) {
 #pragma unroll
-    for (int j = 0; j < K; ++j) {
-      expert[j * batch + b] = idx[j];
-      weight[j * batch + b] = w[j];
-      if (idx[j] >= 0) atomicAdd(&hist[idx[j]], 1);
+      for (int j = 0; j < K; ++j) {
+        expert[j * batch + b] = idx[j];
+        weight[j * batch + b] = w[j];
+        if (idx[j] >= 0) atomicAdd(&hist[idx[j]], 1);
+      }
     }
   }
   __syncthreads();
@@ -252,11 +307,12 @@ __global__ void __launch_bounds__(kBlock)
   place(expert, experts, top_k, batch, c0, min(batch, c0 + per_block), next, mask, row, column);
 }
 
-// All of it in one launch, by one cluster of up to 8 blocks, for batches of at
-// most kOneCluster columns: three dependent launches cost more than the work of
-// two tiles a block.  The blocks read one another's counts through distributed shared memory.
+// All of it in one launch, by one cluster of up to 8 blocks, for small batches:
+// three dependent launches cost more than the work.  Up to kGrouped columns, kGroup lanes take a column.  The blocks read one another's counts through distributed shared memory.
 constexpr int kMaxCluster = 8;
-constexpr int64_t kOneCluster = 2 * kMaxCluster * kBlock;
+constexpr int64_t kOneCluster = kMaxCluster * kBlock;
+constexpr int kGroup = 8;
+constexpr int64_t kGrouped = 2 * kMaxCluster * kBlock / kGroup;
 __device__ __forceinline__ int read_block(const int* p, int rank) {
   uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(p)), r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(rank));
@@ -267,7 +323,7 @@ __device__ __forceinline__ int read_block(const int* p, int rank) {
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;\n" ::: "memory");
 }
-template <class T, int K>
+template <class T, int K, int G>
 __global__ void __launch_bounds__(kBlock)
     route_one_cluster_kernel(const T* __restrict__ x, int64_t ld, int experts, int batch, int per_block, int over_all,
                              int* expert, float* __restrict__ weight, int* row, int* column, int* __restrict__ offset) {
@@ -281,15 +337,18 @@ __global__ void __launch_bounds__(kBlock)
   for (int i = threadIdx.x; i < kWarps * experts; i += kBlock) mask[i] = 0;
   __syncthreads();
   const int c0 = rank * per_block, c1 = min(batch, c0 + per_block);
-  for (int b = c0 + threadIdx.x; b < c1; b += kBlock) {
+  for (int b0 = c0; b0 < c1; b0 += kBlock / G) {
+    const int b = b0 + threadIdx.x / G;
     int idx[K];
     float w[K];
-    choose<T, K>(x + b, ld, experts, over_all, idx, w);
+    choose<T, K, G>(x + min(b, c1 - 1), ld, experts, over_all, idx, w);
+    if (b < c1 && threadIdx.x % G == 0) {
 #pragma unroll
-    for (int j = 0; j < K; ++j) {
-      expert[j * batch + b] = idx[j];
-      weight[j * batch + b] = w[j];
-      if (idx[j] >= 0) atomicAdd(&hist[idx[j]], 1);
+      for (int j = 0; j < K; ++j) {
+        expert[j * batch + b] = idx[j];
+        weight[j * batch + b] = w[j];
+        if (idx[j] >= 0) atomicAdd(&hist[idx[j]], 1);
+      }
     }
   }
   __syncthreads();
@@ -358,7 +417,25 @@ __global__ void __launch_bounds__(kBlock)
     if (idx[j] >= e0 && idx[j] < e0 + kBackPart) dx[(int64_t)idx[j] * d_ld + b] = Num<T>::from_c(g[j] - w[j] * mean);
 }
 
-int64_t blocks_of(int64_t batch) { return std::min<int64_t>((batch + kBlock - 1) / kBlock, 592); }
+// Whether one cluster does all: 16 experts take 5 us with up to 2048 columns (7 in
+// three launches, which also cost the host two launches more), 256 experts
+// 12 us with 256 columns, but 35 with 1024 against 14 on all SMs.
+bool one_cluster(int experts, int64_t batch) { return batch <= kGrouped / 2 || (batch <= kOneCluster && experts <= 64); }
+
+// Columns of a block of the three-launch form: whole tiles for at most 592 blocks.
+// Where the columns do not fill the SMs with work, kGroup lanes take a column and
+// a tile is so much smaller (256 experts: 14.8 us against 44 with 4096 columns, 27
+// against 44 with 16384; 16 experts: 9.9 against 7.0 with 16384).
+bool spread(int experts, int64_t batch) { return batch <= (int64_t)128 * experts; }
+int64_t columns_of_block(int experts, int64_t batch) {
+  const int64_t tile = spread(experts, batch) ? kBlock / kGroup : kBlock;
+  const int64_t tiles = (batch + tile - 1) / tile;
+  return (tiles + 591) / 592 * tile;
+}
+int64_t blocks_of(int experts, int64_t batch) {
+  const int64_t per = columns_of_block(experts, batch);
+  return (batch + per - 1) / per;
+}
 
 // f(T, K) for the type and the number of choices.
 template <class T, class F>
@@ -410,8 +487,8 @@ using namespace ponni_b200;
 extern "C" {
 
 int64_t ponni_b200_route_workspace(int num_experts, int64_t batch) {
-  if (num_experts < 1 || batch <= kOneCluster) return 0;
-  return (int64_t)num_experts * (blocks_of(batch) + 1) * (int64_t)sizeof(int);
+  if (num_experts < 1 || batch < 1 || one_cluster(num_experts, batch)) return 0;
+  return (int64_t)num_experts * (blocks_of(num_experts, batch) + 1) * (int64_t)sizeof(int);
 }
 
 ponni_b200_status ponni_b200_route_columns(int dtype, const void* logits, int64_t ld, int num_experts, int top_k,
@@ -433,8 +510,9 @@ ponni_b200_status ponni_b200_route_columns(int dtype, const void* logits, int64_
       using T = decltype(t);
       constexpr int K = decltype(k)::value;
       const T* x = static_cast<const T*>(logits);
-      if (batch <= kOneCluster) {
-        const int blocks = (int)std::min<int64_t>(kMaxCluster, (batch + kBlock - 1) / kBlock);
+      if (one_cluster(num_experts, batch)) {
+        const int64_t at_once = batch <= kGrouped ? kBlock / kGroup : kBlock;
+        const int blocks = (int)std::min<int64_t>(kMaxCluster, (batch + at_once - 1) / at_once);
         const int per = (int)((batch + blocks - 1) / blocks);
         cudaLaunchConfig_t cfg = {};
         cudaLaunchAttribute attr[1];
@@ -448,17 +526,18 @@ ponni_b200_status ponni_b200_route_columns(int dtype, const void* logits, int64_
         cfg.stream = s;
         cfg.attrs = attr;
         cfg.numAttrs = blocks > 1 ? 1 : 0;
-        const cudaError_t e = cudaLaunchKernelEx(&cfg, route_one_cluster_kernel<T, K>, x, ld, num_experts, (int)batch, per,
-                                                 all, expert, weight, row, column, offset);
+        auto kern = batch <= kGrouped ? route_one_cluster_kernel<T, K, kGroup> : route_one_cluster_kernel<T, K, 1>;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, x, ld, num_experts, (int)batch, per, all, expert, weight, row,
+                                                 column, offset);
         return e == cudaSuccess ? PONNI_B200_OK : ops::fail_cuda(e, "route_columns");
       }
-      const int64_t tiles = (batch + kBlock - 1) / kBlock, most = blocks_of(batch);
-      const int64_t per_block = (tiles + most - 1) / most * kBlock;
-      const int blocks = (int)((batch + per_block - 1) / per_block);
+      const int64_t per_block = columns_of_block(num_experts, batch);
+      const int blocks = (int)blocks_of(num_experts, batch);
       int* counts = static_cast<int*>(workspace);
       int* totals = counts + (int64_t)num_experts * blocks;
-      choose_kernel<T, K><<<blocks, kBlock, num_experts * sizeof(int), s>>>(x, ld, num_experts, batch, per_block, all,
-                                                                           expert, weight, counts);
+      auto choose = spread(num_experts, batch) ? choose_kernel<T, K, kGroup> : choose_kernel<T, K, 1>;
+      choose<<<blocks, kBlock, num_experts * sizeof(int), s>>>(x, ld, num_experts, batch, per_block, all, expert, weight,
+                                                             counts);
       cudaError_t e = cudaGetLastError();
       if (e == cudaSuccess)
         e = ops::launch_after(scan_kernel, dim3(num_experts), dim3(kBlock), 0, s, counts, blocks, totals);
