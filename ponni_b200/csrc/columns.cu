@@ -409,7 +409,8 @@ ponni_b200_status check_columns(const char* what, int dtype, const void* columns
   using namespace ops;
   const std::string at(what);
   if (!is_real_type(dtype)) return fail(PONNI_B200_ERR_UNSUPPORTED, at + ": values must be fp32, fp16 or bf16");
-  if (!columns || !row || !rows) return fail(PONNI_B200_ERR_INVALID_ARGUMENT, at + ": pointer is NULL");
+  if (!columns || !row || !rows || !aligned_to(element_bytes(dtype), columns, rows) || !aligned_to(4, row))
+    return fail(PONNI_B200_ERR_INVALID_ARGUMENT, at + ": pointer is NULL or not aligned to its type");
   if (features < 1) return fail(PONNI_B200_ERR_INVALID_ARGUMENT, at + ": needs at least one feature");
   if (top_k < 1 || top_k > kMaxTopK) return fail(PONNI_B200_ERR_UNSUPPORTED, at + ": top_k must be 1 to 8");
   if (batch < 1 || batch > INT32_MAX / top_k)
@@ -458,7 +459,8 @@ ponni_b200_status ponni_b200_gather_columns(int dtype, const void* x, int64_t ld
   return ops::entry(device, [&]() -> ponni_b200_status {
     ponni_b200_status st = check_columns("gather_columns", dtype, x, ld, features, batch, top_k, row, rows, rows_ld);
     if (st) return st;
-    if (!num_used) return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "gather_columns: pointer is NULL");
+    if (!num_used || !ops::aligned_to(4, num_used))
+      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "gather_columns: pointer is NULL or not aligned to its type");
     return by_type(dtype, [&](auto t) -> ponni_b200_status {
       using T = decltype(t);
       const int per = kTileWords * Word<T>::n;
@@ -480,6 +482,8 @@ ponni_b200_status ponni_b200_combine_rows(int dtype, const void* rows, int64_t r
   return ops::entry(device, [&]() -> ponni_b200_status {
     ponni_b200_status st = check_columns("combine_rows", dtype, y, ld, features, batch, top_k, row, rows, rows_ld);
     if (st) return st;
+    if (!ops::aligned_to(4, weight))
+      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "combine_rows: pointer not aligned to its type");
     return by_type(dtype, [&](auto t) -> ponni_b200_status {
       using T = decltype(t);
       const int per = kTileWords * Word<T>::n;
@@ -504,8 +508,10 @@ ponni_b200_status ponni_b200_combine_rows_backward(int dtype, const void* d_y, i
     ponni_b200_status st =
         check_columns("combine_rows_backward", dtype, d_y, ld, features, batch, top_k, row, rows, rows_ld);
     if (st) return st;
-    if (!weight || !num_used || !d_rows || !d_weight)
-      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "combine_rows_backward: pointer is NULL");
+    if (!weight || !num_used || !d_rows || !d_weight || !ops::aligned_to(4, weight, num_used, d_weight) ||
+        !ops::aligned_to(ops::element_bytes(dtype), d_rows))
+      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT,
+                       "combine_rows_backward: pointer is NULL or not aligned to its type");
     if (d_ld < features)
       return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "combine_rows_backward: row stride smaller than the row");
     return by_type(dtype, [&](auto t) -> ponni_b200_status {

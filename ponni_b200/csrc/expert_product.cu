@@ -1397,8 +1397,9 @@ ponni_b200_status check_product(const std::string& at, int dtype, const void* ro
     return fail(PONNI_B200_ERR_INVALID_ARGUMENT, at + ": inputs and outputs must be 1 to 2^24");
   if (num_rows < 0 || num_rows > INT32_MAX - 65536)
     return fail(PONNI_B200_ERR_INVALID_ARGUMENT, at + ": the number of rows must be below 2^31 - 65536");
-  if ((num_rows > 0 && !rows) || !weights || !offset)
-    return fail(PONNI_B200_ERR_INVALID_ARGUMENT, at + ": pointer is NULL");
+  if ((num_rows > 0 && !rows) || !weights || !offset || !aligned_to(element_bytes(dtype), rows, weights) ||
+      !aligned_to(4, offset))
+    return fail(PONNI_B200_ERR_INVALID_ARGUMENT, at + ": pointer is NULL or not aligned to its type");
   if (rows_ld < inputs || w_ld < outputs || (experts > 1 && w_stride < (int64_t)(inputs - 1) * w_ld + outputs))
     return fail(PONNI_B200_ERR_INVALID_ARGUMENT, at + ": stride smaller than the row or the expert");
   return PONNI_B200_OK;
@@ -1466,7 +1467,8 @@ ponni_b200_status ponni_b200_expert_product(int dtype, const void* rows, int64_t
     if (activation != -1 && (!is_pointwise(activation) || activation == PONNI_B200_BIAS))
       return ops::fail(PONNI_B200_ERR_UNSUPPORTED, "expert_product: the activation must be an activation layer kind");
     if (num_rows == 0) return PONNI_B200_OK;
-    if (!out) return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "expert_product: pointer is NULL");
+    if (!out || !ops::aligned_to(ops::element_bytes(dtype), out, bias) || !ops::aligned_to(256, workspace))
+      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "expert_product: pointer is NULL or not aligned");
     if (out_ld < outputs)
       return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "expert_product: stride smaller than the row");
     Args p = {};
@@ -1518,8 +1520,9 @@ ponni_b200_status ponni_b200_expert_product_backward(int dtype, const void* d_ou
     ponni_b200_status st = check_product("expert_product_backward", dtype, rows, rows_ld, num_rows, weights, w_ld,
                                          w_stride, offset, experts, inputs, outputs);
     if (st) return st;
-    if (num_rows > 0 && !d_out)
-      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "expert_product_backward: pointer is NULL");
+    if ((num_rows > 0 && !d_out) || !ops::aligned_to(ops::element_bytes(dtype), d_out, d_rows, d_weights, d_bias) ||
+        !ops::aligned_to(256, workspace))
+      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "expert_product_backward: pointer is NULL or not aligned");
     if (d_out_ld < outputs || (d_rows && d_rows_ld < inputs))
       return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "expert_product_backward: stride smaller than the row");
     const int sms = ops::num_sms(device);

@@ -326,9 +326,12 @@ ponni_b200_status ponni_b200_gradient_set_clip(ponni_b200_gradient_set* set, dou
   if (!set) return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "clip: gradient set is NULL");
   return ops::entry(set->device, [&]() -> ponni_b200_status {
     if (!(max_norm > 0.0)) return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "clip: max_norm must be positive");
-    if (!norm) return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "clip: norm pointer is NULL");
+    if (!norm || !ops::aligned_to(4, norm))
+      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "clip: norm pointer is NULL or not aligned to 4 bytes");
     if (flat && (flat_dtype < PONNI_B200_F32 || flat_dtype > PONNI_B200_BF16))
       return ops::fail(PONNI_B200_ERR_UNSUPPORTED, "clip: the packed vector must be fp32, fp64, fp16 or bf16");
+    if (flat && !ops::aligned_to(ops::element_bytes(flat_dtype), flat))
+      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "clip: the packed vector is not aligned to its type");
     if (!workspace || workspace_bytes < ponni_b200_gradient_set_workspace(set) ||
         reinterpret_cast<uintptr_t>(workspace) % 8 != 0)
       return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "clip: workspace is too small or not aligned to 8 bytes");

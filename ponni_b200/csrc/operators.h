@@ -58,6 +58,14 @@ ponni_b200_status entry(int device, F&& body) noexcept {
 inline bool is_real_type(int dtype) {
   return dtype == PONNI_B200_F32 || dtype == PONNI_B200_F16 || dtype == PONNI_B200_BF16;
 }
+// Every pointer a multiple of `bytes` (a misaligned one would fault in the kernels).
+template <class... P>
+bool aligned_to(int bytes, P... p) {
+  uintptr_t all = 0;
+  ((all |= reinterpret_cast<uintptr_t>(p)), ...);
+  return all % bytes == 0;
+}
+
 inline int element_bytes(int dtype) { return dtype == PONNI_B200_F64 ? 8 : dtype == PONNI_B200_F32 ? 4 : 2; }
 
 // Launch with programmatic stream serialisation: the kernel may start while its

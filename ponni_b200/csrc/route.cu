@@ -401,6 +401,7 @@ __global__ void __launch_bounds__(kBlock)
 #pragma unroll
   for (int j = 0; j < K; ++j) {
     idx[j] = expert[j * batch + b];
+    if (idx[j] >= experts) idx[j] = -1;
     w[j] = weight[j * batch + b];
     g[j] = idx[j] >= 0 ? w[j] * d_weight[j * batch + b] : 0.0f;
     mean += g[j];
@@ -466,7 +467,8 @@ ponni_b200_status check_route(int dtype, const void* logits, int64_t ld, int exp
                               int normalise) {
   using namespace ops;
   if (!is_real_type(dtype)) return fail(PONNI_B200_ERR_UNSUPPORTED, "route: logits must be fp32, fp16 or bf16");
-  if (!logits) return fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route: logits pointer is NULL");
+  if (!logits || !aligned_to(element_bytes(dtype), logits))
+    return fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route: logits pointer is NULL or not aligned to its type");
   if (experts < 1 || experts > kMaxExperts)
     return fail(PONNI_B200_ERR_UNSUPPORTED, "route: the number of experts must be 1 to 1024");
   if (top_k < 1 || top_k > kMaxTopK || top_k > experts)
@@ -498,8 +500,9 @@ ponni_b200_status ponni_b200_route_columns(int dtype, const void* logits, int64_
   return ops::entry(device, [&]() -> ponni_b200_status {
     ponni_b200_status st = check_route(dtype, logits, ld, num_experts, top_k, batch, normalise);
     if (st) return st;
-    if (!expert || !weight || !row || !column || !offset)
-      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route: output pointer is NULL");
+    if (!expert || !weight || !row || !column || !offset ||
+        !ops::aligned_to(4, expert, weight, row, column, offset, workspace))
+      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route: output pointer is NULL or not aligned to 4 bytes");
     const int64_t need = ponni_b200_route_workspace(num_experts, batch);
     if (need && (!workspace || workspace_bytes < need))
       return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route: workspace is too small");
@@ -556,8 +559,9 @@ ponni_b200_status ponni_b200_route_columns_backward(int dtype, const void* logit
   return ops::entry(device, [&]() -> ponni_b200_status {
     ponni_b200_status st = check_route(dtype, logits, ld, num_experts, top_k, batch, normalise);
     if (st) return st;
-    if (!expert || !weight || !d_weight || !d_logits)
-      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route backward: pointer is NULL");
+    if (!expert || !weight || !d_weight || !d_logits || !ops::aligned_to(4, expert, weight, d_weight) ||
+        !ops::aligned_to(ops::element_bytes(dtype), d_logits))
+      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route backward: pointer is NULL or not aligned to its type");
     if (d_ld < batch)
       return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "route backward: row stride smaller than the batch size");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
