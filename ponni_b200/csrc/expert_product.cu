@@ -76,6 +76,7 @@ struct Args {
   int unit_rows;  // kWeights: rows of a unit (a multiple of kBK); 0: a group is one unit
   int vec;        // c may be written 16 bytes at a time
   int bulk;       // and by the copy engine (map_c)
+  int boxes;      // of output staging a warp
   int stages;
   int device;
   int* error;
@@ -95,12 +96,19 @@ template <int P, int BN, int CG> struct Shape {
   static constexpr int parts = BN >= 128 ? 4 : 2;
   static constexpr int groups = 4 / parts;  // of warps, which take tiles in turn
   static constexpr int part_cols = BN / parts;
-  // Output staging of a warp: two boxes of 32 rows x 64 bytes for the copy engine
+  // Output staging of a warp: boxes of 32 rows x 64 bytes for the copy engine
   // (16-bit operands in pairs or 64 wide), else its rows of 32 bytes: the boxes cost
   // the single 128-wide tiles stages, and with them 10% on weight-bound products.
   static constexpr bool bulk_store = P == 1 && (CG == 2 || BN == 64);
-  static constexpr int epi_bytes = bulk_store ? kEpiWarps * 4096 : kEpiBytes;
 };
+
+// Staging bytes.  Products of up to 8 K blocks, which store a tile after little else,
+// get two boxes a warp (256 -> 128: 131 us against 142 with one); longer ones
+// one box and a stage more (64 us against 61 for 16384 rows, 1024 -> 2048).
+template <class S>
+__host__ __device__ constexpr int epi_bytes(int boxes) {
+  return S::bulk_store ? kEpiWarps * 2048 * boxes : kEpiBytes;
+}
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile(
@@ -394,8 +402,9 @@ __global__ void __launch_bounds__(kBlock, 1)
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   unsigned char* base_ptr = smem_raw + (base - raw);
   unsigned char* epi = base_ptr + p.stages * S::stage_bytes;
-  float* bias_s = reinterpret_cast<float*>(epi + S::epi_bytes);
-  int* lo = reinterpret_cast<int*>(epi + S::epi_bytes + kBiasBytes);
+  const int epi_total = epi_bytes<S>(p.boxes);
+  float* bias_s = reinterpret_cast<float*>(epi + epi_total);
+  int* lo = reinterpret_cast<int*>(epi + epi_total + kBiasBytes);
   int* hi = lo + p.experts;
   const uint32_t bar0 = smem_u32(bars);
   auto full = [&](int s) { return bar0 + 8u * s; };
@@ -610,8 +619,8 @@ __global__ void __launch_bounds__(kBlock, 1)
     const int group = ((warp - 2) >> 2) / S::parts;
     int turn = 0;
     constexpr int kChunks = S::part_cols / 32;
-    unsigned char* stage = epi + w * (S::epi_bytes / kEpiWarps);
-    int box = 0;  // of the two store boxes
+    unsigned char* stage = epi + w * (epi_total / kEpiWarps);
+    int box = 0;  // of the store boxes
     float* bias_w = bias_s + w * 64;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const int n_end = MODE == kRows ? p.inputs : p.outputs;
@@ -692,7 +701,10 @@ __global__ void __launch_bounds__(kBlock, 1)
         if constexpr (S::bulk_store) {
           if (p.bulk && (MODE == kWeights || m_valid == 32)) {  // (rows past the weights' end are clipped)
             // 64-byte rows, 16-byte chunks swizzled by row / 2 as the tensor map has it.
-            if (lane == 0) tma_store_wait_read<1>();
+            if (lane == 0) {
+              if (p.boxes == 2) tma_store_wait_read<1>();
+              else tma_store_wait_read<0>();
+            }
             __syncwarp();
             const uint32_t dst = smem_u32(stage) + (uint32_t)box * 2048;
 #pragma unroll
@@ -706,7 +718,7 @@ __global__ void __launch_bounds__(kBlock, 1)
               if (MODE == kWeights) tma_store_3d(&map_c, n, row0, v.e, dst);
               else tma_store_3d(&map_c, n, v.lo + row0, 0, dst);
             }
-            box ^= 1;
+            box ^= p.boxes - 1;
             return;
           }
           if (lane == 0) tma_store_wait_read<0>();
@@ -1268,9 +1280,12 @@ ponni_b200_status launch_shape(const Operand& a, const Operand& b, Args p, int s
     st = make_map(map_c, c, half, 32, 32);
   }
   if (st) return st;
-  const int fixed = 1024 + S::epi_bytes + kBiasBytes + 2 * p.experts * (int)sizeof(int) + 512;
+  const int k = MODE == kForward ? p.inputs : p.outputs;
+  p.boxes = MODE != kWeights && k <= 8 * kBK ? 2 : 1;
+  const int epi = epi_bytes<S>(p.boxes);
+  const int fixed = 1024 + epi + kBiasBytes + 2 * p.experts * (int)sizeof(int) + 512;
   p.stages = std::min(kMaxStages, (kSmemLimit - fixed) / S::stage_bytes);
-  const int smem = 1024 + p.stages * S::stage_bytes + S::epi_bytes + kBiasBytes + 2 * p.experts * (int)sizeof(int);
+  const int smem = 1024 + p.stages * S::stage_bytes + epi + kBiasBytes + 2 * p.experts * (int)sizeof(int);
   auto kern = product_kernel<T, MODE, P, BN, CG>;
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = ops::allow_smem(reinterpret_cast<const void*>(kern), kSmemLimit - 1024, p.device, allowed);
