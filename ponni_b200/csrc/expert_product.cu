@@ -1224,19 +1224,59 @@ int64_t staged_bytes(int dtype, int64_t rows, int cols) {
   return pad256(rows * pad8(cols) * (dtype == PONNI_B200_F32 ? 6 : 2));
 }
 
+// Tile width.  An MMA of 128 x 64 takes as long as one of 128 x 128 (58 and 64
+// cycles for 16 k), so 64 is for products of at most 64 columns; 256 halves the
+// reads of the row tile against 128 and is taken unless its padding costs over
+// an eighth more columns, or the rows are so few that the weights' traffic
+// decides (at most half a tile of rows a group): 128 then spreads them more evenly
+// over the SMs.
+int tile_width(int n, int64_t rows, int experts, bool weights) {
+  if (n <= 64) return 64;
+  if (n <= 128 || (!weights && rows <= (int64_t)64 * experts)) return 128;
+  auto padded = [&](int w) { return (int64_t)(n + w - 1) / w * w; };
+  return padded(256) * 8 > padded(128) * 9 ? 128 : 256;
+}
+
+// Whether two CTAs share a tile of 256 rows: half the weight traffic, but more
+// rows of padding at the end of a group.  16-bit rows x 1024 x 1024, 16 experts:
+// 23.1 us against 22.2 in pairs with 256 rows each, 24.3 / 28.4 with 512, 39.7 / 36.6
+// with 1024, 128.5 / 117.2 with 4096; the weight gradient has no such padding (31.1 /
+// 28.8 with 512).  fp32 spends its time on the parts' traffic and the sums of every K
+// block: 969.8 / 1060 with 4096 rows each, 4245 / 4170 with 16384.
+bool use_pairs(int64_t rows, int experts, int mode, bool parts) {
+  const int64_t least = parts ? 8192 : mode == kWeights ? 256 : 768;
+  return rows >= least * experts;
+}
+
+struct TileShape {
+  int columns, ctas;  // of a tile; its rows are 128 a CTA
+};
+TileShape tile_shape(int dtype, int mode, int64_t rows, int experts, int inputs, int outputs) {
+  const bool parts = dtype == PONNI_B200_F32;
+  TileShape t = {tile_width(mode == kRows ? inputs : outputs, rows, experts, mode == kWeights), 1};
+  if (t.columns > 64 && use_pairs(rows, experts, mode, parts)) t.ctas = 2;
+  if (parts && t.ctas == 1) t.columns = std::min(t.columns, 128);
+  return t;
+}
+
 // Rows of a unit of d_W: whole groups where their tiles fill the SMs twice or the
-// groups are short (2048 rows on average: a split costs another launch, 9.5 us
-// against 19 for 16 experts of 256 x 256 with 64 and 128 rows each); else units small
-// enough for about four tiles an SM (the tail of uneven groups), 1024 rows at least
-// (a unit's partial sums cost 8 bytes an element of W_e).
-int unit_rows_of(int64_t rows, int experts, int inputs, int outputs, int sms) {
-  const int64_t per = (int64_t)((inputs + kBM - 1) / kBM) * ((outputs + 255) / 256);
-  if (per * experts >= 2 * sms || rows <= (int64_t)2048 * experts) return 0;
-  const int64_t unit = std::max<int64_t>(1024, (rows * per / (4 * sms) + kBK - 1) / kBK * kBK);
+// groups are short (2048 rows on average, 512 of fp32: a split costs another
+// launch, 9.5 us against 19 for 16 experts of 256 x 256 with 64 and 128 rows each);
+// else so many that the tiles make about three waves (two leave the SMs a third
+// idle where the last is ragged, more waves cost partial sums, 8 bytes an element of
+// W_e and unit): 1024 rows at least, 256 of fp32, whose K blocks take four times as long.
+int unit_rows_of(int dtype, int64_t rows, int experts, int inputs, int outputs, int sms) {
+  const bool parts = dtype == PONNI_B200_F32;
+  const TileShape t = tile_shape(dtype, kWeights, rows, experts, inputs, outputs);
+  const int64_t m = t.ctas * kBM;
+  const int64_t per = ((inputs + m - 1) / m) * ((outputs + t.columns - 1) / t.columns), slots = sms / t.ctas;
+  if (per * experts >= 2 * slots || rows <= (int64_t)(parts ? 512 : 2048) * experts) return 0;
+  const int64_t units = std::max<int64_t>(1, 3 * slots / per - experts / 2);  // a group's last unit is half full
+  const int64_t unit = std::max<int64_t>(parts ? 256 : 1024, ((rows + units - 1) / units + kBK - 1) / kBK * kBK);
   return unit < rows ? (int)std::min<int64_t>(unit, 1 << 30) : 0;
 }
-int64_t partial_bytes(int64_t rows, int experts, int inputs, int outputs, int sms) {
-  const int unit = unit_rows_of(rows, experts, inputs, outputs, sms);
+int64_t partial_bytes(int dtype, int64_t rows, int experts, int inputs, int outputs, int sms) {
+  const int unit = unit_rows_of(dtype, rows, experts, inputs, outputs, sms);
   return unit ? pad256((rows / unit + experts) * (int64_t)inputs * outputs * 4) : 0;
 }
 
@@ -1308,37 +1348,12 @@ ponni_b200_status launch_shape(const Operand& a, const Operand& b, Args p, int s
   return e == cudaSuccess ? PONNI_B200_OK : ops::fail_cuda(e, "expert_product");
 }
 
-// Tile width.  An MMA of 128 x 64 takes as long as one of 128 x 128 (58 and 64
-// cycles for 16 k), so 64 is for products of at most 64 columns; 256 halves the
-// reads of the row tile against 128 and is taken unless its padding costs over
-// an eighth more columns, or the rows are so few that the weights' traffic
-// decides (at most half a tile of rows a group): 128 then spreads them more evenly
-// over the SMs.
-int tile_width(int n, int64_t rows, int experts, bool weights) {
-  if (n <= 64) return 64;
-  if (n <= 128 || (!weights && rows <= (int64_t)64 * experts)) return 128;
-  auto padded = [&](int w) { return (int64_t)(n + w - 1) / w * w; };
-  return padded(256) * 8 > padded(128) * 9 ? 128 : 256;
-}
-
-// Whether two CTAs share a tile of 256 rows: half the weight traffic, but more
-// rows of padding at the end of a group.  16-bit rows x 1024 x 1024, 16 experts:
-// 23.1 us against 22.2 in pairs with 256 rows each, 24.3 / 28.4 with 512, 39.7 / 36.6
-// with 1024, 128.5 / 117.2 with 4096; the weight gradient has no such padding (31.1 /
-// 28.8 with 512).  fp32 spends its time on the parts' traffic and the sums of every K
-// block: 969.8 / 1060 with 4096 rows each, 4245 / 4170 with 16384.
-bool use_pairs(const Args& p, int mode, bool split_parts) {
-  const int64_t least = split_parts ? 8192 : mode == kWeights ? 256 : 768;
-  return p.rows >= least * p.experts;
-}
-
 template <class T, int MODE>
 ponni_b200_status launch_product(const Operand& a, const Operand& b, const Args& p, int sms, cudaStream_t stream) {
   constexpr int P = sizeof(T) == 4 ? 3 : 1;
   const int n = MODE == kRows ? p.inputs : p.outputs;
-  int w = tile_width(n, p.rows, p.experts, MODE == kWeights);
-  const int cg = w > 64 && use_pairs(p, MODE, P == 3) ? 2 : 1, m = cg * kBM;
-  if (P == 3 && cg == 1) w = std::min(w, 128);
+  const TileShape shape = tile_shape(P == 3 ? PONNI_B200_F32 : PONNI_B200_BF16, MODE, p.rows, p.experts, p.inputs, p.outputs);
+  const int w = shape.columns, cg = shape.ctas, m = cg * kBM;
   const int64_t m_tiles = MODE == kWeights
                               ? (int64_t)((p.inputs + m - 1) / m) * (p.experts + (p.unit_rows ? p.rows / p.unit_rows : 0))
                               : p.rows / m + std::min<int64_t>(p.experts, p.rows);
@@ -1464,7 +1479,7 @@ int64_t ponni_b200_expert_product_workspace(int dtype, int64_t num_rows, int exp
     if (backward) n += staged_bytes(dtype, num_rows, outputs);
   }
   if (backward)
-    n += partial_bytes(num_rows, experts, inputs, outputs, ops::num_sms(device)) +
+    n += partial_bytes(dtype, num_rows, experts, inputs, outputs, ops::num_sms(device)) +
          bias_bytes(num_rows, experts, outputs, ops::num_sms(device));
   return n;
 }
@@ -1557,10 +1572,10 @@ ponni_b200_status ponni_b200_expert_product_backward(int dtype, const void* d_ou
     if (d_rows || d_weights) st = operand(d, stages, space, dtype, d_out, d_out_ld, 0, num_rows, outputs, 1);
     if (!st && d_rows) st = operand(w, stages, space, dtype, weights, w_ld, w_stride, inputs, outputs, experts);
     if (!st && d_weights) st = operand(x, stages, space, dtype, rows, rows_ld, 0, num_rows, inputs, 1);
-    const int unit = unit_rows_of(num_rows, experts, inputs, outputs, sms);
+    const int unit = unit_rows_of(dtype, num_rows, experts, inputs, outputs, sms);
     void* partial = nullptr;
     if (!st && d_weights && unit) {
-      partial = space.take(partial_bytes(num_rows, experts, inputs, outputs, sms));
+      partial = space.take(partial_bytes(dtype, num_rows, experts, inputs, outputs, sms));
       if (!partial) st = ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "expert_product_backward: workspace is too small");
     }
     const int parts = bias_parts(num_rows, experts, outputs, sms);
