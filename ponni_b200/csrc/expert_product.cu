@@ -1120,6 +1120,7 @@ struct Stage {
   void* dst;
   int64_t rows, ld, group_rows, group_stride;  // source row r: (r / group_rows) * group_stride + (r % group_rows) * ld
   int cols, pitch;
+  int vec;  // the source's rows start on 16-byte boundaries
 };
 struct Stages {
   Stage s[3];
@@ -1152,9 +1153,15 @@ __global__ void __launch_bounds__(256) stage_kernel(const Stages all) {
     const T* src = static_cast<const T*>(s.src) +
                    (s.group_rows == s.rows ? r * s.ld : r / s.group_rows * s.group_stride + r % s.group_rows * s.ld);
     for (int c = x; c < vecs; c += tx) {
-      T v[8];
+      alignas(16) T v[8];
+      if (s.vec && c * 8 + 8 <= s.cols) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = c * 8 + i < s.cols ? __ldg(src + c * 8 + i) : Num<T>::from_c(0.0f);
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+          reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(src + c * 8) + i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c * 8 + i < s.cols ? __ldg(src + c * 8 + i) : Num<T>::from_c(0.0f);
+      }
       if constexpr (sizeof(T) == 4) {
         uint32_t h[3][8];
 #pragma unroll
@@ -1165,10 +1172,7 @@ __global__ void __launch_bounds__(256) stage_kernel(const Stages all) {
           *reinterpret_cast<uint4*>(dst + q * plane) = make_uint4(pack_hi16(h[q][0], h[q][1]), pack_hi16(h[q][2], h[q][3]),
                                                                   pack_hi16(h[q][4], h[q][5]), pack_hi16(h[q][6], h[q][7]));
       } else {
-        alignas(16) T o[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = v[i];
-        *reinterpret_cast<uint4*>(static_cast<T*>(s.dst) + r * s.pitch + c * 8) = *reinterpret_cast<uint4*>(o);
+        *reinterpret_cast<uint4*>(static_cast<T*>(s.dst) + r * s.pitch + c * 8) = *reinterpret_cast<uint4*>(v);
       }
     }
   }
@@ -1447,7 +1451,9 @@ ponni_b200_status operand(Operand& o, Stages& stages, Space& space, int dtype, c
   void* dst = space.take(staged_bytes(dtype, rows * depth, cols));
   if (!dst) return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "expert_product: workspace is too small");
   o = {dst, pitch, rows * pitch, cols, rows, depth * planes};
-  stages.s[stages.n++] = {p, dst, rows * depth, ld, rows, stride, cols, (int)pitch};
+  const int64_t z = ops::element_bytes(dtype);
+  const bool vec = reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * z % 16 == 0 && (depth == 1 || stride * z % 16 == 0);
+  stages.s[stages.n++] = {p, dst, rows * depth, ld, rows, stride, cols, (int)pitch, vec};
   return PONNI_B200_OK;
 }
 
