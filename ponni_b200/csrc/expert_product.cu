@@ -24,7 +24,10 @@
 // block of 64 goes into its own TMEM accumulator, the five small products first,
 // and is added to the tile's sum in fp32 registers: the tensor core truncates
 // when it accumulates, so long sums in TMEM would drift by a part of 2^-24 for
-// every step.
+// every step.  These products are bound by shared memory: a block's 24 MMAs of
+// 128 x 128 x 16 read 192 KB and its copies write 96 KB, 2250 cycles at 128 bytes a
+// cycle against 1536 of the tensor cores.  (K blocks of 32 and twice the stages are
+// 10% slower.)
 //
 // One persistent CTA per SM: a TMA producer, an MMA warp and sixteen epilogue
 // warps.  Every role walks the same tile sequence, which it derives from the
