@@ -338,13 +338,13 @@ ponni_b200_status ponni_b200_fill_synthetic(ponni_b200_dtype dtype, void* device
  *
  * All pointers are device memory; the calls are asynchronous on `stream` (a
  * cudaStream_t; NULL is the legacy default stream), allocate nothing (the
- * creation of a gradient set excepted), may be captured, and restore the
- * caller's current device.  `dtype` is a ponni_b200_dtype.  A workspace is
- * caller-owned scratch of at least the bytes that the matching _workspace
- * function returns, aligned to 256 bytes (a route workspace to 4, a clip workspace
- * to 8), in use until the call's kernels end.  Buffers of one call must not
- * overlap.  The text of the calling thread's last operator error is
- * ponni_b200_operator_error(). */
+ * creation of a gradient set excepted), may be captured (after a first call of
+ * the kind, which loads its kernel), and restore the caller's current device.
+ * `dtype` is a ponni_b200_dtype.  A workspace is caller-owned scratch of at least
+ * the bytes that the matching _workspace function returns, aligned to 256 bytes (a
+ * route workspace to 4, a clip workspace to 8), in use until the call's kernels
+ * end.  Buffers of one call must not overlap.  The text of the calling thread's
+ * last operator error is ponni_b200_operator_error(). */
 const char* ponni_b200_operator_error(void);
 /* Waits for `stream` and reports what the operators' kernels found on the
  * device since the last check: PONNI_B200_ERR_DEVICE (a bounded wait gave up),
@@ -401,7 +401,9 @@ ponni_b200_status ponni_b200_combine_rows_backward(int dtype, const void* d_y, i
 /* out[r] = activation(rows[r] weights[e] + bias[e]) for r in [offset[e],
  * offset[e + 1]); rows in no group give zero.  weights[e] is [inputs, outputs]
  * as in Matvec (row stride w_ld, expert stride w_stride elements), bias
- * [experts, outputs] or NULL; one type, fp32 / fp16 / bf16, sums in fp32.
+ * [experts, outputs] or NULL; one type, fp32 / fp16 / bf16, sums in fp32.  An
+ * infinite fp32 operand gives what plain arithmetic gives in sums of up to 65536
+ * terms, NaN in longer ones.
  * `activation` is the ponni_b200_layer_kind of an activation (PONNI_B200_RELU to
  * PONNI_B200_MISH) with its flags and scalars, or -1.  The workspace holds copies
  * of operands that the copy engine cannot read in place: fp32 ones, and 16-bit

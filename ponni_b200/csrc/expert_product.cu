@@ -129,8 +129,9 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
 }
-// Arrival on another CTA's barrier of what this thread has read or written in
-// tensor memory or shared memory (ordered by the tcgen05 and proxy fences before it).
+// Arrival on another CTA's barrier after reading tensor memory, which the tcgen05
+// fence before it orders: no release of this thread's stores, which would cost
+// half a microsecond each.
 __device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_addr) : "memory");
 }
@@ -222,7 +223,9 @@ template <int MODE, int BN, int CG> struct Tiles {
 
 // The sum of one output element straight from the fp32 operands: taken where the
 // split parts gave NaN, because an infinite value times another's zero part is
-// NaN where the plain product is infinite.
+// NaN where the plain product is infinite.  Sums of more than kPlainTerms terms
+// stay NaN: a tile of them would outlast the other roles' bounded waits.
+constexpr int kPlainTerms = 65536;
 template <int MODE>
 __device__ __noinline__ float plain_sum(const Args& p, int e, int lo, int hi, int m, int n) {
   const float* a = static_cast<const float*>(p.a);
@@ -556,7 +559,7 @@ __global__ void __launch_bounds__(kBlock, 1)
             if (!ok) break;
             tail_ph ^= 1u << s;
             clear_tail(kb);
-            if (lane == 0) arrive_remote(mapa_shared(peer_full(s), 0));
+            if (lane == 0) mbar_arrive_cluster(mapa_shared(peer_full(s), 0));  // releases the cleared rows
           }
           next_stage();
         }
@@ -679,7 +682,8 @@ __global__ void __launch_bounds__(kBlock, 1)
           bool nan = false;
 #pragma unroll
           for (int i = 0; i < 32; ++i) nan |= x[i] != x[i];
-          if (nan) {
+          const int terms = MODE == kForward ? p.inputs : MODE == kRows ? p.outputs : v.hi - v.lo;
+          if (nan && terms <= kPlainTerms) {
             float y[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) y[i] = x[i];

@@ -33,8 +33,7 @@ ponni_b200_status launched(const char* what) {
   return e == cudaSuccess ? PONNI_B200_OK : fail_cuda(e, what);
 }
 
-// The word is a static device variable, so that the first call allocates
-// nothing and may be made while a stream is captured.
+// A static device variable: the first call on a device allocates nothing.
 static __device__ int g_error_word;
 
 int* error_word(int device) {

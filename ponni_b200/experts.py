@@ -430,5 +430,7 @@ def clip_gradients(tensors, max_norm: float, out=None):
 def check_operators(device=None) -> None:
     """Waits for the current stream; raises PonniError if an operator found group offsets out of order or gave up."""
     torch = _torch()
-    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    dev = torch.device("cuda" if device is None else device)
+    if dev.index is None:
+        dev = torch.device("cuda", torch.cuda.current_device())
     _call(_abi.lib().ponni_b200_operator_check(dev.index, torch_stream_handle(dev)))
