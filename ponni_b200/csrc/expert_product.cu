@@ -97,7 +97,10 @@ template <int P, int BN, int CG> struct Shape {
   // Epilogue warps: four lane quarters (a warp reads the TMEM lanes of its
   // number modulo 4) times `parts` strips of columns.
   static constexpr int parts = BN >= 128 ? 4 : 2;
-  static constexpr int groups = 4 / parts;  // of warps, which take tiles in turn
+  // Groups of warps, which take tiles in turn.  Only where a tile is one accumulator
+  // (16-bit operands): a group may wait for a barrier's next phase, not for one further on.
+  static constexpr int groups = 4 / parts;
+  static_assert(groups == 1 || P == 1, "tiles of several accumulators are not taken in turn");
   static constexpr int part_cols = BN / parts;
   // Output staging of a warp: boxes of 32 rows x 64 bytes for the copy engine
   // (16-bit operands in pairs or 64 wide), else its rows of 32 bytes: the boxes cost
@@ -657,7 +660,7 @@ __global__ void __launch_bounds__(kBlock, 1)
     };
     while (ok && tiles.next(v)) {
       if (S::groups > 1 && turn++ % S::groups != group) {  // another group's tile
-        for (int i = 0; i < (P == 3 ? v.k_blocks : min(1, v.k_blocks)); ++i) next_acc();
+        if (v.k_blocks > 0) next_acc();
         continue;
       }
       const int m_end = MODE == kWeights ? p.inputs : v.hi - v.lo;
@@ -1266,7 +1269,7 @@ TileShape tile_shape(int dtype, int mode, int64_t rows, int experts, int inputs,
   const bool parts = dtype == PONNI_B200_F32;
   TileShape t = {tile_width(mode == kRows ? inputs : outputs, rows, experts, mode == kWeights), 1};
   if (t.columns > 64 && use_pairs(rows, experts, mode, parts)) t.ctas = 2;
-  if (parts && t.ctas == 1) t.columns = std::min(t.columns, 128);
+  if (parts && t.ctas == 1) t.columns = 128;
   return t;
 }
 
@@ -1369,7 +1372,9 @@ ponni_b200_status launch_product(const Operand& a, const Operand& b, const Args&
                               ? (int64_t)((p.inputs + m - 1) / m) * (p.experts + (p.unit_rows ? p.rows / p.unit_rows : 0))
                               : p.rows / m + std::min<int64_t>(p.experts, p.rows);
   const int64_t tiles = m_tiles * ((n + w - 1) / w);
-  if (w == 64) return launch_shape<T, MODE, P, 64, 1>(a, b, p, sms, tiles, stream);
+  if constexpr (P == 1) {
+    if (w == 64) return launch_shape<T, MODE, P, 64, 1>(a, b, p, sms, tiles, stream);
+  }
   if (w == 128)
     return cg == 2 ? launch_shape<T, MODE, P, 128, 2>(a, b, p, sms, tiles, stream)
                    : launch_shape<T, MODE, P, 128, 1>(a, b, p, sms, tiles, stream);

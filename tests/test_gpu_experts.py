@@ -251,6 +251,39 @@ def test_product(groups, inputs, outputs, dt):
     pb.check_operators()
 
 
+@pytest.mark.parametrize("inputs,outputs", [(200, 24), (24, 200), (40, 40), (1200, 37), (128, 128), (72, 300)])
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_product_many_tiles_a_cta(inputs, outputs, dt):
+    """Several tiles for every CTA, of widths that the tile shapes divide and do not."""
+    g = gen(inputs + outputs)
+    dtype = DT[dt]
+    counts = [30_011, 0, 17_000, 129, 40_100]
+    n, off = sum(counts), offsets(counts)
+    rows, w = randn(g, n, inputs, dtype=dtype), randn(g, 5, inputs, outputs, dtype=dtype) * inputs ** -0.5
+    b, d = randn(g, 5, outputs, dtype=dtype), randn(g, n, outputs, dtype=dtype)
+    want, size = R.product(rows, w, off, b)
+    R.check_sum(pb.expert_product(rows, w, off, bias=b), want, size, inputs + 1, "forward")
+    ref = R.product_gradient(d, rows, w, off)
+    for got, (want, size), terms in zip(pb.expert_product_backward(d, rows, w, off), ref, (outputs, max(counts), max(counts))):
+        R.check_sum(got, want, size, terms, "gradient")
+    pb.check_operators()
+
+
+@pytest.mark.parametrize("counts", [[1, 2, 3, 5, 9, 16, 17, 0], [0, 33, 0], [8]])
+@pytest.mark.parametrize("inputs,outputs", [(2500, 130), (1024, 128), (1027, 5), (130, 1000)])
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_product_few_rows(inputs, outputs, counts, dt):
+    """A few rows of many inputs: sums split over K and over the blocks of a cluster."""
+    g = gen(inputs)
+    dtype = DT[dt]
+    e, n, off = len(counts), sum(counts) + 1, offsets(counts)
+    rows, w = randn(g, n, inputs, dtype=dtype), randn(g, e, inputs, outputs, dtype=dtype) * inputs ** -0.5
+    b = randn(g, e, outputs, dtype=dtype)
+    want, size = R.product(rows, w, off, b)
+    R.check_sum(pb.expert_product(rows, w, off, bias=b), want, size, inputs + 1)
+    pb.check_operators()
+
+
 @pytest.mark.parametrize("layer", [pb.Relu, pb.LeakyRelu, pb.Elu, pb.Selu, pb.Gelu, pb.Silu, pb.Sigmoid, pb.Tanh,
                                    pb.Softplus, pb.HardSigmoid, pb.HardSwish, pb.Mish])
 @pytest.mark.parametrize("counts", [[3, 0, 2], [200, 90, 300]])
