@@ -297,7 +297,8 @@ __device__ __noinline__ float4 activate4(float4 v, int kind, int flags, float s0
 // SiLU and exact GELU of 32 values whose results are rounded to 16 bits.  The
 // special-function unit bounds the epilogue of narrow products (256 -> 256: two of
 // its operations a value would take 139 of the 256 us measured with them), so two
-// values share one reciprocal: 1/a = b (1/ab).  The arguments are kept where ab is
+// values share one reciprocal: 1/a = b (1/ab) (213 us; 219 with two reciprocals,
+// 226 with half of the exponentials by polynomial).  The arguments are kept where ab is
 // finite, which also keeps a NaN from its neighbour.
 __device__ __forceinline__ void fast_silu32(float (&v)[32]) {
 #pragma unroll
