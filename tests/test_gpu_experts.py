@@ -487,6 +487,12 @@ def test_clip(sizes, dts):
         assert ((a.double() - want).abs() <= (ulp[a.dtype] + 2.0 ** -22) * want.abs() + 2.0 ** -25).all()
 
 
+def test_clip_of_nothing():
+    s = pb.GradientSet([torch.empty(0, device="cuda"), torch.empty(0, device="cuda", dtype=torch.float16)])
+    assert s.clip(1.0).item() == 0.0
+    assert s.clip(1.0, out=torch.empty(0, device="cuda")).item() == 0.0
+
+
 def test_clip_unaligned_and_functional():
     g = gen(2)
     base = randn(g, 5000)
