@@ -9,7 +9,9 @@
 // (the read comes from L2 where the set fits it: the second pass goes through
 // the chunks in reverse).  The tensors are cut into chunks once, when the set
 // is made; a block sums its chunks in a fixed order and the partial sums are
-// added in a fixed order, so the norm does not change from run to run.
+// added in a fixed order, so the norm does not change from run to run.  Measured:
+// 150 M values in 200 tensors, bf16 and fp32, 64 us for the norm (450 MB, 7.0 TB/s)
+// and 188 us to pack them into fp32 (1.05 GB, 5.6 TB/s).
 // Squares are summed in fp32 over one vector and in fp64 from there: a sum of
 // 2^30 squares keeps fp32's full precision, and the fp32 part is redone in
 // fp64 where it over- or underflows.
