@@ -48,6 +48,7 @@
 #include <type_traits>
 
 #include "device_math.cuh"
+#include "expert_tiles.h"
 #include "operators.h"
 #include "tc_common.cuh"
 
@@ -57,9 +58,8 @@ namespace ponni_b200 {
 namespace {
 using namespace tc;
 
-enum Mode { kForward, kRows, kWeights };
+using namespace grouped;
 
-constexpr int kBM = 128, kBK = 64;
 constexpr int kEpiWarps = 16;
 constexpr int kBlock = 32 * (2 + kEpiWarps);
 constexpr int kEpiPitch = 48;  // bytes of a staged output row segment of 32 (+16: conflict-free)
@@ -101,10 +101,10 @@ template <int P, int BN, int CG> struct Shape {
   // Epilogue warps: four lane quarters (a warp reads the TMEM lanes of its
   // number modulo 4) times `parts` strips of columns.
   static constexpr int parts = BN >= 128 ? 4 : 2;
-  // Groups of warps, which take tiles in turn.  Only where a tile is one accumulator
-  // (16-bit operands): a group may wait for a barrier's next phase, not for one further on.
+  // Groups of warps, which take tiles by their accumulators (Turns).  Only where a tile is
+  // one accumulator (16-bit operands).
   static constexpr int groups = 4 / parts;
-  static_assert(groups == 1 || P == 1, "tiles of several accumulators are not taken in turn");
+  static_assert(groups == 1 || (P == 1 && acc_bufs % groups == 0), "an accumulator belongs to one group");
   static constexpr int part_cols = BN / parts;
   // Output staging of a warp: boxes of 32 rows x 64 bytes for the copy engine
   // (16-bit operands in pairs or 64 wide), else its rows of 32 bytes: the boxes cost
@@ -164,69 +164,6 @@ __device__ __forceinline__ void check_offsets(const int* __restrict__ offset, in
   }
 }
 __device__ __forceinline__ int clamped(int o, int lo, int64_t rows) { return (int)min(max((int64_t)o, (int64_t)lo), rows); }
-
-struct Tile {
-  int e, m0, n0;
-  int lo, hi;    // kForward, kRows: the group's rows; kWeights: the unit's
-  int k_blocks;
-  int64_t slot;  // kWeights, split: the unit's partial sums
-};
-
-// The tile sequence of this CTA (pair): its number, then every further one that
-// many CTAs (pairs) on, of all tiles: experts in order, row tiles innermost
-// (neighbours share the weight tile).  m0 is the CTA's own first row.
-template <int MODE, int BN, int CG> struct Tiles {
-  const int* lo;
-  const int* hi;
-  int experts, m_tiles, n_tiles, k_blocks, unit_rows;
-  int e = 0;
-  int64_t t, base = 0;
-
-  __device__ Tiles(const Args& p, const int* lo_, const int* hi_) : lo(lo_), hi(hi_), experts(p.experts), t(blockIdx.x / CG) {
-    const int n = MODE == kRows ? p.inputs : p.outputs, k = MODE == kForward ? p.inputs : p.outputs;
-    m_tiles = (p.inputs + CG * kBM - 1) / (CG * kBM);
-    n_tiles = (n + BN - 1) / BN;
-    k_blocks = (k + kBK - 1) / kBK;
-    unit_rows = p.unit_rows;
-  }
-  __device__ __forceinline__ int64_t count(int i) const {
-    const int rows = hi[i] - lo[i];
-    if (MODE != kWeights) return (int64_t)((rows + CG * kBM - 1) / (CG * kBM)) * n_tiles;
-    return (int64_t)(unit_rows ? (rows + unit_rows - 1) / unit_rows : 1) * m_tiles * n_tiles;
-  }
-  __device__ __forceinline__ bool next(Tile& v) {
-    int64_t c = 0;
-    while (e < experts && t >= base + (c = count(e))) {
-      base += c;
-      ++e;
-    }
-    if (e >= experts) return false;
-    int64_t local = t - base;
-    t += gridDim.x / CG;
-    v.e = e;
-    v.lo = lo[e];
-    v.hi = hi[e];
-    if (MODE != kWeights) {
-      const int m = (v.hi - v.lo + CG * kBM - 1) / (CG * kBM);
-      v.n0 = (int)(local / m) * BN;
-      v.m0 = (int)(local % m) * CG * kBM;
-      v.k_blocks = k_blocks;
-    } else {
-      const int per = m_tiles * n_tiles;
-      const int unit = (int)(local / per), i = (int)(local % per);
-      v.m0 = i % m_tiles * CG * kBM;
-      v.n0 = i / m_tiles * BN;
-      v.slot = base / per + unit;
-      if (unit_rows) {
-        v.lo += unit * unit_rows;
-        v.hi = min(v.hi, v.lo + unit_rows);
-      }
-      v.k_blocks = (v.hi - v.lo + kBK - 1) / kBK;
-    }
-    if (CG == 2) v.m0 += kBM * (int)(blockIdx.x & 1);
-    return true;
-  }
-};
 
 // The sum of one output element straight from the fp32 operands: taken where the
 // split parts gave NaN, because an infinite value times another's zero part is
@@ -463,7 +400,7 @@ __global__ void __launch_bounds__(kBlock, 1)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  Tiles<MODE, BN, CG> tiles(p, lo, hi);
+  Tiles<MODE, BN, CG> tiles({p.experts, p.inputs, p.outputs, p.unit_rows}, lo, hi, blockIdx.x / CG, gridDim.x / CG, (int)rank);
   Tile v;
   int64_t issued = 0;  // stages filled so far (thread 0)
   if (warp == 0) {
@@ -631,7 +568,7 @@ __global__ void __launch_bounds__(kBlock, 1)
     // ------------------------------------------------------- epilogue ----
     const int quarter = warp & 3, part = ((warp - 2) >> 2) % S::parts, w = warp - 2;
     const int group = ((warp - 2) >> 2) / S::parts;
-    int turn = 0;
+    Turns<S::groups> turns;
     constexpr int kChunks = S::part_cols / 32;
     unsigned char* stage = epi + w * (epi_total / kEpiWarps);
     int box = 0;  // of the store boxes
@@ -664,7 +601,7 @@ __global__ void __launch_bounds__(kBlock, 1)
       next_acc();
     };
     while (ok && tiles.next(v)) {
-      if (S::groups > 1 && turn++ % S::groups != group) {  // another group's tile
+      if (!turns.mine(group, v.k_blocks > 0, buf)) {
         if (v.k_blocks > 0) next_acc();
         continue;
       }

@@ -1,0 +1,102 @@
+// The tile sequence of the products grouped by expert (expert_product.cu), which
+// every role of the kernel derives for itself, and which epilogue warps take a
+// tile.  Plain index arithmetic, compiled for the host too (tests/cpp/test_expert_tiles.cpp).
+#pragma once
+#include <cstdint>
+
+#ifdef __CUDACC__
+#define PONNI_B200_HD __host__ __device__ __forceinline__
+#else
+#define PONNI_B200_HD inline
+#endif
+
+namespace ponni_b200 {
+namespace grouped {
+
+enum Mode { kForward, kRows, kWeights };
+
+constexpr int kBM = 128, kBK = 64;
+
+struct Tile {
+  int e, m0, n0;
+  int lo, hi;    // kForward, kRows: the group's rows; kWeights: the unit's
+  int k_blocks;
+  int64_t slot;  // kWeights, split: the unit's partial sums
+};
+
+struct Sizes {
+  int experts, inputs, outputs;
+  int unit_rows;  // kWeights: rows of a unit (a multiple of kBK); 0: a group is one unit
+};
+
+// The tile sequence of a CTA (pair): tile `first`, then every `step`-th one, of
+// all tiles: experts in order, row tiles innermost (neighbours share the weight
+// tile).  m0 is the first row of CTA `rank` of the pair.
+template <int MODE, int BN, int CG> struct Tiles {
+  const int* lo;
+  const int* hi;
+  int experts, m_tiles, n_tiles, k_blocks, unit_rows, rank;
+  int e = 0;
+  int64_t t, step, base = 0;
+
+  PONNI_B200_HD Tiles(const Sizes& p, const int* lo_, const int* hi_, int64_t first, int64_t step_, int rank_)
+      : lo(lo_), hi(hi_), experts(p.experts), unit_rows(p.unit_rows), rank(rank_), t(first), step(step_) {
+    const int n = MODE == kRows ? p.inputs : p.outputs, k = MODE == kForward ? p.inputs : p.outputs;
+    m_tiles = (p.inputs + CG * kBM - 1) / (CG * kBM);
+    n_tiles = (n + BN - 1) / BN;
+    k_blocks = (k + kBK - 1) / kBK;
+  }
+  PONNI_B200_HD int64_t count(int i) const {
+    const int rows = hi[i] - lo[i];
+    if (MODE != kWeights) return (int64_t)((rows + CG * kBM - 1) / (CG * kBM)) * n_tiles;
+    return (int64_t)(unit_rows ? (rows + unit_rows - 1) / unit_rows : 1) * m_tiles * n_tiles;
+  }
+  PONNI_B200_HD bool next(Tile& v) {
+    int64_t c = 0;
+    while (e < experts && t >= base + (c = count(e))) {
+      base += c;
+      ++e;
+    }
+    if (e >= experts) return false;
+    const int64_t local = t - base;
+    t += step;
+    v.e = e;
+    v.lo = lo[e];
+    v.hi = hi[e];
+    if (MODE != kWeights) {
+      const int m = (v.hi - v.lo + CG * kBM - 1) / (CG * kBM);
+      v.n0 = (int)(local / m) * BN;
+      v.m0 = (int)(local % m) * CG * kBM;
+      v.k_blocks = k_blocks;
+    } else {
+      const int per = m_tiles * n_tiles;
+      const int unit = (int)(local / per), i = (int)(local % per);
+      v.m0 = i % m_tiles * CG * kBM;
+      v.n0 = i / m_tiles * BN;
+      v.slot = base / per + unit;
+      if (unit_rows) {
+        v.lo += unit * unit_rows;
+        if (v.hi > v.lo + unit_rows) v.hi = v.lo + unit_rows;
+      }
+      v.k_blocks = (v.hi - v.lo + kBK - 1) / kBK;
+    }
+    if (CG == 2) v.m0 += kBM * rank;
+    return true;
+  }
+};
+
+// Which of GROUPS groups of epilogue warps takes a tile.  A parity wait tells a
+// barrier's next phase from the present one, not from the one after the next, so a
+// group may not wait for a use of an accumulator before the use before it is
+// over.  Tiles therefore go by the accumulator that they use: with an even number of
+// them each belongs to one group, which has waited for its use before.  Tiles without
+// sums (experts without rows) use none; they are dealt out by a count of their own.
+template <int GROUPS> struct Turns {
+  int empty = 0;
+  PONNI_B200_HD bool mine(int group, bool sums, int buf) {
+    return GROUPS == 1 || (sums ? buf : empty++) % GROUPS == group;
+  }
+};
+
+}  // namespace grouped
+}  // namespace ponni_b200

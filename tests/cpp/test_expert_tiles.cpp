@@ -1,0 +1,138 @@
+// Host checks of the grouped product's tile sequence (ponni_b200/csrc/expert_tiles.h).
+#include <cstdio>
+#include <cstdlib>
+#include <random>
+#include <vector>
+
+#include "expert_tiles.h"
+
+using namespace ponni_b200::grouped;
+
+static int failures = 0;
+#define CHECK(c, ...)                            \
+  do {                                           \
+    if (!(c)) {                                  \
+      if (++failures < 20) {                     \
+        std::printf("%s: ", #c);                 \
+        std::printf(__VA_ARGS__);                \
+        std::printf("\n");                       \
+      }                                          \
+    }                                            \
+  } while (0)
+
+struct Groups {
+  std::vector<int> lo, hi;
+};
+static Groups groups_of(const std::vector<int>& rows) {
+  Groups g;
+  int at = 0;
+  for (int r : rows) {
+    g.lo.push_back(at);
+    g.hi.push_back(at += r);
+  }
+  return g;
+}
+
+// Accumulators complete in the order of the CTA's tiles.  A wait for use n of an
+// accumulator by its parity is safe once use n - 1 is known to be over: the same
+// group has waited for that use or for a later accumulator of the sequence.
+template <int BN, int GROUPS, int BUFS>
+static void check_waits(const Sizes& p, const Groups& g, int ctas) {
+  for (int cta = 0; cta < ctas; ++cta)
+    for (int group = 0; group < GROUPS; ++group) {
+      Tiles<kWeights, BN, 1> tiles(p, g.lo.data(), g.hi.data(), cta, ctas, 0);
+      Turns<GROUPS> turns;
+      Tile v;
+      int64_t sums = 0, known = -1;  // accumulators so far; the last one known to be complete
+      while (tiles.next(v)) {
+        const int64_t at = sums;
+        const bool mine = turns.mine(group, v.k_blocks > 0, (int)(at % BUFS));
+        if (v.k_blocks > 0) ++sums;
+        if (!mine || v.k_blocks == 0) continue;
+        CHECK(known >= at - BUFS, "%d experts, CTA %d, group %d: accumulator %lld awaited while %lld is the last known",
+              p.experts, cta, group, (long long)at, (long long)known);
+        known = at;
+      }
+    }
+}
+
+// Every tile of every CTA is taken by one group.
+template <int BN, int GROUPS, int BUFS>
+static void check_taken(const Sizes& p, const Groups& g, int ctas) {
+  for (int cta = 0; cta < ctas; ++cta) {
+    std::vector<int> taken;
+    for (int group = 0; group < GROUPS; ++group) {
+      Tiles<kWeights, BN, 1> tiles(p, g.lo.data(), g.hi.data(), cta, ctas, 0);
+      Turns<GROUPS> turns;
+      Tile v;
+      int64_t sums = 0;
+      size_t i = 0;
+      while (tiles.next(v)) {
+        if (taken.size() <= i) taken.push_back(0);
+        taken[i++] += turns.mine(group, v.k_blocks > 0, (int)(sums % BUFS));
+        if (v.k_blocks > 0) ++sums;
+      }
+    }
+    for (int t : taken) CHECK(t == 1, "a tile of CTA %d is taken %d times", cta, t);
+  }
+}
+
+static void empty_groups() {
+  // Empty and long groups in an order that gives one group of warps four accumulators in a row.
+  check_waits<64, 2, 4>({8, 18944, 64, 0}, groups_of({4096, 0, 4096, 0, 4096, 0, 4096, 4096}), 148);
+  std::mt19937 rng(1);
+  for (int experts : {2, 16, 64, 128, 256, 1024})
+    for (double empty : {0.0, 0.2, 0.5, 0.9})
+      for (int inputs : {64, 300, 1024, 2048})
+        for (int round = 0; round < 5; ++round) {
+          std::vector<int> rows(experts);
+          for (int& r : rows) r = std::uniform_real_distribution<>(0, 1)(rng) < empty ? 0 : 1 + (int)(rng() % 300);
+          const Groups g = groups_of(rows);
+          const Sizes p = {experts, inputs, 64, 0};
+          check_waits<64, 2, 4>(p, g, 148);
+          check_taken<64, 2, 4>(p, g, 148);
+        }
+}
+
+// All tiles together cover every group's rows and columns once.
+template <int MODE, int BN, int CG>
+static void check_cover(const Sizes& p, const Groups& g, int ctas) {
+  const int m_all = MODE == kWeights ? (p.inputs + kBM - 1) / kBM : 0;
+  const int n_tiles = ((MODE == kRows ? p.inputs : p.outputs) + BN - 1) / BN;
+  int64_t want = 0, got = 0;
+  for (int e = 0; e < p.experts; ++e) {
+    const int rows = g.hi[e] - g.lo[e];
+    if (MODE != kWeights) want += (int64_t)((rows + kBM - 1) / kBM) * n_tiles;
+    else want += (int64_t)m_all * n_tiles * (p.unit_rows ? (rows + p.unit_rows - 1) / p.unit_rows : 1);
+  }
+  std::vector<char> seen;
+  for (int cta = 0; cta < ctas * CG; ++cta) {
+    Tiles<MODE, BN, CG> tiles(p, g.lo.data(), g.hi.data(), cta / CG, ctas, cta % CG);
+    Tile v;
+    while (tiles.next(v)) {
+      const int m_end = MODE == kWeights ? p.inputs : v.hi - v.lo;
+      CHECK(v.e >= 0 && v.e < p.experts && v.lo >= g.lo[v.e] && v.hi <= g.hi[v.e] && v.m0 % kBM == 0, "expert %d", v.e);
+      if (v.m0 < m_end) ++got;
+    }
+  }
+  CHECK(got == want, "%lld tiles, not %lld", (long long)got, (long long)want);
+}
+
+static void cover() {
+  const Groups g = groups_of({0, 1, 128, 129, 0, 1000, 255, 256, 257, 0});
+  for (int inputs : {1, 128, 300})
+    for (int outputs : {1, 64, 129, 700}) {
+      check_cover<kForward, 128, 1>({10, inputs, outputs, 0}, g, 7);
+      check_cover<kForward, 256, 2>({10, inputs, outputs, 0}, g, 7);
+      check_cover<kRows, 64, 1>({10, inputs, outputs, 0}, g, 7);
+      check_cover<kWeights, 128, 2>({10, inputs, outputs, 0}, g, 7);
+      check_cover<kWeights, 64, 1>({10, inputs, outputs, 128}, g, 7);
+    }
+}
+
+int main() {
+  empty_groups();
+  cover();
+  if (failures) std::printf("%d failures\n", failures);
+  return failures != 0;
+}

@@ -1,0 +1,75 @@
+"""Mixture-of-experts operators at the ends of their ranges, on the GPU.
+
+Where it can be, the data are small integers: their products and sums are exact in
+fp32 in any order (below 2^24), so a result has to equal the 64-bit value rounded
+to the result's type, and a lost, doubled or foreign row shows.
+"""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import ponni_b200 as pb  # noqa: E402
+from tests import expert_ref as R  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+DT = R.DTYPES
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def randn(g, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+def integers(g, *shape, dtype=torch.float32, most=2):
+    return torch.randint(-most, most + 1, shape, generator=g, device="cuda").to(dtype)
+
+
+def offsets(counts):
+    return torch.tensor([0] + list(torch.tensor(counts).cumsum(0)), dtype=torch.int32, device="cuda")
+
+
+def exact_weights(d, rows, counts):
+    """The weight gradient of integer data, exactly."""
+    out = torch.zeros(len(counts), rows.shape[1], d.shape[1], dtype=torch.float64, device="cuda")
+    lo = 0
+    for e, n in enumerate(counts):
+        out[e] = rows[lo:lo + n].double().t() @ d[lo:lo + n].double()
+        lo += n
+    return out
+
+
+# ------------------------------------------------------- groups without rows ----
+@pytest.mark.parametrize("experts,inputs,outputs", [(128, 2048, 64), (256, 1024, 40), (128, 2048, 130), (64, 520, 300)])
+@pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
+def test_weight_gradient_many_empty_groups(experts, inputs, outputs, dt):
+    g = gen(experts + outputs)
+    counts = torch.randint(1, 90, (experts,), generator=g, device="cuda").cpu()
+    counts[torch.rand(experts, generator=g, device="cuda").cpu() < 0.5] = 0
+    counts[experts // 3] = 3000
+    counts = counts.tolist()
+    n = sum(counts)
+    rows, d = integers(g, n, inputs, dtype=DT[dt]), integers(g, n, outputs, dtype=DT[dt])
+    w = torch.zeros(experts, inputs, outputs, dtype=DT[dt], device="cuda")
+    _, dw, db = pb.expert_product_backward(d, rows, w, offsets(counts), need_rows=False)
+    assert torch.equal(dw, exact_weights(d, rows, counts).to(DT[dt]))
+    ones = torch.ones(n, 1, dtype=DT[dt], device="cuda")
+    assert torch.equal(db, exact_weights(d, ones, counts)[:, 0].to(DT[dt]))
+    pb.check_operators()
+
+
+def test_weight_gradient_alternating_empty_groups():
+    """Long and empty groups in an order that gives one half of the epilogue four tiles in a row."""
+    g = gen(3)
+    counts = [4096, 0, 4096, 0, 4096, 0, 4096, 4096]
+    n = sum(counts)
+    rows, d = integers(g, n, 18944, dtype=torch.bfloat16, most=1), integers(g, n, 64, dtype=torch.bfloat16, most=1)
+    w = torch.zeros(8, 18944, 64, dtype=torch.bfloat16, device="cuda")
+    for _ in range(3):
+        _, dw, _ = pb.expert_product_backward(d, rows, w, offsets(counts), bias=False, need_rows=False)
+        assert torch.equal(dw, exact_weights(d, rows, counts).bfloat16())
+    pb.check_operators()
