@@ -65,8 +65,6 @@ constexpr int kBlock = 32 * (2 + kEpiWarps);
 constexpr int kEpiPitch = 48;  // bytes of a staged output row segment of 32 (+16: conflict-free)
 constexpr int kEpiBytes = kEpiWarps * 32 * kEpiPitch;
 constexpr int kBiasBytes = kEpiWarps * 64 * 4;
-constexpr int kMaxStages = 8;
-constexpr int kSmemLimit = 232448;
 
 struct Args {
   const void* a;  // kForward: rows; kRows: d_out; kWeights: rows (as the caller gave them)
@@ -349,6 +347,7 @@ __global__ void __launch_bounds__(kBlock, 1)
   __shared__ uint64_t bars[3 * kMaxStages + 2 * 4 + 1];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
+  static_assert(sizeof bars + sizeof tmem_slot + sizeof abort_word + 16 <= kStaticBytes, "static shared memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   unsigned char* base_ptr = smem_raw + (base - raw);
@@ -1282,12 +1281,11 @@ ponni_b200_status launch_shape(const Operand& a, const Operand& b, Args p, int s
   const int k = MODE == kForward ? p.inputs : p.outputs;
   p.boxes = MODE != kWeights && k <= 8 * kBK ? 2 : 1;
   const int epi = epi_bytes<S>(p.boxes);
-  const int fixed = 1024 + epi + kBiasBytes + 2 * p.experts * (int)sizeof(int) + 512;
-  p.stages = std::min(kMaxStages, (kSmemLimit - fixed) / S::stage_bytes);
-  const int smem = 1024 + p.stages * S::stage_bytes + epi + kBiasBytes + 2 * p.experts * (int)sizeof(int);
+  const Memory memory = memory_of(S::stage_bytes, epi + kBiasBytes, p.experts);
+  p.stages = memory.stages;
   auto kern = product_kernel<T, MODE, P, BN, CG>;
   static std::atomic<uint64_t> allowed{0};
-  cudaError_t e = ops::allow_smem(reinterpret_cast<const void*>(kern), kSmemLimit - 1024, p.device, allowed);
+  cudaError_t e = ops::allow_smem(reinterpret_cast<const void*>(kern), kDynamicBytes, p.device, allowed);
   if (e != cudaSuccess) return ops::fail_cuda(e, "expert_product");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
@@ -1299,7 +1297,7 @@ ponni_b200_status launch_shape(const Operand& a, const Operand& b, Args p, int s
   attr[1].val.clusterDim.z = 1;
   cfg.gridDim = dim3((unsigned)(CG * std::max<int64_t>(1, std::min<int64_t>(sms / CG, tiles))));
   cfg.blockDim = dim3(kBlock);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = memory.bytes;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = CG == 2 ? 2 : 1;

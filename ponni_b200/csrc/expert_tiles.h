@@ -98,5 +98,19 @@ template <int GROUPS> struct Turns {
   }
 };
 
+// Shared memory of the kernel.  A block has 227 KB, static and dynamic together;
+// kStaticBytes of them cover the static part (barriers, the TMEM address).  The launch asks
+// for `bytes`, and the kernel is allowed kDynamicBytes.
+constexpr int kStaticBytes = 512, kDynamicBytes = 232448 - kStaticBytes, kMaxStages = 8;
+struct Memory {
+  int stages, bytes;
+};
+// Stages of `stage_bytes` beside `other` bytes and two bounds for every expert; 1024 bytes align the first stage.
+inline Memory memory_of(int stage_bytes, int other, int experts) {
+  const int fixed = 1024 + other + 2 * experts * (int)sizeof(int), fit = (kDynamicBytes - fixed) / stage_bytes;
+  const int stages = fit < kMaxStages ? fit : kMaxStages;
+  return {stages, fixed + stages * stage_bytes};
+}
+
 }  // namespace grouped
 }  // namespace ponni_b200

@@ -130,7 +130,21 @@ static void cover() {
     }
 }
 
+// Every launch asks for no more than the kernel is allowed, for every number of experts:
+// stages of 24 to 96 KB (tile shapes), staging of 24, 32 and 64 KB, a bias strip a warp.
+static void memory() {
+  for (int stage : {24576, 32768, 49152, 98304})
+    for (int epi : {24576, 32768, 65536})
+      for (int experts = 1; experts <= 1024; ++experts) {
+        if (stage == 98304 && epi > 24576) continue;  // (fp32 parts: the small staging)
+        const Memory m = memory_of(stage, epi + 4096, experts);
+        CHECK(m.stages >= 1 && m.bytes <= kDynamicBytes && m.bytes + kStaticBytes <= 227 * 1024,
+              "%d experts, stages of %d: %d bytes", experts, stage, m.bytes);
+      }
+}
+
 int main() {
+  memory();
   empty_groups();
   cover();
   if (failures) std::printf("%d failures\n", failures);

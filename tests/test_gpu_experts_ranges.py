@@ -73,3 +73,36 @@ def test_weight_gradient_alternating_empty_groups():
         _, dw, _ = pb.expert_product_backward(d, rows, w, offsets(counts), bias=False, need_rows=False)
         assert torch.equal(dw, exact_weights(d, rows, counts).bfloat16())
     pb.check_operators()
+
+
+# ------------------------------------------------------------- many experts ----
+@pytest.mark.parametrize("experts", [640, 641, 704, 705, 1024])
+@pytest.mark.parametrize("dt,each,inputs,outputs", [
+    ("bf16", 3, 24, 100), ("f16", 3, 100, 40),  # 128 and 64 columns, few rows each
+    ("bf16", 66, 24, 250),                      # 256 columns, one CTA
+    ("bf16", 770, 130, 24), ("f16", 770, 24, 200),  # pairs
+    ("f32", 50, 24, 130),                       # parts
+])
+def test_product_many_experts(experts, dt, each, inputs, outputs):
+    g = gen(experts)
+    counts = [each] * experts
+    counts[5], counts[6] = 0, 2 * each
+    n, off = sum(counts), offsets(counts)
+    rows, w, d = (integers(g, *s, dtype=DT[dt], most=1) for s in ((n, inputs), (experts, inputs, outputs), (n, outputs)))
+    b = integers(g, experts, outputs, dtype=DT[dt])
+    want, _ = R.product(rows, w, off, b)
+    assert torch.equal(pb.expert_product(rows, w, off, bias=b), want.to(DT[dt]))
+    for got, (want, _) in zip(pb.expert_product_backward(d, rows, w, off), R.product_gradient(d, rows, w, off)):
+        assert torch.equal(got, want.to(DT[dt]))
+    pb.check_operators()
+
+
+@pytest.mark.parametrize("experts", [641, 704])
+def test_product_many_experts_f32_pairs(experts):
+    g = gen(experts)
+    each, inputs, outputs = 8192, 16, 130
+    off = offsets([each] * experts)
+    rows, w = integers(g, experts * each, inputs, most=1), integers(g, experts, inputs, outputs, most=1)
+    want = torch.bmm(rows.view(experts, each, inputs), w)  # integers: exact
+    assert torch.equal(pb.expert_product(rows, w, off).view_as(want), want)
+    pb.check_operators()
