@@ -25,6 +25,7 @@ ponni_b200_status fail(ponni_b200_status s, const std::string& msg) {
 }
 
 ponni_b200_status fail_cuda(cudaError_t e, const char* what) {
+  cudaGetLastError();  // reported here, not again by the caller's next look at the runtime's error
   return fail(PONNI_B200_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 

@@ -106,3 +106,23 @@ def test_product_many_experts_f32_pairs(experts):
     want = torch.bmm(rows.view(experts, each, inputs), w)  # integers: exact
     assert torch.equal(pb.expert_product(rows, w, off).view_as(want), want)
     pb.check_operators()
+
+
+# -------------------------------------------------------------------- errors ----
+def test_a_failed_call_leaves_no_error_behind():
+    """The operator check waits for its stream, which a capture forbids: the call reports it, and the runtime's error is clear."""
+    import ctypes
+    runtime, L = ctypes.CDLL("libcudart.so.12"), pb._abi.lib()
+    pb.check_operators()
+    side = torch.cuda.Stream()
+    stream = ctypes.c_void_p(side.cuda_stream)
+    graph = ctypes.c_void_p()
+    assert runtime.cudaStreamBeginCapture(stream, 1) == 0  # 1: only this thread's calls are held to the capture
+    status = L.ponni_b200_operator_check(0, stream)
+    left = runtime.cudaPeekAtLastError()
+    runtime.cudaStreamEndCapture(stream, ctypes.byref(graph))  # the forbidden wait has ended the capture
+    runtime.cudaGetLastError()
+    assert status == 4 and left == 0
+    x = torch.randn(4, 10, device="cuda")
+    assert pb.gather_columns(x, pb.route_columns(x, 1)).shape == (10, 4)
+    pb.check_operators()
