@@ -163,6 +163,20 @@ __device__ __forceinline__ void check_offsets(const int* __restrict__ offset, in
 }
 __device__ __forceinline__ int clamped(int o, int lo, int64_t rows) { return (int)min(max((int64_t)o, (int64_t)lo), rows); }
 
+// Bounds of all groups into shared memory, by the whole block, which may use them on return.
+__device__ __forceinline__ void read_bounds(int* edge, const int* __restrict__ offset, int experts, int64_t rows) {
+  bool descends = false;
+  for (int e = threadIdx.x; e <= experts; e += blockDim.x) {
+    const int b = bound(offset[e], rows);
+    edge[e] = b;
+    descends |= e > 0 && b < bound(offset[e - 1], rows);
+  }
+  if (__syncthreads_or(descends)) {
+    if (threadIdx.x == 0) ascending(edge, experts);
+    __syncthreads();
+  }
+}
+
 // The sum of one output element straight from the fp32 operands: taken where the
 // split parts gave NaN, because an infinite value times another's zero part is
 // NaN where the plain product is infinite.  Sums of more than kPlainTerms terms
@@ -354,8 +368,7 @@ __global__ void __launch_bounds__(kBlock, 1)
   unsigned char* epi = base_ptr + p.stages * S::stage_bytes;
   const int epi_total = epi_bytes<S>(p.boxes);
   float* bias_s = reinterpret_cast<float*>(epi + epi_total);
-  int* lo = reinterpret_cast<int*>(epi + epi_total + kBiasBytes);
-  int* hi = lo + p.experts;
+  int* edge = reinterpret_cast<int*>(epi + epi_total + kBiasBytes);
   const uint32_t bar0 = smem_u32(bars);
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
@@ -387,19 +400,14 @@ __global__ void __launch_bounds__(kBlock, 1)
     else tmem_alloc(smem_u32(&tmem_slot), 512);
   }
   ops::wait_for_predecessor();
-  for (int e = tid; e < p.experts; e += kBlock) {
-    const int l = clamped(p.offset[e], 0, p.rows);
-    lo[e] = l;
-    hi[e] = clamped(p.offset[e + 1], l, p.rows);
-  }
   if (blockIdx.x == 0) check_offsets(p.offset, p.experts, p.rows, p.error);
   tc_fence_before();
+  read_bounds(edge, p.offset, p.experts, p.rows);
   if constexpr (CG == 2) cluster_sync();  // the barriers exist before the other CTA's arrivals
-  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  Tiles<MODE, BN, CG> tiles({p.experts, p.inputs, p.outputs, p.unit_rows}, lo, hi, blockIdx.x / CG, gridDim.x / CG, (int)rank);
+  Tiles<MODE, BN, CG> tiles({p.experts, p.inputs, p.outputs, p.unit_rows}, edge, blockIdx.x / CG, gridDim.x / CG, (int)rank);
   Tile v;
   int64_t issued = 0;  // stages filled so far (thread 0)
   if (warp == 0) {
@@ -985,6 +993,7 @@ __global__ void __launch_bounds__(256)
     sum_units_kernel(const float* __restrict__ partial, T* __restrict__ c, const int* __restrict__ offset, int experts,
                      int64_t rows, int unit_rows, int64_t per_expert) {
   __shared__ int64_t first_s;
+  const int64_t most = slots(rows, unit_rows, experts);  // (offsets out of order would give more)
   ops::wait_for_predecessor();
   const int e = blockIdx.y;
   auto units = [&](int i) {
@@ -998,8 +1007,9 @@ __global__ void __launch_bounds__(256)
     if (threadIdx.x == 0) first_s = n;
   }
   __syncthreads();
-  const int n = units(e);
-  const float* src = partial + first_s * per_expert;
+  const int64_t first = min(first_s, most);
+  const int n = (int)min((int64_t)units(e), most - first);
+  const float* src = partial + first * per_expert;
   for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < per_expert; i += (int64_t)gridDim.x * 256) {
     float s = 0.0f;
 #pragma unroll 4
@@ -1235,7 +1245,7 @@ int unit_rows_of(int dtype, int64_t rows, int experts, int inputs, int outputs, 
 }
 int64_t partial_bytes(int dtype, int64_t rows, int experts, int inputs, int outputs, int sms) {
   const int unit = unit_rows_of(dtype, rows, experts, inputs, outputs, sms);
-  return unit ? pad256((rows / unit + experts) * (int64_t)inputs * outputs * 4) : 0;
+  return unit ? pad256(slots(rows, unit, experts) * inputs * outputs * 4) : 0;
 }
 
 // Parts of a group's rows in the bias gradient: about four blocks an SM, of 128

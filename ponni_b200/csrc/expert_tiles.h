@@ -29,25 +29,35 @@ struct Sizes {
   int unit_rows;  // kWeights: rows of a unit (a multiple of kBK); 0: a group is one unit
 };
 
+// A bound of a group as the caller's offset has it, kept within the rows.
+PONNI_B200_HD int bound(int offset, int64_t rows) { return offset < 0 ? 0 : offset > rows ? (int)rows : offset; }
+// Bounds that descend somewhere (which is reported) become a running maximum: the
+// groups stay disjoint, so that all of them together have no more units than slots().
+PONNI_B200_HD void ascending(int* edge, int experts) {
+  for (int e = 1; e <= experts; ++e)
+    if (edge[e] < edge[e - 1]) edge[e] = edge[e - 1];
+}
+// Units of all groups at most: every group's last one may be short.
+PONNI_B200_HD int64_t slots(int64_t rows, int unit_rows, int experts) { return rows / unit_rows + experts; }
+
 // The tile sequence of a CTA (pair): tile `first`, then every `step`-th one, of
 // all tiles: experts in order, row tiles innermost (neighbours share the weight
 // tile).  m0 is the first row of CTA `rank` of the pair.
 template <int MODE, int BN, int CG> struct Tiles {
-  const int* lo;
-  const int* hi;
+  const int* edge;  // bounds of the groups (bound, ascending): group e is [edge[e], edge[e + 1])
   int experts, m_tiles, n_tiles, k_blocks, unit_rows, rank;
   int e = 0;
   int64_t t, step, base = 0;
 
-  PONNI_B200_HD Tiles(const Sizes& p, const int* lo_, const int* hi_, int64_t first, int64_t step_, int rank_)
-      : lo(lo_), hi(hi_), experts(p.experts), unit_rows(p.unit_rows), rank(rank_), t(first), step(step_) {
+  PONNI_B200_HD Tiles(const Sizes& p, const int* edge_, int64_t first, int64_t step_, int rank_)
+      : edge(edge_), experts(p.experts), unit_rows(p.unit_rows), rank(rank_), t(first), step(step_) {
     const int n = MODE == kRows ? p.inputs : p.outputs, k = MODE == kForward ? p.inputs : p.outputs;
     m_tiles = (p.inputs + CG * kBM - 1) / (CG * kBM);
     n_tiles = (n + BN - 1) / BN;
     k_blocks = (k + kBK - 1) / kBK;
   }
   PONNI_B200_HD int64_t count(int i) const {
-    const int rows = hi[i] - lo[i];
+    const int rows = edge[i + 1] - edge[i];
     if (MODE != kWeights) return (int64_t)((rows + CG * kBM - 1) / (CG * kBM)) * n_tiles;
     return (int64_t)(unit_rows ? (rows + unit_rows - 1) / unit_rows : 1) * m_tiles * n_tiles;
   }
@@ -61,8 +71,8 @@ template <int MODE, int BN, int CG> struct Tiles {
     const int64_t local = t - base;
     t += step;
     v.e = e;
-    v.lo = lo[e];
-    v.hi = hi[e];
+    v.lo = edge[e];
+    v.hi = edge[e + 1];
     if (MODE != kWeights) {
       const int m = (v.hi - v.lo + CG * kBM - 1) / (CG * kBM);
       v.n0 = (int)(local / m) * BN;
@@ -105,9 +115,9 @@ constexpr int kStaticBytes = 512, kDynamicBytes = 232448 - kStaticBytes, kMaxSta
 struct Memory {
   int stages, bytes;
 };
-// Stages of `stage_bytes` beside `other` bytes and two bounds for every expert; 1024 bytes align the first stage.
+// Stages of `stage_bytes` beside `other` bytes and the groups' bounds; 1024 bytes align the first stage.
 inline Memory memory_of(int stage_bytes, int other, int experts) {
-  const int fixed = 1024 + other + 2 * experts * (int)sizeof(int), fit = (kDynamicBytes - fixed) / stage_bytes;
+  const int fixed = 1024 + other + (experts + 1) * (int)sizeof(int), fit = (kDynamicBytes - fixed) / stage_bytes;
   const int stages = fit < kMaxStages ? fit : kMaxStages;
   return {stages, fixed + stages * stage_bytes};
 }

@@ -20,16 +20,10 @@ static int failures = 0;
     }                                            \
   } while (0)
 
-struct Groups {
-  std::vector<int> lo, hi;
-};
+using Groups = std::vector<int>;  // bounds
 static Groups groups_of(const std::vector<int>& rows) {
-  Groups g;
-  int at = 0;
-  for (int r : rows) {
-    g.lo.push_back(at);
-    g.hi.push_back(at += r);
-  }
+  Groups g = {0};
+  for (int r : rows) g.push_back(g.back() + r);
   return g;
 }
 
@@ -40,7 +34,7 @@ template <int BN, int GROUPS, int BUFS>
 static void check_waits(const Sizes& p, const Groups& g, int ctas) {
   for (int cta = 0; cta < ctas; ++cta)
     for (int group = 0; group < GROUPS; ++group) {
-      Tiles<kWeights, BN, 1> tiles(p, g.lo.data(), g.hi.data(), cta, ctas, 0);
+      Tiles<kWeights, BN, 1> tiles(p, g.data(), cta, ctas, 0);
       Turns<GROUPS> turns;
       Tile v;
       int64_t sums = 0, known = -1;  // accumulators so far; the last one known to be complete
@@ -62,7 +56,7 @@ static void check_taken(const Sizes& p, const Groups& g, int ctas) {
   for (int cta = 0; cta < ctas; ++cta) {
     std::vector<int> taken;
     for (int group = 0; group < GROUPS; ++group) {
-      Tiles<kWeights, BN, 1> tiles(p, g.lo.data(), g.hi.data(), cta, ctas, 0);
+      Tiles<kWeights, BN, 1> tiles(p, g.data(), cta, ctas, 0);
       Turns<GROUPS> turns;
       Tile v;
       int64_t sums = 0;
@@ -101,17 +95,17 @@ static void check_cover(const Sizes& p, const Groups& g, int ctas) {
   const int n_tiles = ((MODE == kRows ? p.inputs : p.outputs) + BN - 1) / BN;
   int64_t want = 0, got = 0;
   for (int e = 0; e < p.experts; ++e) {
-    const int rows = g.hi[e] - g.lo[e];
+    const int rows = g[e + 1] - g[e];
     if (MODE != kWeights) want += (int64_t)((rows + kBM - 1) / kBM) * n_tiles;
     else want += (int64_t)m_all * n_tiles * (p.unit_rows ? (rows + p.unit_rows - 1) / p.unit_rows : 1);
   }
   std::vector<char> seen;
   for (int cta = 0; cta < ctas * CG; ++cta) {
-    Tiles<MODE, BN, CG> tiles(p, g.lo.data(), g.hi.data(), cta / CG, ctas, cta % CG);
+    Tiles<MODE, BN, CG> tiles(p, g.data(), cta / CG, ctas, cta % CG);
     Tile v;
     while (tiles.next(v)) {
       const int m_end = MODE == kWeights ? p.inputs : v.hi - v.lo;
-      CHECK(v.e >= 0 && v.e < p.experts && v.lo >= g.lo[v.e] && v.hi <= g.hi[v.e] && v.m0 % kBM == 0, "expert %d", v.e);
+      CHECK(v.e >= 0 && v.e < p.experts && v.lo >= g[v.e] && v.hi <= g[v.e + 1] && v.m0 % kBM == 0, "expert %d", v.e);
       if (v.m0 < m_end) ++got;
     }
   }
@@ -130,6 +124,29 @@ static void cover() {
     }
 }
 
+// Offsets of any kind: every tile lies within the rows, every unit has its slot.
+static void offsets_out_of_order() {
+  std::mt19937 rng(2);
+  for (int experts : {1, 2, 9, 64, 1024})
+    for (int rows : {1, 5000, 100000})
+      for (int round = 0; round < 20; ++round) {
+        const int unit = 256;
+        std::vector<int> edge(experts + 1);
+        for (int e = 0; e <= experts; ++e) {
+          int o = round == 0 ? (e % 2) * rows : (int)(rng() % (2 * rows)) - rows / 2;
+          if (round == 1) o = e % 2 ? INT32_MAX : INT32_MIN;
+          edge[e] = bound(o, rows);
+        }
+        ascending(edge.data(), experts);
+        Tiles<kWeights, 128, 1> tiles({experts, 128, 128, unit}, edge.data(), 0, 1, 0);
+        Tile v;
+        while (tiles.next(v))
+          CHECK(v.lo >= 0 && v.lo <= v.hi && v.hi <= rows && v.slot >= 0 && v.slot < slots(rows, unit, experts),
+                "%d experts, %d rows: rows %d to %d in slot %lld of %lld", experts, rows, v.lo, v.hi, (long long)v.slot,
+                (long long)slots(rows, unit, experts));
+      }
+}
+
 // Every launch asks for no more than the kernel is allowed, for every number of experts:
 // stages of 24 to 96 KB (tile shapes), staging of 24, 32 and 64 KB, a bias strip a warp.
 static void memory() {
@@ -145,6 +162,7 @@ static void memory() {
 
 int main() {
   memory();
+  offsets_out_of_order();
   empty_groups();
   cover();
   if (failures) std::printf("%d failures\n", failures);

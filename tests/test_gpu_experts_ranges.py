@@ -126,3 +126,25 @@ def test_a_failed_call_leaves_no_error_behind():
     x = torch.randn(4, 10, device="cuda")
     assert pb.gather_columns(x, pb.route_columns(x, 1)).shape == (10, 4)
     pb.check_operators()
+
+
+def test_offsets_out_of_order_stay_within_the_workspace():
+    """Alternating offsets would make many groups of all rows: more units of the weight gradient than there is room for."""
+    L = pb._abi.lib()
+    g = gen(4)
+    experts, n, f = 64, 200_000, 64
+    rows, d = randn(g, n, f, dtype=torch.bfloat16), randn(g, n, f, dtype=torch.bfloat16)
+    w = torch.zeros(experts, f, f, dtype=torch.bfloat16, device="cuda")
+    dw = torch.empty_like(w)
+    off = (torch.arange(experts + 1, device="cuda") % 2 * n).to(torch.int32)
+    need = L.ponni_b200_expert_product_workspace(pb._abi.BF16, n, experts, f, f, 1, 1, 0)
+    assert need > 0
+    buf = torch.full((need + (64 << 20),), 77, dtype=torch.uint8, device="cuda")
+    pb.check_operators()
+    stream = pb.torch_stream_handle(rows.device)
+    assert L.ponni_b200_expert_product_backward(pb._abi.BF16, d.data_ptr(), f, rows.data_ptr(), f, n, w.data_ptr(), f, f * f,
+                                                off.data_ptr(), experts, f, f, None, 0, dw.data_ptr(), None, buf.data_ptr(),
+                                                need, 0, stream) == 0
+    with pytest.raises(pb.PonniError, match="ascending"):
+        pb.check_operators()
+    assert (buf[need:] == 77).all()
