@@ -295,7 +295,11 @@ ponni_b200_status ponni_b200_gradient_set_create(const void* const* tensors, con
     set->num_chunks = (int64_t)table.size();
     if (!table.empty()) {
       cudaError_t e = cudaMalloc(&set->chunks, table.size() * sizeof(Chunk));
-      if (e == cudaSuccess) e = cudaMemcpy(set->chunks, table.data(), table.size() * sizeof(Chunk), cudaMemcpyHostToDevice);
+      // (A plain copy from pageable memory returns once the table is staged, and a stream that
+      // does not wait for the default one could read it before it has arrived.)
+      if (e == cudaSuccess)
+        e = cudaMemcpyAsync(set->chunks, table.data(), table.size() * sizeof(Chunk), cudaMemcpyHostToDevice, nullptr);
+      if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
       if (e != cudaSuccess) {
         if (set->chunks) cudaFree(set->chunks);
         delete set;
