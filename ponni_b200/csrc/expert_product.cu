@@ -251,20 +251,29 @@ __device__ __noinline__ float4 activate4(float4 v, int kind, int flags, float s0
 // special-function unit bounds the epilogue of narrow products (256 -> 256: two of
 // its operations a value would take 139 of the 256 us measured with them), so two
 // values share one reciprocal: 1/a = b (1/ab) (213 us; 219 with two reciprocals,
-// 226 with half of the exponentials by polynomial).  The arguments are kept where ab is
-// finite, which also keeps a NaN from its neighbour.
-__device__ __forceinline__ void fast_silu32(float (&v)[32]) {
+// 226 with half of the exponentials by polynomial).  That needs ab finite and keeps no NaN
+// from its neighbour: false, and nothing done, where a value is NaN or below -43 (exponentials
+// up to 2^62.1); such rows take activate_one, as a few rows do.
+__device__ __forceinline__ float min_or_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ bool fast_silu32(float (&v)[32]) {
+  float least[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+  for (int i = 4; i < 32; ++i) least[i % 4] = min_or_nan(least[i % 4], v[i]);
+  if (!(min_or_nan(min_or_nan(least[0], least[1]), min_or_nan(least[2], least[3])) >= -43.0f)) return false;
 #pragma unroll
   for (int i = 0; i < 32; i += 2) {
     float a, b;
     f2::mul(a, b, v[i], v[i + 1], -kLog2e, -kLog2e);
-    a = fast_exp2(fminf(a, 60.0f));  // sigmoid at least 2^-60
-    b = fast_exp2(fminf(b, 60.0f));
-    f2::add(a, b, a, b, 1.0f, 1.0f);
+    f2::add(a, b, fast_exp2(a), fast_exp2(b), 1.0f, 1.0f);
     const float r = fast_rcp(a * b);
     f2::mul(a, b, b, a, r, r);
     f2::mul(v[i], v[i + 1], v[i], v[i + 1], a, b);
   }
+  return true;
 }
 __device__ __forceinline__ void fast_gelu32(float (&v)[32]) {
 #pragma unroll
@@ -299,7 +308,7 @@ __device__ __forceinline__ void activate_all(float (&v)[32], int kind, int flags
     return;
   }
   if constexpr (sizeof(T) == 2) {
-    if (kind == EPI_SILU) return fast_silu32(v);
+    if (kind == EPI_SILU && fast_silu32(v)) return;
     if (kind == EPI_GELU && !(flags & 0x2)) return fast_gelu32(v);
   } else if (kind == EPI_SILU) {
 #pragma unroll

@@ -148,3 +148,37 @@ def test_offsets_out_of_order_stay_within_the_workspace():
     with pytest.raises(pb.PonniError, match="ascending"):
         pb.check_operators()
     assert (buf[need:] == 77).all()
+
+
+# --------------------------------------------------------------- activations ----
+@pytest.mark.parametrize("layer", [pb.Relu, pb.LeakyRelu, pb.Elu, pb.Selu, pb.Gelu, pb.Silu, pb.Sigmoid, pb.Tanh,
+                                   pb.Softplus, pb.HardSigmoid, pb.HardSwish, pb.Mish])
+@pytest.mark.parametrize("rows", [1, 3, 64, 1000])  # a few rows, tiles of one CTA, pairs
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+def test_activation_of_extreme_values(layer, rows, dt):
+    """The product is value times one, so that the activation sees each value as it is; neighbours keep theirs."""
+    dtype = DT[dt]
+    lowest = torch.finfo(dtype).min
+    values = [v for v in (0.0, -1.0, 1.0, -20.0, -41.0, -43.5, -50.0, -88.0, -100.0, -1000.0, 100.0, -1e20, 1e20, lowest,
+                          float("-inf"), float("inf"), float("nan"), 0.5) if v != v or abs(v) in (0.0, float("inf")) or
+              abs(v) <= -lowest]
+    outputs = 130
+    w = torch.tensor(values, device="cuda").repeat(20)[:outputs].to(dtype).view(1, 1, outputs)
+    x = torch.ones(rows, 1, dtype=dtype, device="cuda")
+    act = layer(outputs)
+    off = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    y = pb.expert_product(x, w, off, activation=act)
+    want = R.activate(w.double().view(-1), act.label, act.scalar).expand(rows, outputs)
+    if dt == "f16":
+        want = torch.where(want.abs() >= 65520.0, want * float("inf"), want)  # beyond fp16's range
+    if layer is pb.Relu:
+        want = want.nan_to_num(nan=0.0, posinf=float("inf"))  # x > 0 ? x : 0
+    assert torch.equal(torch.isnan(y), torch.isnan(want))
+    fine = torch.isfinite(want)
+    inf = ~fine & ~torch.isnan(want)
+    assert torch.equal(y[inf].double(), want[inf])
+    # Each function is off by a few units of fp32, relative to its value (SiLU: and to its argument, at most 100,
+    # in the exponent: 100 * 2^-24), or to one where it is a difference from one; below 2^-120 by as much.
+    one = 0.0 if layer is pb.Silu else 2.0 ** -20
+    bound = (R.ULP[dtype] + 2.0 ** -17) * want.abs() + one + (2.0 ** -24 if dt == "f16" else 2.0 ** -120)
+    assert ((y.double() - want).abs() <= bound)[fine].all()
