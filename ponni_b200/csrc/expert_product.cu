@@ -23,8 +23,8 @@
 // products are kept (the three dropped are below 2^-24 of the magnitudes).  Each K
 // block of 64 goes into its own TMEM accumulator, the five small products first,
 // and is added to the tile's sum in fp32 registers: the tensor core truncates
-// when it accumulates, so long sums in TMEM would drift by a part of 2^-24 for
-// every step.  These products are bound by shared memory: a block's 24 MMAs of
+// when it accumulates, so long sums in TMEM drift by a part of 2^-24 for
+// every step (16-bit products are added up every kSegment blocks).  These products are bound by shared memory: a block's 24 MMAs of
 // 128 x 128 x 16 read 192 KB and its copies write 96 KB, 2250 cycles at 128 bytes a
 // cycle against 1536 of the tensor cores.  (K blocks of 32 and twice the stages are
 // 10% slower.)
@@ -60,6 +60,12 @@ using namespace tc;
 
 using namespace grouped;
 
+// K blocks of a 16-bit product that are summed in one accumulator before the epilogue adds
+// them to its fp32 sum.  The tensor core truncates as it accumulates: 32 blocks drift by 2^-16
+// of the sum at most, a thirty-second of fp16's rounding, whole groups of 2^20 rows would by
+// 2^-8.  (16384 rows, 4 experts of 8192 -> 2048: 365 us, 367 with 16 blocks, 364 without
+// segments; 2048 -> 2048, where 16 blocks make two segments: 197 us against 195.)
+constexpr int kSegment = 32;
 constexpr int kEpiWarps = 16;
 constexpr int kBlock = 32 * (2 + kEpiWarps);
 constexpr int kEpiPitch = 48;  // bytes of a staged output row segment of 32 (+16: conflict-free)
@@ -103,6 +109,9 @@ template <int P, int BN, int CG> struct Shape {
   // one accumulator (16-bit operands).
   static constexpr int groups = 4 / parts;
   static_assert(groups == 1 || (P == 1 && acc_bufs % groups == 0), "an accumulator belongs to one group");
+  // K blocks that are summed in one accumulator.  (Groups of warps: all of a tile's; the host gives
+  // them sums of at most kSegment blocks.)
+  static constexpr int segment = P == 3 ? 1 : groups > 1 ? 1 << 30 : kSegment;
   static constexpr int part_cols = BN / parts;
   // Output staging of a warp: boxes of 32 rows x 64 bytes for the copy engine
   // (16-bit operands in pairs or 64 wide), else its rows of 32 bytes: the boxes cost
@@ -134,6 +143,25 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
 }
+// 8 accumulator columns of this thread's TMEM lane, from `taddr` on and back.
+__device__ __forceinline__ void tmem_add8(uint32_t taddr, float* v) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 8; i += 2)
+    f2::add(v[i], v[i + 1], v[i], v[i + 1], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const float* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(taddr),
+               "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
+               "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])),
+               "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
+               : "memory");
+}
+
 // Arrival on another CTA's barrier after reading tensor memory, which the tcgen05
 // fence before it orders: no release of this thread's stores, which would cost
 // half a microsecond each.
@@ -530,7 +558,7 @@ __global__ void __launch_bounds__(kBlock, 1)
       while (ok && tiles.next(v)) {
         for (int kb = 0; kb < v.k_blocks; ++kb) {
           const uint32_t d = tmem + (uint32_t)(buf * S::acc_cols);
-          if (P == 3 || kb == 0) {
+          if (kb % S::segment == 0) {
             ok = wait_phase_abort(acc_empty(buf), acc_ph, abort_flag, PONNI_B200_WAIT_LIMIT);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -552,7 +580,7 @@ __global__ void __launch_bounds__(kBlock, 1)
           const uint32_t a0 = a_lo0 + (stage >> 4), b0 = b_lo0 + ((stage + S::a_bytes) >> 4);
           if constexpr (P == 1) {
 #pragma unroll
-            for (int k = 0; k < kBK / 16; ++k) mma(d, a0 + k * a_step, b0 + k * b_step, (kb > 0 || k > 0) ? 1u : 0u);
+            for (int k = 0; k < kBK / 16; ++k) mma(d, a0 + k * a_step, b0 + k * b_step, (kb % S::segment > 0 || k > 0) ? 1u : 0u);
           } else {
             constexpr uint32_t ap = kBM * kBK * 2 / 16, bp = S::b_rows * kBK * 2 / 16;
             constexpr int qa[6] = {1, 0, 2, 0, 1, 0}, qb[6] = {1, 2, 0, 1, 0, 0};
@@ -563,7 +591,7 @@ __global__ void __launch_bounds__(kBlock, 1)
                 mma(d, a0 + qa[q] * ap + k * a_step, b0 + qb[q] * bp + k * b_step, (q > 0 || k > 0) ? 1u : 0u);
           }
           commit(empty(s));
-          if (P == 3 || kb == v.k_blocks - 1) {
+          if (kb % S::segment == S::segment - 1 || kb == v.k_blocks - 1) {
             if (!skip) commit(acc_full(buf));
             skip = false;
             if (++buf == S::acc_bufs) {
@@ -706,6 +734,24 @@ __global__ void __launch_bounds__(kBlock, 1)
       };
       if (P == 1 && v.k_blocks > 0) {
         if (!(ok = wait_acc())) break;
+        if (v.k_blocks > S::segment) {
+          // A long sum: the accumulators of its segments added up, and put back in place of the last one.
+          float sum[S::part_cols] = {};
+#pragma unroll 1
+          for (int kb = S::segment;; kb += S::segment) {
+            const uint32_t t = tmem + lane_base + (uint32_t)(buf * S::acc_cols + part * S::part_cols);
+#pragma unroll
+            for (int i = 0; i < S::part_cols; i += 8) tmem_add8(t + i, sum + i);
+            if (kb >= v.k_blocks) break;
+            release_acc();
+            if (!(ok = wait_acc())) break;
+          }
+          if (!ok) break;
+          const uint32_t t = tmem + lane_base + (uint32_t)(buf * S::acc_cols + part * S::part_cols);
+#pragma unroll
+          for (int i = 0; i < S::part_cols; i += 8) tmem_st8(t + i, sum + i);
+          asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+        }
         const uint32_t t = tmem + lane_base + (uint32_t)(buf * S::acc_cols + part * S::part_cols);
         // One chunk at a time: both at once is slower (239 against 202 us for 256 -> 256
         // without activation), the stores then come in bursts.
@@ -1202,13 +1248,16 @@ int64_t staged_bytes(int dtype, int64_t rows, int cols) {
 }
 
 // Tile width.  An MMA of 128 x 64 takes as long as one of 128 x 128 (58 and 64
-// cycles for 16 k), so 64 is for products of at most 64 columns; 256 halves the
+// cycles for 16 k), so 64 is for products of at most 64 columns, whose sums (`terms` at
+// most) fit one segment: its two groups of epilogue warps cannot share an accumulator's
+// sums (2^18 rows, 64 experts, gradient of 1024 x 64: 119 us with 128 columns, 115 with 64
+// and sums that drift; 20000 rows, 20 experts of 512 x 48: 21.5 and 19.5); 256 halves the
 // reads of the row tile against 128 and is taken unless its padding costs over
 // an eighth more columns, or the rows are so few that the weights' traffic
 // decides (at most half a tile of rows a group): 128 then spreads them more evenly
 // over the SMs.
-int tile_width(int n, int64_t rows, int experts, bool weights) {
-  if (n <= 64) return 64;
+int tile_width(int n, int64_t terms, int64_t rows, int experts, bool weights) {
+  if (n <= 64 && terms <= kSegment * kBK) return 64;
   if (n <= 128 || (!weights && rows <= (int64_t)64 * experts)) return 128;
   auto padded = [&](int w) { return (int64_t)(n + w - 1) / w * w; };
   return padded(256) * 8 > padded(128) * 9 ? 128 : 256;
@@ -1230,7 +1279,8 @@ struct TileShape {
 };
 TileShape tile_shape(int dtype, int mode, int64_t rows, int experts, int inputs, int outputs) {
   const bool parts = dtype == PONNI_B200_F32;
-  TileShape t = {tile_width(mode == kRows ? inputs : outputs, rows, experts, mode == kWeights), 1};
+  const int64_t terms = mode == kForward ? inputs : mode == kRows ? outputs : rows;
+  TileShape t = {tile_width(mode == kRows ? inputs : outputs, terms, rows, experts, mode == kWeights), 1};
   if (t.columns > 64 && use_pairs(rows, experts, mode, parts)) t.ctas = 2;
   if (parts && t.ctas == 1) t.columns = 128;
   return t;

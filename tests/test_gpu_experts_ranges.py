@@ -62,6 +62,23 @@ def test_weight_gradient_many_empty_groups(experts, inputs, outputs, dt):
     pb.check_operators()
 
 
+@pytest.mark.parametrize("experts,inputs,outputs", [(128, 2048, 64), (1024, 300, 17)])
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_weight_gradient_short_and_empty_groups(experts, inputs, outputs, dt):
+    """Sums of at most one accumulator: tiles 64 columns wide, taken in turn by two halves of the epilogue."""
+    g = gen(experts)
+    counts = torch.randint(1, 2 * 1800 // experts, (experts,), generator=g, device="cuda").cpu()
+    counts[torch.rand(experts, generator=g, device="cuda").cpu() < 0.5] = 0
+    counts = counts.tolist()
+    n = sum(counts)
+    rows, d = integers(g, n, inputs, dtype=DT[dt]), integers(g, n, outputs, dtype=DT[dt])
+    w = torch.zeros(experts, inputs, outputs, dtype=DT[dt], device="cuda")
+    for _ in range(3):
+        _, dw, _ = pb.expert_product_backward(d, rows, w, offsets(counts), need_rows=False)
+        assert torch.equal(dw, exact_weights(d, rows, counts).to(DT[dt]))
+    pb.check_operators()
+
+
 def test_weight_gradient_alternating_empty_groups():
     """Long and empty groups in an order that gives one half of the epilogue four tiles in a row."""
     g = gen(3)
@@ -182,3 +199,55 @@ def test_activation_of_extreme_values(layer, rows, dt):
     one = 0.0 if layer is pb.Silu else 2.0 ** -20
     bound = (R.ULP[dtype] + 2.0 ** -17) * want.abs() + one + (2.0 ** -24 if dt == "f16" else 2.0 ** -120)
     assert ((y.double() - want).abs() <= bound)[fine].all()
+
+
+# ----------------------------------------------------------------- long sums ----
+def check_drift(got, want, terms):
+    """Sums of positive products.  The matrix units may drop up to a unit of fp32 (2^-23 of the partial sum) at each
+    step of 16 terms within an accumulator's 2048, which is 2^-16; the accumulators are added in fp32, a rounding
+    (2^-24) each.  Rounding the result to its type is off by half a unit, and on average, over results spread
+    across a factor of four, by nothing."""
+    off = (got.double() - want) / want
+    held = 2.0 ** -16 + (terms / 2048 + 1) * 2.0 ** -24
+    assert off.abs().max() <= R.ULP[got.dtype] * (1 + held) + held
+    assert off.mean().abs() <= held + 4 * R.ULP[got.dtype] / got.numel() ** 0.5
+
+
+def positive(g, *shape, dtype, scale=1.0, along=-1):
+    """In [1, 4) * scale, by a factor of its own for every index of dimension `along`."""
+    size = [1] * len(shape)
+    size[along] = shape[along]
+    spread = (1 + torch.rand(*size, generator=g, device="cuda")) * scale
+    return ((1 + torch.rand(*shape, generator=g, device="cuda")) * spread).to(dtype)
+
+
+@pytest.mark.parametrize("n", [40, 128, 250])
+@pytest.mark.parametrize("rows", [100, 1000])  # one CTA a tile, pairs
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_long_sums_do_not_drift(dt, rows, n):
+    g = gen(n)
+    terms, dtype = 200_000, DT[dt]
+    off = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    x = positive(g, rows, terms, dtype=dtype, scale=2.0 ** -8, along=0)
+    w = positive(g, 1, terms, n, dtype=dtype, scale=2.0 ** -4)
+    check_drift(pb.expert_product(x, w, off), x.double() @ w[0].double(), terms)
+    wt = w.transpose(1, 2).contiguous()
+    dr, _, _ = pb.expert_product_backward(x, x.new_zeros(rows, n), wt, off, bias=False, need_weights=False)
+    check_drift(dr, x.double() @ wt[0].double().t(), terms)
+    pb.check_operators()
+
+
+@pytest.mark.parametrize("inputs,outputs", [(300, 40), (64, 128), (200, 250), (2500, 2600)])
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_long_weight_gradients_do_not_drift(dt, inputs, outputs):
+    """(2500 x 2600 fills the SMs with whole groups, the others are split into units.)"""
+    g = gen(outputs)
+    n, dtype = 270_000, DT[dt]
+    off = torch.tensor([0, 100, n - 50], dtype=torch.int32, device="cuda")
+    x, d = positive(g, n, inputs, dtype=dtype, scale=2.0 ** -8), positive(g, n, outputs, dtype=dtype, scale=2.0 ** -4)
+    w = torch.zeros(2, inputs, outputs, dtype=dtype, device="cuda")
+    _, dw, _ = pb.expert_product_backward(d, x, w, off, bias=False, need_rows=False)
+    take = slice(0, 300)
+    check_drift(dw[1, take, take], x[100:n - 50, take].double().t() @ d[100:n - 50, take].double(), n)
+    check_drift(dw[0, take, take], x[:100, take].double().t() @ d[:100, take].double(), 100)
+    pb.check_operators()
