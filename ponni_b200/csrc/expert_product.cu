@@ -287,11 +287,14 @@ __device__ __forceinline__ float min_or_nan(float a, float b) {
   asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
-__device__ __forceinline__ bool fast_silu32(float (&v)[32]) {
+__device__ __forceinline__ float least_of(const float (&v)[32]) {
   float least[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
   for (int i = 4; i < 32; ++i) least[i % 4] = min_or_nan(least[i % 4], v[i]);
-  if (!(min_or_nan(min_or_nan(least[0], least[1]), min_or_nan(least[2], least[3])) >= -43.0f)) return false;
+  return min_or_nan(min_or_nan(least[0], least[1]), min_or_nan(least[2], least[3]));
+}
+__device__ __forceinline__ bool fast_silu32(float (&v)[32]) {
+  if (!(least_of(v) >= -43.0f)) return false;
 #pragma unroll
   for (int i = 0; i < 32; i += 2) {
     float a, b;
@@ -338,9 +341,11 @@ __device__ __forceinline__ void activate_all(float (&v)[32], int kind, int flags
   if constexpr (sizeof(T) == 2) {
     if (kind == EPI_SILU && fast_silu32(v)) return;
     if (kind == EPI_GELU && !(flags & 0x2)) return fast_gelu32(v);
-  } else if (kind == EPI_SILU) {
+  } else if (kind == EPI_SILU && least_of(v) >= -80.0f) {
+    // As activation() has it where no exponential overflows, in line: 2^20 rows of 256 -> 256 in
+    // 1590 us against 2050, 1465 with an approximate division.
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] *= fast_rcp(1.0f + expf(-v[i]));
+    for (int i = 0; i < 32; ++i) v[i] = v[i] / (1.0f + expf(-v[i]));
     return;
   }
 #pragma unroll

@@ -251,3 +251,14 @@ def test_long_weight_gradients_do_not_drift(dt, inputs, outputs):
     check_drift(dw[1, take, take], x[100:n - 50, take].double().t() @ d[100:n - 50, take].double(), n)
     check_drift(dw[0, take, take], x[:100, take].double().t() @ d[:100, take].double(), 100)
     pb.check_operators()
+
+
+@pytest.mark.parametrize("rows", [2, 100])  # a few rows, tiles
+def test_single_precision_silu(rows):
+    """Of an argument down to -88: exp is off by a few units, and its argument by half of one, 88 * 2^-25 in the exponent."""
+    z = torch.linspace(-88.0, 20.0, 500, device="cuda")
+    y = pb.expert_product(torch.ones(rows, 1, device="cuda"), z.view(1, 1, 500), offsets([rows]), activation=pb.Silu(500))
+    want = R.activate(z.double(), "SiLU").expand(rows, 500)
+    assert ((y.double() - want).abs() <= 2.0 ** -17 * want.abs()).all()
+    near = want[0, z > -1].abs()
+    assert ((y[:, z > -1].double() - want[:, z > -1]).abs() <= 2.0 ** -21 * near + 2.0 ** -140).all()
