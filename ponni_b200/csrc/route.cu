@@ -46,9 +46,14 @@ __device__ __forceinline__ void load_logits(const T* __restrict__ x, int64_t ld,
   }
 }
 
-// exp(v - best) for v <= best, 1 where they are equal (both may be infinite);
-// ex2 within 2^-22 of its value.  best is at least -FLT_MAX, so that v = -inf gives 0.
-__device__ __forceinline__ float from_best(float v, float best) {
+// exp(v - best) for v <= best, 1 where they are equal (both may be infinite).
+// best is at least -FLT_MAX, so that v = -inf gives 0.
+__device__ __forceinline__ float from_best(float v, float best) { return v == best ? 1.0f : expf(v - best); }
+// The same by the exponential unit alone, of a product rounded once: off by 2^-22 and 2^-24 of
+// best - v, 5e-6 where that is 80.  For the terms of a sum of which the best is 1, and for
+// results rounded to 16 bits (131072 columns, 64 experts, all weights: 31.7 us, with expf in
+// the sum 35.8; their 16-bit gradient 20.4, 24.6).
+__device__ __forceinline__ float near_best(float v, float best) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"((v - best) * 1.4426950408889634f));
   return v == best ? 1.0f : y;
@@ -86,10 +91,10 @@ __device__ __forceinline__ void scan_logits(const T* __restrict__ x, int64_t ld,
       float now = best;
 #pragma unroll
       for (int u = 0; u < kChunk; ++u) now = fmaxf(now, v[u]);
-      sum *= from_best(best, now);
+      sum *= near_best(best, now);
       best = now;
 #pragma unroll
-      for (int u = 0; u < kChunk; ++u) sum += from_best(v[u], best);
+      for (int u = 0; u < kChunk; ++u) sum += near_best(v[u], best);
     }
 #pragma unroll
     for (int u = 0; u < kChunk; ++u) {
@@ -151,7 +156,7 @@ __device__ __forceinline__ void choose(const T* __restrict__ x, int64_t ld, int 
       }
     }
     if (over_all) {
-      sum *= from_best(best, at_least_finite(top[0]));
+      sum *= near_best(best, at_least_finite(top[0]));
 #pragma unroll
       for (int d = 1; d < G; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     }
@@ -414,10 +419,11 @@ __global__ void __launch_bounds__(kBlock)
   const bool any = idx[0] >= 0;
   const float best = any && over_all ? as_logit(x[(int64_t)idx[0] * ld + b]) : 0.0f;
   const float scale = any ? -w[0] * mean : 0.0f;
+  auto term = [&](float v) { return sizeof(T) == 2 ? near_best(v, best) : from_best(v, best); };
 #pragma unroll
   for (int u = 0; u < kBackPart; ++u)
     if (e0 + u < experts)
-      dx[(e0 + u) * d_ld + b] = Num<T>::from_c(over_all && any ? from_best(as_logit(raw[u]), best) * scale : 0.0f);
+      dx[(e0 + u) * d_ld + b] = Num<T>::from_c(over_all && any ? term(as_logit(raw[u])) * scale : 0.0f);
 #pragma unroll
   for (int j = 0; j < K; ++j)
     if (idx[j] >= e0 && idx[j] < e0 + kBackPart) dx[(int64_t)idx[j] * d_ld + b] = Num<T>::from_c(g[j] - w[j] * mean);

@@ -262,3 +262,25 @@ def test_single_precision_silu(rows):
     assert ((y.double() - want).abs() <= 2.0 ** -17 * want.abs()).all()
     near = want[0, z > -1].abs()
     assert ((y[:, z > -1].double() - want[:, z > -1]).abs() <= 2.0 ** -21 * near + 2.0 ** -140).all()
+
+
+# ------------------------------------------------------------------- routing ----
+@pytest.mark.parametrize("experts,batch", [(2, 1), (3, 700), (6, 5000)])
+@pytest.mark.parametrize("normalise", ["selected", "all"])
+def test_routing_weights_far_below_the_best(experts, batch, normalise):
+    """Logits on a grid, so that their differences are exact.  exp is off by at most 2 units (2^-23), the sum of n by
+    2 + (n - 1) / 2, the quotient by 1/2; the gradient takes two weights, an exponential and four roundings."""
+    g = gen(batch)
+    x = torch.randint(-10_000, 10_000, (experts, batch), generator=g, device="cuda").float() / 256
+    k = experts if normalise == "selected" else 1
+    r = pb.route_columns(x, k, normalise=normalise)
+    p = torch.softmax(x.double(), 0)
+    weight = torch.gather(p, 0, r.expert.long())
+    unit, of_weight = 2.0 ** -23, 4 + experts / 2
+    assert ((r.weight.double() - weight).abs() <= of_weight * unit * weight + 2.0 ** -148).all()
+    if k == 1:
+        d_w = torch.randn(1, batch, generator=g, device="cuda")
+        d = pb.route_columns_backward(x, r, d_w, normalise="all")
+        other = torch.ones_like(x, dtype=torch.bool).scatter_(0, r.expert.long(), False)
+        want = -p * weight * d_w.double()
+        assert ((d.double() - want).abs() <= (2 * of_weight + 4) * unit * want.abs() + 2.0 ** -147)[other].all()
