@@ -19,8 +19,9 @@
 // contraction, so the last K block's are zeroed in shared memory (both
 // operands: the neighbour's values may be infinite).
 //
-// fp32 operands are split exactly into three bf16 parts x = x0 + x1 + x2 and six
-// products are kept (the three dropped are below 2^-24 of the magnitudes).  Each K
+// fp32 operands are split exactly into three bf16 parts x = x0 + x1 + x2, the nearest
+// each time, and six products are kept (x1 y2, x2 y1 and x2 y2 are dropped: together below 2^-23
+// of the magnitude, near 2^-25 on average, of either sign).  Each K
 // block of 64 goes into its own TMEM accumulator, the five small products first,
 // and is added to the tile's sum in fp32 registers: the tensor core truncates
 // when it accumulates, so long sums in TMEM drift by a part of 2^-24 for
@@ -1151,13 +1152,35 @@ struct Stages {
   int n;
 };
 
-// split3 of finite values; infinities and NaN stay whole in the first part.
-__device__ __forceinline__ void split_any(float x, uint32_t& h0, uint32_t& h1, uint32_t& h2) {
-  split3(x, h0, h1, h2);
-  if ((__float_as_uint(x) & 0x7F800000u) == 0x7F800000u) {
-    h0 = x != x ? 0x7FC00000u : h0;
-    h1 = h2 = 0u;
+// Parts of two values, packed (x in the lower halves): each part is the nearest bf16 value to
+// what the ones before leave, so that the products that are dropped are small and of either
+// sign (parts cut off instead are four times as far off, always towards zero).
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&h)[3]) {
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    h[q] = pack2(x, y, (__nv_bfloat16*)0);
+    if (q < 2) f2::sub(x, y, x, y, __uint_as_float(h[q] << 16), __uint_as_float(h[q] & 0xFFFF0000u));
   }
+}
+// What would round up past the largest bf16 is cut off in its first part; infinities and NaN
+// stay whole in it.
+constexpr uint32_t kLastRounded = 0x7F7F7FFFu;  // magnitude bits of the largest value that split_pair takes
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+__device__ __forceinline__ void split_extreme(float x, float y, uint32_t (&h)[3]) {
+  float v[2] = {x, y};
+  uint32_t first[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const bool finite = magnitude(v[i]) < 0x7F800000u;
+    first[i] = v[i] != v[i] ? 0x7FC00000u
+               : magnitude(v[i]) > kLastRounded ? __float_as_uint(v[i]) & 0xFFFF0000u
+                                                : (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v[i])) << 16;
+    v[i] = finite ? v[i] - __uint_as_float(first[i]) : 0.0f;
+  }
+  split_pair(v[0], v[1], h);
+  h[2] = h[1];
+  h[1] = h[0];
+  h[0] = pack_hi16(first[0], first[1]);
 }
 
 // A thread lays out 8 elements: one 16-byte store a plane.  (Two elements a thread,
@@ -1187,14 +1210,19 @@ __global__ void __launch_bounds__(256) stage_kernel(const Stages all) {
         for (int i = 0; i < 8; ++i) v[i] = c * 8 + i < s.cols ? __ldg(src + c * 8 + i) : Num<T>::from_c(0.0f);
       }
       if constexpr (sizeof(T) == 4) {
-        uint32_t h[3][8];
+        uint32_t h[4][3], most = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) split_any(v[i], h[0][i], h[1][i], h[2][i]);
+        for (int i = 0; i < 8; ++i) most = max(most, magnitude(v[i]));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split_pair(v[2 * i], v[2 * i + 1], h[i]);
+        if (most > kLastRounded) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) split_extreme(v[2 * i], v[2 * i + 1], h[i]);
+        }
         __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(s.dst) + r * s.pitch + c * 8;
 #pragma unroll
         for (int q = 0; q < 3; ++q)
-          *reinterpret_cast<uint4*>(dst + q * plane) = make_uint4(pack_hi16(h[q][0], h[q][1]), pack_hi16(h[q][2], h[q][3]),
-                                                                  pack_hi16(h[q][4], h[q][5]), pack_hi16(h[q][6], h[q][7]));
+          *reinterpret_cast<uint4*>(dst + q * plane) = make_uint4(h[0][q], h[1][q], h[2][q], h[3][q]);
       } else {
         *reinterpret_cast<uint4*>(static_cast<T*>(s.dst) + r * s.pitch + c * 8) = *reinterpret_cast<uint4*>(v);
       }

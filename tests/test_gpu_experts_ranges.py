@@ -284,3 +284,32 @@ def test_routing_weights_far_below_the_best(experts, batch, normalise):
         other = torch.ones_like(x, dtype=torch.bool).scatter_(0, r.expert.long(), False)
         want = -p * weight * d_w.double()
         assert ((d.double() - want).abs() <= (2 * of_weight + 4) * unit * want.abs() + 2.0 ** -147)[other].all()
+
+
+# --------------------------------------------------------- parts of fp32 values ----
+def test_single_precision_parts_are_the_nearest():
+    """Factors just below two: cut-off parts would lose 2^-23 of every product, the nearest ones (2 - 2^-23) nothing."""
+    value = 2.0 - 2.0 ** -23
+    x = torch.full((600, 16), value, device="cuda")
+    x[::2] *= -1
+    w = torch.full((2, 16, 130), value, device="cuda")
+    off = offsets([400, 200])
+    want = (x.double() @ w[0].double()).float()
+    assert torch.equal(pb.expert_product(x, w, off), want)
+    d = torch.full((600, 130), value, device="cuda")
+    dr, dw, _ = pb.expert_product_backward(d[:, :16].contiguous(), x, w[:, :, :16].contiguous(), off)
+    assert torch.equal(dr, torch.full_like(dr, 64.0 - 2.0 ** -17))
+    assert not dw.any()  # (as many rows of either sign)
+    pb.check_operators()
+
+
+def test_single_precision_ends_of_the_range():
+    """Values that round up past the largest bf16, subnormal ones and zeros, times one; parts of a product of them."""
+    top = torch.finfo(torch.float32).max
+    v = torch.tensor([top, -top, top * (1 - 2.0 ** -9), top * (1 - 2.0 ** -10), 3.3961775e38, 0.0, -0.0, 1.0 + 2.0 ** -23,
+                      2.0 ** -100 * (2 - 2.0 ** -23)], device="cuda")
+    x = v.view(-1, 1).repeat(100, 1)
+    w = torch.ones(1, 1, 24, device="cuda")
+    assert torch.equal(pb.expert_product(x, w, offsets([len(x)])), x.expand(-1, 24))
+    w[..., 1::2] = 0.5
+    assert torch.equal(pb.expert_product(x, w, offsets([len(x)])), x * w[0])
