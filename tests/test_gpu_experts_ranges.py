@@ -313,3 +313,65 @@ def test_single_precision_ends_of_the_range():
     assert torch.equal(pb.expert_product(x, w, offsets([len(x)])), x.expand(-1, 24))
     w[..., 1::2] = 0.5
     assert torch.equal(pb.expert_product(x, w, offsets([len(x)])), x * w[0])
+
+
+# --------------------------------------------------- NaN and infinity in fp32 ----
+@pytest.mark.parametrize("counts", [[150, 0, 300, 40], [9000, 8000]])
+def test_single_precision_nan_and_infinity(counts):
+    """Wherever they stand, results are NaN, infinite or finite as in plain arithmetic."""
+    g = gen(len(counts))
+    experts, n, off = len(counts), sum(counts), offsets(counts)
+    inputs, outputs = 200, 130
+    rows, w, d = randn(g, n, inputs), randn(g, experts, inputs, outputs) * inputs ** -0.5, randn(g, n, outputs)
+    w[0, 5] = 1.0  # (parts that are zero)
+    inf, nan = float("inf"), float("nan")
+    rows[3, 5], rows[7, 9], rows[20, 5], rows[21, 0], rows[n - 1, 5] = inf, nan, -inf, 0.0, inf
+    rows[20, 6] = nan
+    w[0, 7, 11], w[-1, 0, 3], w[-1, 1, 3], w[0, 8, 12] = inf, inf, -inf, nan
+    d[2, 5], d[30, 60], d[31, 60], d[n - 3, 129] = -inf, inf, nan, inf
+    y, (dr, dw, db) = pb.expert_product(rows, w, off), pb.expert_product_backward(d, rows, w, off)
+    want, size = R.product(rows, w, off)
+    grads = R.product_gradient(d, rows, w, off)
+    for got, ref, mag, terms in ((y, want, size, inputs), (dr, *grads[0], outputs), (dw, *grads[1], max(counts)),
+                                 (db, *grads[2], max(counts))):
+        assert torch.equal(torch.isnan(got), torch.isnan(ref))
+        infinite = torch.isinf(ref)
+        assert torch.equal(got[infinite].double(), ref[infinite]) and torch.equal(torch.isinf(got), infinite)
+        fine = torch.isfinite(ref)
+        R.check_sum(got[fine], ref[fine], mag[fine], terms)
+    pb.check_operators()
+
+
+def test_single_precision_long_sums_with_nan_and_infinity_end_in_time():
+    """65536 terms in pairs of CTAs: no role's bounded wait runs out while a tile is summed again."""
+    n, terms, outputs = 8400, 65536, 250
+    g = gen(1)
+    x, w = randn(g, n, terms), randn(g, 1, terms, outputs)
+    w[0, 0] = 1.0
+    x[:, -1] = 0.0
+    x[5, 0], x[300:330, 0], x[8000, 7] = float("inf"), float("-inf"), float("nan")
+    y = pb.expert_product(x, w, offsets([n]))
+    pb.check_operators()
+    assert (y[5] == float("inf")).all() and (y[300:330] == float("-inf")).all() and torch.isnan(y[8000]).all()
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[5], keep[300:330], keep[8000] = False, False, False
+    assert torch.isfinite(y[keep]).all()
+
+
+def test_single_precision_nan_costs_little():
+    g = gen(2)
+    x, w, off = randn(g, 8192, 1024), randn(g, 1, 1024, 1024), offsets([8192])
+
+    def time(x):
+        pb.expert_product(x, w, off)
+        begin, end = torch.cuda.Event(True), torch.cuda.Event(True)
+        begin.record()
+        for _ in range(3):
+            pb.expert_product(x, w, off)
+        end.record()
+        end.synchronize()
+        return begin.elapsed_time(end)
+
+    bad = x.clone()
+    bad[:, -1] = float("nan")
+    assert time(bad) < 30 * time(x)  # (a sum one by one for every value that is NaN: 280 times)
