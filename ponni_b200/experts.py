@@ -86,6 +86,34 @@ def _like(t, shape, dtype, device, what: str):
         _refuse(f"{what} must be a dense {dtype} tensor of shape {tuple(shape)} on {device}")
 
 
+def _span(t):
+    """Addresses from the first element to behind the last one."""
+    at = t.data_ptr()
+    return at, at + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def _check_apart(out, *inputs):
+    """Refuses an output that shares elements with an input (the kernels read and write in no order).
+
+    Column ranges of one buffer side by side, with the same row stride, are apart.
+    """
+    if out.numel() == 0:
+        return
+    lo, hi = _span(out)
+    for t in inputs:
+        if t is None or t.numel() == 0:
+            continue
+        a, b = _span(t)
+        if a >= hi or b <= lo:
+            continue
+        z, ld = out.element_size(), out.stride(0)
+        if t.dim() == 2 and t.element_size() == z and t.stride(0) == ld and (a - lo) % z == 0:
+            at = (a - lo) // z % ld
+            if at >= out.shape[1] and at + t.shape[1] <= ld:
+                continue
+        _refuse("out overlaps an input")
+
+
 class Routing(NamedTuple):
     """What route_columns decides.
 
@@ -193,7 +221,9 @@ def gather_columns(x, routing: Routing, out=None):
     features, batch = x.shape
     dev = x.device
     top_k = _check_routing(routing, dev, batch)
-    out = _row_output(out, batch * top_k, features, x)
+    given, out = out, _row_output(out, batch * top_k, features, x)
+    if given is not None:
+        _check_apart(out, x, routing.row, routing.offset)
     _call(_abi.lib().ponni_b200_gather_columns(
         code, x.data_ptr(), ld, features, batch, top_k, routing.row.data_ptr(),
         routing.offset.data_ptr() + 4 * (routing.offset.numel() - 1), out.data_ptr(), _matrix(out, "out"), dev.index,
@@ -210,7 +240,9 @@ def _combine(rows, routing, weight, out):
     top_k = _check_routing(routing, dev, batch)
     if total != batch * top_k:
         _refuse(f"the routing has {batch * top_k} rows, not {total}", 2)
-    out = _output(out, (features, batch), rows, "out")
+    given, out = out, _output(out, (features, batch), rows, "out")
+    if given is not None:
+        _check_apart(out, rows, routing.row, routing.weight)
     _call(_abi.lib().ponni_b200_combine_rows(code, rows.data_ptr(), ld, features, batch, top_k, routing.row.data_ptr(),
                                              weight, out.data_ptr(), _matrix(out, "out"), dev.index,
                                              torch_stream_handle(dev)))
@@ -311,7 +343,9 @@ def expert_product(rows, weights, offset, bias=None, activation: Layer | None = 
         if activation.num_outputs != outputs:
             _refuse(f"the activation has {activation.num_outputs} features, the product {outputs} outputs", 2)
         kind, flags, s0, s1 = activation.kind, activation.flags, activation.scalar[0], activation.scalar[1]
-    out = _row_output(out, total, outputs, rows)
+    given, out = out, _row_output(out, total, outputs, rows)
+    if given is not None:
+        _check_apart(out, rows, weights, bias, offset)
     L = _abi.lib()
     x, w = rows.data_ptr(), weights.data_ptr()
     space, need, at = _space(L, code, total, experts, inputs, outputs, x | w, ld | w_ld | stride, 0, dev)

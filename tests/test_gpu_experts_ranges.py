@@ -375,3 +375,40 @@ def test_single_precision_nan_costs_little():
     bad = x.clone()
     bad[:, -1] = float("nan")
     assert time(bad) < 30 * time(x)  # (a sum one by one for every value that is NaN: 280 times)
+
+
+# -------------------------------------------------------------- shared memory ----
+def test_outputs_that_overlap_inputs_are_refused():
+    g = gen(1)
+    rows, w, off = randn(g, 300, 64), randn(g, 2, 64, 64), offsets([100, 200])
+    r = pb.route_columns(randn(g, 2, 64), 1)
+    x = randn(g, 64, 64)
+    buf = randn(g, 300, 100)
+    for f in (lambda: pb.expert_product(rows, w, off, out=rows),
+              lambda: pb.expert_product(rows[:200], w, offsets([100, 100]), out=rows[100:]),
+              lambda: pb.expert_product(buf[:, :64], w, off, out=buf[:, 36:]),
+              lambda: pb.expert_product(rows[:128], w, offsets([100, 28]), out=w.view(128, 64)),
+              lambda: pb.gather_columns(x, r, out=x),
+              lambda: pb.combine_rows(x, r, out=x),
+              lambda: pb.gather_columns_backward(x, r, out=x)):
+        with pytest.raises(pb.PonniError, match="overlaps"):
+            f()
+    assert torch.equal(pb.gather_columns(x, r).double(), R.gather(x, r.row))
+
+
+def test_outputs_beside_inputs_are_not():
+    """Columns of one buffer side by side, and rows of one buffer one behind the other."""
+    g = gen(2)
+    w, off = randn(g, 2, 64, 64), offsets([100, 200])
+    buf = randn(g, 300, 130)
+    x = buf[:, 1:65].clone()
+    out = buf[:, 66:]
+    assert pb.expert_product(buf[:, 1:65], w, off, out=out) is out
+    want, size = R.product(x, w, off)
+    R.check_sum(out, want, size, 64)
+    assert torch.equal(buf[:, 1:65], x)
+    buf = randn(g, 600, 64)
+    x = buf[300:].clone()
+    pb.expert_product(buf[300:], w, off, out=buf[:300])
+    want, size = R.product(x, w, off)
+    R.check_sum(buf[:300], want, size, 64)
