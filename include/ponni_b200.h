@@ -442,7 +442,9 @@ int64_t ponni_b200_gradient_set_workspace(const ponni_b200_gradient_set* set);
  * else the (scaled) gradients are written to flat, gradient_set_count values
  * of flat_dtype in tensor order -- the order of
  * ponni_b200_set_trainable_parameters_device -- and stay as they are
- * themselves. */
+ * themselves.  Tensors of the set may overlap only where they are packed; flat
+ * may overlap a tensor only where that is the very place of its values (a view
+ * of flat), and they are then scaled there. */
 ponni_b200_status ponni_b200_gradient_set_clip(ponni_b200_gradient_set* set, double max_norm, void* flat, int flat_dtype,
                                                float* norm, void* workspace, int64_t workspace_bytes, void* stream);
 

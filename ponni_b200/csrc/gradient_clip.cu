@@ -21,16 +21,25 @@
 #include <algorithm>
 #include <new>
 #include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "device_math.cuh"
 #include "operators.h"
 
 struct ponni_b200_gradient_set {
+  // A tensor's addresses, type and place in the packed vector.
+  struct Extent {
+    uintptr_t begin, end, reach;  // reach: the largest end up to here
+    int64_t flat;
+    int32_t dtype;
+  };
   int device = 0;
   int64_t total = 0;
   int64_t num_chunks = 0;
-  void* chunks = nullptr;  // device table
+  void* chunks = nullptr;       // device table
+  std::vector<Extent> extents;  // by address
+  bool overlap = false;         // two of them share elements
 };
 
 namespace ponni_b200 {
@@ -215,7 +224,7 @@ __device__ __forceinline__ void clip_chunks(const Chunk* __restrict__ chunks, in
 
 __global__ void __launch_bounds__(kBlock)
     clip_kernel(const Chunk* __restrict__ chunks, int64_t num_chunks, const double* __restrict__ partial,
-                int num_partial, double max_norm, void* __restrict__ flat, int flat_dtype, float* __restrict__ norm_out) {
+                int num_partial, double max_norm, void* flat, int flat_dtype, float* __restrict__ norm_out) {
   __shared__ double sums[kBlock / 32];
   ops::let_successor_start();
   ops::wait_for_predecessor();
@@ -232,7 +241,7 @@ __global__ void __launch_bounds__(kBlock)
 constexpr int kCluster = 8, kOneClusterChunks = 4 * kCluster;
 __global__ void __launch_bounds__(kBlock)
     clip_one_cluster_kernel(const Chunk* __restrict__ chunks, int64_t num_chunks, double max_norm,
-                            void* __restrict__ flat, int flat_dtype, float* __restrict__ norm_out) {
+                            void* flat, int flat_dtype, float* __restrict__ norm_out) {
   __shared__ double sums[kBlock / 32];
   __shared__ double mine;
   const double t = block_sum(chunk_squares(chunks, num_chunks), sums);
@@ -250,6 +259,17 @@ __global__ void __launch_bounds__(kBlock)
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
   clip_chunks(chunks, num_chunks, norm, max_norm, flat, flat_dtype);
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;\n" ::: "memory");
+}
+
+// Whether the packed vector shares no element with a tensor, or the tensor lies in it just
+// where its packed values go (gradients that are views of one vector): a thread then
+// writes what it has read.
+bool packs_apart(const ponni_b200_gradient_set& set, const void* flat, int flat_dtype) {
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(flat), z = ops::element_bytes(flat_dtype), hi = lo + set.total * z;
+  auto at = std::partition_point(set.extents.begin(), set.extents.end(), [&](const auto& x) { return x.reach <= lo; });
+  for (; at != set.extents.end() && at->begin < hi; ++at)
+    if (at->end > lo && (at->dtype != flat_dtype || at->begin != lo + at->flat * z)) return false;
+  return true;
 }
 
 }  // namespace
@@ -280,19 +300,31 @@ ponni_b200_status ponni_b200_gradient_set_create(const void* const* tensors, con
     // About eight chunks a block, 2048 to 16384 elements each.
     const int64_t per = std::min<int64_t>(16384, std::max<int64_t>(2048, total / (kMaxBlocks * 8) / 512 * 512));
     std::vector<Chunk> table;
+    std::vector<ponni_b200_gradient_set::Extent> extents;
     int64_t flat = 0;
     for (int i = 0; i < num_tensors; ++i) {
       const int64_t z = ops::element_bytes(dtypes[i]);
       for (int64_t at = 0; at < counts[i]; at += per)
         table.push_back({static_cast<char*>(const_cast<void*>(tensors[i])) + at * z, flat + at,
                          (int32_t)std::min(per, counts[i] - at), dtypes[i]});
+      const uintptr_t begin = reinterpret_cast<uintptr_t>(tensors[i]);
+      if (counts[i]) extents.push_back({begin, begin + (uintptr_t)(counts[i] * z), 0, flat, dtypes[i]});
       flat += counts[i];
+    }
+    std::sort(extents.begin(), extents.end(), [](const auto& a, const auto& b) { return a.begin < b.begin; });
+    bool overlap = false;
+    uintptr_t reach = 0;
+    for (auto& x : extents) {
+      overlap |= x.begin < reach;
+      x.reach = reach = std::max(reach, x.end);
     }
     ponni_b200_gradient_set* set = new (std::nothrow) ponni_b200_gradient_set;
     if (!set) return ops::fail(PONNI_B200_ERR_CUDA, "gradient set: out of host memory");
     set->device = device;
     set->total = total;
     set->num_chunks = (int64_t)table.size();
+    set->extents = std::move(extents);
+    set->overlap = overlap;
     if (!table.empty()) {
       cudaError_t e = cudaMalloc(&set->chunks, table.size() * sizeof(Chunk));
       // (A plain copy from pageable memory returns once the table is staged, and a stream that
@@ -338,6 +370,10 @@ ponni_b200_status ponni_b200_gradient_set_clip(ponni_b200_gradient_set* set, dou
       return ops::fail(PONNI_B200_ERR_UNSUPPORTED, "clip: the packed vector must be fp32, fp64, fp16 or bf16");
     if (flat && !ops::aligned_to(ops::element_bytes(flat_dtype), flat))
       return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "clip: the packed vector is not aligned to its type");
+    if (!flat && set->overlap)
+      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "clip: tensors of the set overlap, which only a packed vector allows");
+    if (flat && !packs_apart(*set, flat, flat_dtype))
+      return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "clip: the packed vector overlaps a tensor of the set");
     if (!workspace || workspace_bytes < ponni_b200_gradient_set_workspace(set) ||
         reinterpret_cast<uintptr_t>(workspace) % 8 != 0)
       return ops::fail(PONNI_B200_ERR_INVALID_ARGUMENT, "clip: workspace is too small or not aligned to 8 bytes");

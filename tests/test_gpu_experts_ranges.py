@@ -412,3 +412,17 @@ def test_outputs_beside_inputs_are_not():
     pb.expert_product(buf[300:], w, off, out=buf[:300])
     want, size = R.product(x, w, off)
     R.check_sum(buf[:300], want, size, 64)
+
+
+@pytest.mark.parametrize("sizes", [[5, 1000, 3], [100_001, 70_000, 2_000_003]])
+def test_clip_of_views_of_the_packed_vector(sizes):
+    flat = randn(gen(5), sum(sizes))
+    keep = flat.double()
+    parts = list(flat.split(sizes))
+    norm = pb.clip_gradients(parts, 0.25, out=flat)
+    assert abs(norm.item() - keep.norm().item()) <= 2.0 ** -22 * keep.norm().item()
+    assert ((flat.double() - keep * 0.25 / keep.norm()).abs() <= 2.0 ** -21 * keep.abs() * 0.25 / keep.norm()).all()
+    with pytest.raises(pb.PonniError, match="overlap"):
+        pb.clip_gradients([parts[0], flat], 0.25)
+    with pytest.raises(pb.PonniError, match="overlaps"):
+        pb.clip_gradients(parts[::-1], 0.25, out=flat)
