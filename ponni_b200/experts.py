@@ -133,8 +133,10 @@ def _check_routing(r: Routing, device, batch: int):
     torch = _torch()
     shape = r.row.shape
     if len(shape) != 2 or shape[1] != batch:
-        _refuse(f"the routing is for {shape[-1]} columns, not {batch}", 2)
+        _refuse(f"the routing has rows of shape {tuple(shape)}, not of {batch} columns", 2)
     _like(r.row, shape, torch.int32, device, "routing.row")
+    if r.offset.dim() != 1 or r.offset.numel() < 2:  # its last entry is read on the device
+        _refuse(f"routing.offset has shape {tuple(r.offset.shape)}, not [experts + 1]", 2)
     _like(r.offset, r.offset.shape, torch.int32, device, "routing.offset")
     return shape[0]
 
@@ -236,7 +238,7 @@ def _combine(rows, routing, weight, out):
     ld = _matrix(rows, "rows")
     total, features = rows.shape
     dev = rows.device
-    batch = routing.row.shape[-1]
+    batch = routing.row.shape[-1] if routing.row.dim() else 0
     top_k = _check_routing(routing, dev, batch)
     if total != batch * top_k:
         _refuse(f"the routing has {batch * top_k} rows, not {total}", 2)

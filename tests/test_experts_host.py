@@ -71,3 +71,16 @@ def test_plain_gradient_by_differences():
             up, down = R.route(x + step, 3, normalise), R.route(x - step, 3, normalise)
             assert torch.equal(up[0], expert) and torch.equal(down[0], expert)
             assert torch.allclose(((up[1] - down[1]) * d).sum(0) / 2e-5, grad[e], atol=1e-8)
+
+
+def test_routings_of_a_wrong_shape_are_refused():
+    """The checks themselves, on host tensors (the entry points refuse those before)."""
+    from ponni_b200 import experts as X
+    row, none = torch.zeros(2, 6, dtype=torch.int32), torch.zeros(0, dtype=torch.int32)
+    good = pb.Routing(row, row.float(), row, row.view(-1), torch.zeros(5, dtype=torch.int32))
+    assert X._check_routing(good, row.device, 6) == 2
+    for bad in (good._replace(offset=none), good._replace(offset=none.view(0, 1)), good._replace(offset=good.offset[:1]),
+                good._replace(offset=good.offset[0]), good._replace(offset=good.offset.view(5, 1)),
+                good._replace(row=row[0]), good._replace(row=row[0, 0]), good._replace(row=row.long())):
+        with pytest.raises(pb.PonniError):
+            X._check_routing(bad, row.device, 6)

@@ -426,3 +426,15 @@ def test_clip_of_views_of_the_packed_vector(sizes):
         pb.clip_gradients([parts[0], flat], 0.25)
     with pytest.raises(pb.PonniError, match="overlaps"):
         pb.clip_gradients(parts[::-1], 0.25, out=flat)
+
+
+def test_routings_without_offsets_are_refused():
+    x = torch.randn(4, 10, device="cuda")
+    r = pb.route_columns(x, 2)
+    rows = torch.zeros(20, 4, device="cuda")
+    for bad in (r._replace(offset=r.offset[:0]), r._replace(offset=r.offset[:1]), r._replace(row=r.row[0]),
+                r._replace(row=r.row[0, 0])):
+        for f in (lambda: pb.gather_columns(x, bad), lambda: pb.combine_rows_backward(x, rows, bad)):
+            with pytest.raises(pb.PonniError):
+                f()
+    pb.check_operators()
