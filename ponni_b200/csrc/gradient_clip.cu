@@ -142,15 +142,29 @@ __global__ void __launch_bounds__(kBlock)
   if (threadIdx.x == 0) partial[blockIdx.x] = t;
 }
 
+// The factor, and as two of fp32: one far below 1 (a norm of 1e38 and more) would lose its
+// precision below fp32's normal range or be zero, so 2^100 of it are taken off and put
+// back behind the first product, which stays in range.
+struct Scale {
+  double exact;
+  float first, second;
+  __device__ explicit Scale(double s) : exact(s), first((float)s), second(1.0f) {
+    if (s < 0x1p-100) {
+      first = (float)(s * 0x1p100);
+      second = 0x1p-100f;
+    }
+  }
+};
+
 template <class T, class O>
-__device__ __forceinline__ O scaled(T x, double scale) {
-  if constexpr (sizeof(T) == 8) return (O)Num<O>::from_c((typename Num<O>::C)((double)x * scale));
-  else if constexpr (sizeof(O) == 8) return (double)Num<T>::to_c(x) * scale;
-  else return Num<O>::from_c(Num<T>::to_c(x) * (float)scale);
+__device__ __forceinline__ O scaled(T x, const Scale& scale) {
+  if constexpr (sizeof(T) == 8) return (O)Num<O>::from_c((typename Num<O>::C)((double)x * scale.exact));
+  else if constexpr (sizeof(O) == 8) return (double)Num<T>::to_c(x) * scale.exact;
+  else return Num<O>::from_c(Num<T>::to_c(x) * scale.first * scale.second);
 }
 
 template <class T, class O>
-__device__ __forceinline__ void rescale(const T* p, O* out, int count, double scale) {
+__device__ __forceinline__ void rescale(const T* p, O* out, int count, const Scale& scale) {
   constexpr int n = Vec<T>::n;
   int done = 0;
   if (sizeof(T) == sizeof(O) && reinterpret_cast<uintptr_t>(p) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
@@ -194,7 +208,7 @@ __device__ __forceinline__ void rescale(const T* p, O* out, int count, double sc
 
 // flat_dtype < 0: in place.
 template <class T>
-__device__ __forceinline__ void rescale_to(const Chunk& c, void* flat, int flat_dtype, double scale) {
+__device__ __forceinline__ void rescale_to(const Chunk& c, void* flat, int flat_dtype, const Scale& scale) {
   const T* p = static_cast<const T*>(c.p);
   switch (flat_dtype) {
     case PONNI_B200_F32: rescale(p, static_cast<float*>(flat) + c.flat, c.count, scale); break;
@@ -210,7 +224,7 @@ __device__ __forceinline__ void clip_chunks(const Chunk* __restrict__ chunks, in
                                             double max_norm, void* flat, int flat_dtype) {
   const bool clip = norm > max_norm && norm < (double)INFINITY;
   if (!clip && flat_dtype < 0) return;
-  const double scale = clip ? max_norm / norm : 1.0;
+  const Scale scale(clip ? max_norm / norm : 1.0);
   for (int64_t i = num_chunks - 1 - blockIdx.x; i >= 0; i -= gridDim.x) {
     const Chunk c = chunks[i];
     switch (c.dtype) {

@@ -438,3 +438,20 @@ def test_routings_without_offsets_are_refused():
             with pytest.raises(pb.PonniError):
                 f()
     pb.check_operators()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("max_norm", [1.0, 1e-4, 1e-9])
+def test_clip_of_gradients_near_the_largest_value(dt, max_norm):
+    """A factor below fp32's normal range: it is held to a unit of fp32, and the product another."""
+    for n in (1000, 3_000_000):
+        x = (torch.rand(n, generator=gen(n), device="cuda") * 3e38).to(DT[dt])
+        keep = x.double()
+        want = keep * (max_norm / keep.norm())
+        ok = want.abs() >= 2.0 ** -120  # (below, fp32 itself has fewer digits)
+        out = torch.empty(n, dtype=DT[dt], device="cuda")
+        pb.clip_gradients([x], max_norm, out=out)
+        assert ok.sum() > n // 2
+        assert ((out.double() - want).abs() <= (R.ULP[x.dtype] + 2.0 ** -22) * want.abs())[ok].all()
+        pb.clip_gradients([x], max_norm)
+        assert torch.equal(x, out)
