@@ -1107,19 +1107,19 @@ __global__ void __launch_bounds__(256)
   const int64_t most = slots(rows, unit_rows, experts);  // (offsets out of order would give more)
   ops::wait_for_predecessor();
   const int e = blockIdx.y;
-  auto units = [&](int i) {
+  auto units_of = [&](int i) {
     const int l = clamped(offset[i], 0, rows);
-    return (clamped(offset[i + 1], l, rows) - l + unit_rows - 1) / unit_rows;
+    return units(clamped(offset[i + 1], l, rows) - l, unit_rows);
   };
   if (threadIdx.x < 32) {
     int64_t n = 0;
-    for (int i = threadIdx.x; i < e; i += 32) n += units(i);
+    for (int i = threadIdx.x; i < e; i += 32) n += units_of(i);
     for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
     if (threadIdx.x == 0) first_s = n;
   }
   __syncthreads();
   const int64_t first = min(first_s, most);
-  const int n = (int)min((int64_t)units(e), most - first);
+  const int n = (int)min(units_of(e), most - first);
   const float* src = partial + first * per_expert;
   for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < per_expert; i += (int64_t)gridDim.x * 256) {
     float s = 0.0f;

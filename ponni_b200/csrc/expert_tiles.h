@@ -37,6 +37,8 @@ PONNI_B200_HD void ascending(int* edge, int experts) {
   for (int e = 1; e <= experts; ++e)
     if (edge[e] < edge[e - 1]) edge[e] = edge[e - 1];
 }
+// Units of a group (the sum of both may pass 2^31).
+PONNI_B200_HD int64_t units(int64_t rows, int64_t unit_rows) { return (rows + unit_rows - 1) / unit_rows; }
 // Units of all groups at most: every group's last one may be short.
 PONNI_B200_HD int64_t slots(int64_t rows, int unit_rows, int experts) { return rows / unit_rows + experts; }
 
@@ -59,7 +61,7 @@ template <int MODE, int BN, int CG> struct Tiles {
   PONNI_B200_HD int64_t count(int i) const {
     const int rows = edge[i + 1] - edge[i];
     if (MODE != kWeights) return (int64_t)((rows + CG * kBM - 1) / (CG * kBM)) * n_tiles;
-    return (int64_t)(unit_rows ? (rows + unit_rows - 1) / unit_rows : 1) * m_tiles * n_tiles;
+    return (unit_rows ? units(rows, unit_rows) : 1) * m_tiles * n_tiles;
   }
   PONNI_B200_HD bool next(Tile& v) {
     int64_t c = 0;
@@ -86,7 +88,7 @@ template <int MODE, int BN, int CG> struct Tiles {
       v.slot = base / per + unit;
       if (unit_rows) {
         v.lo += unit * unit_rows;
-        if (v.hi > v.lo + unit_rows) v.hi = v.lo + unit_rows;
+        if (v.hi - v.lo > unit_rows) v.hi = v.lo + unit_rows;  // (their sum may pass 2^31)
       }
       v.k_blocks = (v.hi - v.lo + kBK - 1) / kBK;
     }

@@ -147,6 +147,21 @@ static void offsets_out_of_order() {
       }
 }
 
+// Groups near the largest number of rows, in long units.
+static void long_groups() {
+  const int most = INT32_MAX - 65536, unit = 715000000 / kBK * kBK;
+  const Groups g = {0, 100, 1900000000, most};
+  Tiles<kWeights, 128, 1> tiles({3, 128, 128, unit}, g.data(), 0, 1, 0);
+  Tile v;
+  int64_t rows = 0;
+  while (tiles.next(v)) {
+    CHECK(v.lo >= g[v.e] && v.lo < v.hi && v.hi <= g[v.e + 1] && v.hi - v.lo <= unit, "rows %d to %d", v.lo, v.hi);
+    CHECK(v.k_blocks == (v.hi - v.lo + kBK - 1) / kBK, "%d blocks", v.k_blocks);
+    rows += v.hi - v.lo;
+  }
+  CHECK(rows == most, "%lld rows", (long long)rows);
+}
+
 // Every launch asks for no more than the kernel is allowed, for every number of experts:
 // stages of 24 to 96 KB (tile shapes), staging of 24, 32 and 64 KB, a bias strip a warp.
 static void memory() {
@@ -163,6 +178,7 @@ static void memory() {
 int main() {
   memory();
   offsets_out_of_order();
+  long_groups();
   empty_groups();
   cover();
   if (failures) std::printf("%d failures\n", failures);
