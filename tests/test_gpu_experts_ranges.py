@@ -455,3 +455,112 @@ def test_clip_of_gradients_near_the_largest_value(dt, max_norm):
         assert ((out.double() - want).abs() <= (R.ULP[x.dtype] + 2.0 ** -22) * want.abs())[ok].all()
         pb.clip_gradients([x], max_norm)
         assert torch.equal(x, out)
+
+
+# ------------------------------------------------------ long groups, exactly ----
+@pytest.mark.parametrize("inputs,outputs", [(200, 24), (24, 200), (40, 40), (1200, 37), (128, 128), (72, 300), (520, 260)])
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_long_groups_exactly(inputs, outputs, dt):
+    """Many tiles a CTA and weight gradients in units: no row lost, none taken twice, none of the next group's.
+
+    Sums of up to 40100 products of -1, 0 and 1 are exact in fp32 (and 16-bit rows of at most 1200 terms
+    of them before their rounding)."""
+    g = gen(inputs + outputs)
+    dtype, counts = DT[dt], [30_011, 0, 17_000, 129, 40_100, 1, 1024, 2047]
+    n, off = sum(counts) + 5, offsets(counts)
+    rows, w, d = (integers(g, *s, dtype=dtype, most=1) for s in ((n, inputs), (len(counts), inputs, outputs), (n, outputs)))
+    b = integers(g, len(counts), outputs, dtype=dtype)
+    want, _ = R.product(rows, w, off, b)
+    assert torch.equal(pb.expert_product(rows, w, off, bias=b), want.to(dtype))
+    for got, (want, _) in zip(pb.expert_product_backward(d, rows, w, off), R.product_gradient(d, rows, w, off)):
+        assert torch.equal(got, want.to(dtype))
+    pb.check_operators()
+
+
+@pytest.mark.parametrize("total", [1, 63, 64, 65, 4095, 4096, 4097, 20_000, 50_001])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_edges_of_units_exactly(total, dt):
+    """Rows that are not zero only beside the edges of K blocks and groups, each with a value of its own."""
+    dtype, f = DT[dt], 130
+    counts = [total, 7, total // 3]
+    n, off = sum(counts), offsets(counts)
+    at = torch.arange(n, device="cuda")
+    in_group = torch.cat([torch.arange(c, device="cuda") for c in counts])
+    marked = ((in_group % 64 < 2) | (in_group % 64 > 61)).to(dtype)[:, None]
+    rows = marked * (1 + at[:, None] % 3).to(dtype) * torch.ones(n, f, dtype=dtype, device="cuda")
+    d = marked * (1 + (at[:, None] // 3 + torch.arange(f, device="cuda")) % 2).to(dtype)
+    w = torch.zeros(3, f, f, dtype=dtype, device="cuda")
+    _, dw, db = pb.expert_product_backward(d, rows, w, off, need_rows=False)
+    assert torch.equal(dw, exact_weights(d, rows, counts).to(dtype))
+    assert torch.equal(db, exact_weights(d, torch.ones(n, 1, dtype=dtype, device="cuda"), counts)[:, 0].to(dtype))
+
+
+def test_past_32_bit_offsets_exactly():
+    """More than 2^31 elements of rows and of gradients; rows that are not zero on both sides of that element."""
+    n, f = 9_000_000, 256
+    g = gen(3)
+    rows, d = (torch.zeros(n, f, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    edge = 2 ** 31 // f
+    marked = [slice(0, 100), slice(edge - 150, edge + 150), slice(n - 300, n)]
+    for s in marked:
+        rows[s], d[s] = (integers(g, s.stop - s.start, f, dtype=torch.bfloat16) for _ in range(2))
+    w = integers(g, 2, f, f, dtype=torch.bfloat16)
+    counts = [n - 200, 200]
+    off = offsets(counts)
+    y = pb.expert_product(rows, w, off)
+    dr, dw, db = pb.expert_product_backward(d, rows, w, off)
+    want_w, want_b = torch.zeros(2, f, f, dtype=torch.float64, device="cuda"), torch.zeros(2, f, dtype=torch.float64, device="cuda")
+    for s in marked:
+        for e, (lo, hi) in enumerate(((0, n - 200), (n - 200, n))):
+            a, b = max(s.start, lo), min(s.stop, hi)
+            if a < b:
+                x, u = rows[a:b].double(), d[a:b].double()
+                assert torch.equal(y[a:b], (x @ w[e].double()).bfloat16())
+                assert torch.equal(dr[a:b], (u @ w[e].double().t()).bfloat16())
+                want_w[e] += x.t() @ u
+                want_b[e] += u.sum(0)
+    assert torch.equal(dw, want_w.bfloat16()) and torch.equal(db, want_b.bfloat16())
+    for t in (y, dr):
+        assert torch.count_nonzero(t[100:edge - 150]) == 0 and torch.count_nonzero(t[edge + 150:n - 300]) == 0
+    pb.check_operators()
+
+
+def test_columns_past_32_bit_offsets():
+    """More than 2^31 elements on either side: a column's two rows, added up, are twice the column."""
+    features, batch = 600, 3_700_000
+    g = gen(6)
+    x = integers(g, features, batch, dtype=torch.bfloat16, most=100)
+    r = pb.route_columns(randn(g, 4, batch), 2)
+    rows = pb.gather_columns(x, r)
+    assert rows.shape[0] * rows.stride(0) > 2 ** 32
+    for at in (0, batch // 2, batch - 1):
+        for j in range(2):
+            assert torch.equal(rows[r.row[j, at].long()], x[:, at])
+    assert torch.equal(pb.gather_columns_backward(rows, r), 2 * x)
+    even = r._replace(weight=torch.full_like(r.weight, 0.5))
+    assert torch.equal(pb.combine_rows(rows, even), x)
+    d_rows, d_weight = pb.combine_rows_backward(x, rows, even)
+    assert torch.equal(d_rows, rows * 0.5)
+    want = x[:, -1000:].double().square().sum(0)  # at most 600 * 100^2: exact in fp32
+    assert torch.equal(d_weight[:, -1000:].double(), want.expand(2, -1))
+
+
+def test_routing_past_32_bit_offsets():
+    experts, batch = 1024, 2_200_000
+    g = gen(7)
+    x = torch.randn(experts, batch, generator=g, device="cuda", dtype=torch.float16)
+    assert x.numel() > 2 ** 31
+    r = pb.route_columns(x, 1, normalise="all")
+    tail = x[:, -2000:].float()
+    best = tail.max(0).values
+    first = (tail == best).int().argmax(0)  # the lowest of equal ones
+    assert torch.equal(r.expert[0, -2000:].long(), first)
+    p = torch.softmax(tail.double(), 0)
+    assert ((r.weight[0, -2000:].double() - p.gather(0, first[None])[0]).abs() <= 2.0 ** -13 * p.max(0).values).all()
+    by_row = torch.sort(r.expert[0], stable=True).indices
+    assert torch.equal(r.column.long(), by_row) and int(r.offset[-1]) == batch
+    d = pb.route_columns_backward(x, r, torch.ones_like(r.weight), normalise="all")
+    chosen = torch.zeros_like(p).scatter_(0, first[None], 1.0)
+    want = p * (chosen - p.max(0).values)
+    # of 1024 terms: (n + 8) units of 2^-22 of the weight, as for the weights; the rounding to 16 bits
+    assert ((d[:, -2000:].double() - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -11 * p + 2.0 ** -25).all()
