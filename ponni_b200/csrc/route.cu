@@ -91,10 +91,16 @@ __device__ __forceinline__ void scan_logits(const T* __restrict__ x, int64_t ld,
       float now = best;
 #pragma unroll
       for (int u = 0; u < kChunk; ++u) now = fmaxf(now, v[u]);
-      sum *= near_best(best, now);
-      best = now;
+      // In pairs, so that a term passes log2(kChunk) roundings and one for every further chunk.
+      float t[kChunk];
 #pragma unroll
-      for (int u = 0; u < kChunk; ++u) sum += near_best(v[u], best);
+      for (int u = 0; u < kChunk; ++u) t[u] = near_best(v[u], now);
+#pragma unroll
+      for (int d = 1; d < kChunk; d *= 2)
+#pragma unroll
+        for (int u = 0; u + d < kChunk; u += 2 * d) t[u] += t[u + d];
+      sum = fmaf(sum, from_best(best, now), t[0]);
+      best = now;
     }
 #pragma unroll
     for (int u = 0; u < kChunk; ++u) {

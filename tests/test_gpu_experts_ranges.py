@@ -564,3 +564,13 @@ def test_routing_past_32_bit_offsets():
     want = p * (chosen - p.max(0).values)
     # of 1024 terms: (n + 8) units of 2^-22 of the weight, as for the weights; the rounding to 16 bits
     assert ((d[:, -2000:].double() - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -11 * p + 2.0 ** -25).all()
+
+
+def test_routing_weights_over_all_in_single_precision():
+    """64 experts: root mean square of the weights' errors.  A rounding is 2^-24 / sqrt 3 = 3.4e-8.  A term of the sum
+    passes 3 in its chunk of 8 and one for every further chunk, 11 with partial sums of a third of the square on average;
+    the chosen expert's exponential (1.5 roundings) and the quotient: sqrt(11 / 3 + 1.5^2 + 1) * 3.4e-8 = 0.9e-7."""
+    x = randn(gen(11), 64, 100_000) * 1.5
+    r = pb.route_columns(x, 4, normalise="all")
+    want = torch.softmax(x.double(), 0).gather(0, r.expert.long())
+    assert ((r.weight.double() - want).norm() / want.norm()).item() <= 1e-7
