@@ -14,8 +14,9 @@
 // words, 16 bytes each where the rows are aligned.  Word w of column c lies in
 // 16-byte chunk (w / 4) ^ (c / 4 mod 16) of the column's 256 bytes: whole chunks
 // for the row side without conflicts, two-way conflicts for the column side.
-// Measured: 2^20 columns of 256 bf16 features to two rows each in 250 us (1.63 GB,
-// 6.5 TB/s, the rate of a plain copy); with one element a thread it was 394.
+// Measured: 2^20 columns of 256 bf16 features to two rows each in 253 us (1.63 GB,
+// 6.4 TB/s, the rate of a plain copy); with one element a thread it was 394.  The
+// combination of the same rows takes 471 us, its gradient 451 (2.7 GB, 6.0 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

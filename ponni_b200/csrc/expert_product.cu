@@ -33,10 +33,10 @@
 // One persistent CTA per SM: a TMA producer, an MMA warp and sixteen epilogue
 // warps.  Every role walks the same tile sequence, which it derives from the
 // offsets (read once into shared memory): no host copy of the group sizes.
-// Measured alone: 32768 rows, 32 experts of 2048 x 2048 bf16 with SiLU in 217 to
+// Measured alone: 32768 rows, 32 experts of 2048 x 2048 bf16 with SiLU in 208 to
 // 232 us (1.2 PFLOP/s; tensor pipe 78% active at the power limit's 1.39 GHz),
-// 2^20 rows, 8 experts of 256 x 256 in 172 us without activation (6.2 TB/s), 212 with
-// SiLU, 384 rows, 64 experts of 1024 x 2048 in 52 to 57 us (4.7 to 5.2 TB/s).
+// 2^20 rows, 8 experts of 256 x 256 in 174 us without activation (6.2 TB/s), 203 to 222 with
+// SiLU, 384 rows, 64 experts of 1024 x 2048 in 53 to 59 us (4.6 to 5.1 TB/s).
 //
 // A few rows for each expert (serving) are bound by the weights' bytes and by
 // latency: few_rows_kernel streams the weights once, without tensor cores.
@@ -334,7 +334,8 @@ __device__ __noinline__ float4 activate4(float4 v, int kind, int flags, float s0
 // values share one reciprocal: 1/a = b (1/ab) (213 us; 219 with two reciprocals,
 // 226 with half of the exponentials by polynomial).  That needs ab finite and keeps no NaN
 // from its neighbour: false, and nothing done, where a value is NaN or below -43 (exponentials
-// up to 2^62.1); such rows take activate_one, as a few rows do.
+// up to 2^62.1); such rows take activate_one, as a few rows do.  (The check costs 2%, 244 us
+// against 240; the same without it by scaled reciprocals takes as long.)
 __device__ __forceinline__ float min_or_nan(float a, float b) {
   float y;
   asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(y) : "f"(a), "f"(b));

@@ -22,8 +22,8 @@ ponni_b200_status fail_cuda(cudaError_t e, const char* what);
 // Status of the launches just made.
 ponni_b200_status launched(const char* what);
 
-// Device address of the current device's operator error word (zero: no error).
-// Allocated once per device, never freed.
+// Device address of the current device's operator error word (zero: no error), a
+// static device variable.
 int* error_word(int device);
 
 int num_sms(int device);

@@ -8,10 +8,11 @@
 //   weight_j = t_{e_j} / sum t,   the sum over the chosen experts or over all.
 // Rows: all (column, choice) pairs sorted by expert, then by column.
 //
-// One pass over the logits with the running maximum and sum; bound by the
-// insertions' instructions, not by the logits' bytes: 131072 columns of 64 fp32
-// logits, four choices, take 18 us to choose (34 MB: 5 us of HBM), 4 to scan
-// the counts, 8.6 to place, their gradient 16 us (67 MB: 10 us).
+// One pass over the logits with the running maximum and sum; the choice is bound by
+// the insertions' instructions, not by the logits' bytes: 131072 columns of 64 fp32
+// logits, four choices, take 18.5 us to choose (34 MB: 5 us of HBM), 4 to scan
+// the counts, 8.5 to place, their gradient 20 us (67 MB: 10 us; 16 with the exponential
+// unit alone in place of expf, or where only chosen experts have a gradient).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
